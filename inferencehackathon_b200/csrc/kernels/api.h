@@ -276,6 +276,75 @@ int ihb_moe_gather_rows(const void* src, const int* order, int k, int row_bytes,
 int ihb_moe_combine_rows(const float* yg, const int* inv, const float* tw, int k, int H, int T, const float* resid, float* y,
                          cudaStream_t stream);
 
+// ---- paged KV cache: append and attention of a ragged batch (paged_append.cu, paged_attn.cu) ---------------------------------
+// Pages k, v [n_pages][nkv][page][128] (bf16, or e4m3 bytes with one fp32 scale per (page, head): a row reads byte * scale).
+// Row r of sequence b lies in page block_table[b][r / page], row r % page of that page. page: 16, 32, 64 or 128.
+// kv_len [B]: rows of each sequence AFTER the call's append (<= 0: a padding entry). cu_q [B + 1]: first token of each
+// sequence in the call (NULL: one token per sequence, T == B); token i of the n of sequence b stands at row kv_len[b] - n + i.
+// Tokens behind cu_q[B] are left alone. Everything that depends on lengths is read on the device: a captured graph replays
+// with other lengths. err (optional): ERR_BAD_ARGS when a page id, a position or a length does not fit; the rows
+// concerned are then skipped (append) or not seen (attention), nothing out of range is touched.
+typedef struct {
+  void* k;
+  void* v;
+  float* k_scale;          // [n_pages][nkv], e4m3 pages only (NULL: bf16 pages)
+  float* v_scale;
+  int n_pages, nkv, page;
+  int B, T;
+  int max_blocks;          // columns of the block table
+  long long table_stride;  // elements between its rows
+  const int* block_table;
+  const int* kv_len;
+  const int* cu_q;
+  unsigned* err;
+} IhbPaged;
+
+// QK RMSNorm (gammas given) + NeoX RoPE + append. qkv: rows of (nq + 2 nkv) * 128 elements, qkv_stride elements apart,
+// fp32 or bf16; q_out: [T][nq][128], q_stride elements between tokens (NULL: the Q part of qkv is rewritten in place).
+// positions (optional) [T]: rotation angle of each token where it is not its row (token trees). cos / sin [n_pos][64].
+// e4m3 pages: scale = least power of two >= amax / 448 over the rows of the page; when a new row needs a larger one the rows
+// already there are brought to it (exact for powers of two, but for e4m3 subnormals). Row 0 starts a page anew.
+typedef struct {
+  IhbPaged c;
+  void* qkv;
+  int qkv_bf16, nq;
+  long long qkv_stride;
+  void* q_out;
+  int q_bf16;
+  long long q_stride;
+  const float* q_gamma;
+  const float* k_gamma;
+  float eps;
+  const float* cos_t;
+  const float* sin_t;
+  int n_pos;
+  const int* positions;
+} IhbPagedAppend;
+int ihb_paged_append(const IhbPagedAppend* a, cudaStream_t stream);
+
+// out[t][h] = softmax(scale * q . K) V over the rows the token sees: its own row and those before it, or with mask
+// [T][mask_stride] (bytes) the rows before the call's and row j of the call's where mask[t][j] != 0. lse (optional) [T][nq]:
+// natural log of the softmax denominator. A token that sees nothing gets zeros (lse -inf). q / out: fp32 or bf16,
+// element strides per token and head. max_q: most tokens any sequence has in the call. scratch: ihb_paged_attention_scratch
+// bytes, not read before it is written (no initialisation).
+typedef struct {
+  IhbPaged c;
+  const void* q;
+  int q_bf16, nq;
+  long long q_stride_t, q_stride_h;
+  void* out;
+  int out_bf16;
+  long long out_stride_t, out_stride_h;
+  float* lse;
+  const unsigned char* mask;
+  long long mask_stride;
+  int max_q;
+  float scale;
+  void* scratch;
+} IhbPagedAttn;
+int ihb_paged_attention(const IhbPagedAttn* a, cudaStream_t stream);
+size_t ihb_paged_attention_scratch(const IhbPagedAttn* a);
+
 // Returns and clears the CUDA runtime's last-error word (a launch refused for its configuration leaves it set; the next
 // entry point that ends in cudaGetLastError would report it as its own).
 int ihb_clear_last_error(void);

@@ -127,6 +127,26 @@ class IhbMegaArgs(C.Structure):
                 ("ar_loopback", C.c_int), ("delay_cta", C.c_int), ("delay_ns", C.c_int), ("comm", IhbComm)]
 
 
+class IhbPaged(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp),
+                ("n_pages", C.c_int), ("nkv", C.c_int), ("page", C.c_int), ("B", C.c_int), ("T", C.c_int),
+                ("max_blocks", C.c_int), ("table_stride", C.c_longlong),
+                ("block_table", _vp), ("kv_len", _vp), ("cu_q", _vp), ("err", _vp)]
+
+
+class IhbPagedAppend(C.Structure):
+    _fields_ = [("c", IhbPaged), ("qkv", _vp), ("qkv_bf16", C.c_int), ("nq", C.c_int), ("qkv_stride", C.c_longlong),
+                ("q_out", _vp), ("q_bf16", C.c_int), ("q_stride", C.c_longlong), ("q_gamma", _vp), ("k_gamma", _vp),
+                ("eps", C.c_float), ("cos_t", _vp), ("sin_t", _vp), ("n_pos", C.c_int), ("positions", _vp)]
+
+
+class IhbPagedAttn(C.Structure):
+    _fields_ = [("c", IhbPaged), ("q", _vp), ("q_bf16", C.c_int), ("nq", C.c_int), ("q_stride_t", C.c_longlong),
+                ("q_stride_h", C.c_longlong), ("out", _vp), ("out_bf16", C.c_int), ("out_stride_t", C.c_longlong),
+                ("out_stride_h", C.c_longlong), ("lse", _vp), ("mask", _vp), ("mask_stride", C.c_longlong),
+                ("max_q", C.c_int), ("scale", C.c_float), ("scratch", _vp)]
+
+
 def load(build_if_missing: bool = True) -> C.CDLL:
     """Load (building first if the sources changed and nvcc is present) the kernel library."""
     global _lib
@@ -201,6 +221,12 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.ihb_allreduce_counted.restype = C.c_int
     lib.ihb_dequant_bf16.argtypes = [_vp, _vp, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp]
     lib.ihb_dequant_bf16.restype = C.c_int
+    lib.ihb_paged_append.argtypes = [C.POINTER(IhbPagedAppend), _vp]
+    lib.ihb_paged_append.restype = C.c_int
+    lib.ihb_paged_attention.argtypes = [C.POINTER(IhbPagedAttn), _vp]
+    lib.ihb_paged_attention.restype = C.c_int
+    lib.ihb_paged_attention_scratch.argtypes = [C.POINTER(IhbPagedAttn)]
+    lib.ihb_paged_attention_scratch.restype = C.c_size_t
     lib.ihb_mega_decode.argtypes = [C.POINTER(IhbMegaArgs), C.c_int, _vp]
     lib.ihb_mega_decode.restype = C.c_int
     lib.ihb_mega_max_grid.argtypes = [C.POINTER(IhbMegaArgs)]

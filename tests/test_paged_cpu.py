@@ -1,0 +1,130 @@
+"""Paged cache operators without a GPU: refusals, argument blocks, and properties of the page scale on the 64-bit oracle."""
+import ctypes as C
+
+import pytest
+import torch
+
+import paged_oracle as O
+from inferencehackathon_b200.ops import lib as K
+from inferencehackathon_b200.ops import paged
+
+
+def _append_args(**over):
+    nq, nkv, P, B = 4, 2, 16, 3
+    cos, sin = O.rope_tables(64)
+    a = dict(qkv=torch.zeros(B, (nq + 2 * nkv) * 128), nq=nq, nkv=nkv, k_pages=torch.zeros(8, nkv, P, 128, dtype=torch.bfloat16),
+             v_pages=torch.zeros(8, nkv, P, 128, dtype=torch.bfloat16), block_table=torch.zeros(B, 2, dtype=torch.int32),
+             kv_len=torch.ones(B, dtype=torch.int32), cos_t=cos, sin_t=sin)
+    a.update(over)
+    return a
+
+
+def _attn_args(**over):
+    B = 3
+    a = dict(q=torch.zeros(B, 4, 128), k_pages=torch.zeros(8, 2, 16, 128, dtype=torch.bfloat16),
+             v_pages=torch.zeros(8, 2, 16, 128, dtype=torch.bfloat16), block_table=torch.zeros(B, 2, dtype=torch.int32),
+             kv_len=torch.ones(B, dtype=torch.int32))
+    a.update(over)
+    return a
+
+
+E4 = torch.float8_e4m3fn
+COMMON = [
+    (dict(k_pages=torch.zeros(8, 2, 24, 128, dtype=torch.bfloat16), v_pages=torch.zeros(8, 2, 24, 128, dtype=torch.bfloat16)), "page size"),
+    (dict(k_pages=torch.zeros(8, 2, 16, 64, dtype=torch.bfloat16), v_pages=torch.zeros(8, 2, 16, 64, dtype=torch.bfloat16)), "pages must be"),
+    (dict(v_pages=torch.zeros(9, 2, 16, 128, dtype=torch.bfloat16)), "alike"),
+    (dict(k_pages=torch.zeros(8, 2, 16, 128), v_pages=torch.zeros(8, 2, 16, 128)), "bfloat16 or float8"),
+    (dict(k_pages=torch.zeros(8, 2, 16, 128, dtype=E4), v_pages=torch.zeros(8, 2, 16, 128, dtype=E4)), "need k_scale"),
+    (dict(k_pages=torch.zeros(8, 2, 16, 128, dtype=E4), v_pages=torch.zeros(8, 2, 16, 128, dtype=E4), k_scale=torch.ones(8, 2),
+          v_scale=torch.ones(8, 3)), "page scales"),
+    (dict(k_scale=torch.ones(8, 2), v_scale=torch.ones(8, 2)), "no scales"),
+    (dict(k_pages=torch.zeros(8, 2, 16, 256, dtype=torch.bfloat16)[..., ::2], v_pages=torch.zeros(8, 2, 16, 128, dtype=torch.bfloat16)),
+     "contiguous"),
+    (dict(kv_len=torch.ones(3, dtype=torch.int64)), "kv_len"),
+    (dict(kv_len=torch.ones(4, dtype=torch.int32), block_table=torch.zeros(4, 2, dtype=torch.int32)), "one token per sequence"),
+    (dict(block_table=torch.zeros(3, 2, dtype=torch.int64)), "block_table"),
+    (dict(block_table=torch.zeros(2, 2, dtype=torch.int32)), "block_table"),
+    (dict(cu_q=torch.zeros(3, dtype=torch.int32)), "cu_q"),
+    (dict(err=torch.zeros(1)), "err"),
+]
+
+
+@pytest.mark.parametrize("over,what", COMMON + [
+    (dict(qkv=torch.zeros(3, 7 * 128)), "qkv must be"),
+    (dict(qkv=torch.zeros(3, 8 * 128, dtype=torch.float16)), "float32 or bfloat16"),
+    (dict(qkv=torch.zeros(1, 8 * 128).expand(3, -1)), "overlap"),
+    (dict(nkv=1, nq=6), "KV heads"),
+    (dict(cos_t=torch.zeros(64, 64, dtype=torch.float64)), "cos_t"),
+    (dict(q_gamma=torch.ones(128)), "come together"),
+    (dict(q_gamma=torch.ones(64), k_gamma=torch.ones(64)), "gammas"),
+    (dict(positions=torch.zeros(3, dtype=torch.int64)), "positions"),
+    (dict(q_out=torch.zeros(3, 5, 128)), "q_out"),
+    (dict(q_out=torch.zeros(3, 4, 256)[..., ::2]), "q_out"),
+    (dict(), "CUDA tensors"),
+])
+def test_append_refuses(over, what):
+    with pytest.raises(ValueError, match=what):
+        paged.paged_append(**_append_args(**over))
+
+
+@pytest.mark.parametrize("over,what", COMMON + [
+    (dict(q=torch.zeros(3, 5, 128)), "evenly"),
+    (dict(q=torch.zeros(3, 4, 64)), "q must be"),
+    (dict(q=torch.zeros(3, 4, 128, dtype=torch.float16)), "float32 or bfloat16"),
+    (dict(q=torch.zeros(3, 4 * 128 + 4)[:, :512].unflatten(1, (4, 128))), "multiples of 8"),
+    (dict(max_q=2), "max_q"),
+    (dict(max_q=0), "max_q"),
+    (dict(scale=0.0), "scale"),
+    (dict(scale=float("nan")), "scale"),
+    (dict(out=torch.zeros(3, 4, 128, dtype=torch.float16)), "out must be"),
+    (dict(out=torch.zeros(1, 4, 128).expand(3, -1, -1)), "overlap"),
+    (dict(lse=torch.zeros(3, 5)), "lse"),
+    (dict(mask=torch.zeros(3, 1)), "mask"),
+    (dict(mask=torch.zeros(2, 1, dtype=torch.bool)), "mask"),
+    (dict(cu_q=torch.zeros(4, dtype=torch.int32), max_q=3, mask=torch.zeros(3, 2, dtype=torch.bool)), "mask"),
+    (dict(), "CUDA tensors"),
+])
+def test_attention_refuses(over, what):
+    with pytest.raises(ValueError, match=what):
+        paged.paged_attention(**_attn_args(**over))
+
+
+def test_c_entries_refuse_bad_blocks():
+    """The C entry points check again, before anything is launched (no GPU needed: nothing is)."""
+    lib = K.load()
+    assert lib.ihb_paged_append(C.byref(K.IhbPagedAppend()), None) != 0
+    a = K.IhbPagedAttn()
+    assert lib.ihb_paged_attention(C.byref(a), None) != 0
+    assert lib.ihb_paged_attention_scratch(C.byref(a)) == 0
+    a.c = K.IhbPaged(k=16, v=16, n_pages=4, nkv=2, page=24, B=1, T=1, max_blocks=1, block_table=16, kv_len=16)
+    a.q, a.out, a.nq, a.max_q, a.scratch = 16, 16, 4, 1, 16
+    assert lib.ihb_paged_attention(C.byref(a), None) != 0                    # page size
+    a.c.page, a.nq = 16, 5
+    assert lib.ihb_paged_attention(C.byref(a), None) != 0                    # heads
+    a.nq, a.c.T = 4, 2
+    assert lib.ihb_paged_attention(C.byref(a), None) != 0                    # two tokens, one sequence, no cu_q
+
+
+def test_a_page_filled_token_by_token_equals_one_filled_at_once():
+    """Power-of-two scales: both ways give the same scale, and the same bytes but for values that become subnormal (then at
+    most one step of 2^-9 apart)."""
+    gen = torch.Generator().manual_seed(3)
+    P, nq, nkv = 16, 2, 2
+    qkv = torch.randn(P, (nq + 2 * nkv) * 128, generator=gen) * torch.exp2(torch.linspace(-6, 6, P))[:, None]
+    cos, sin = O.rope_tables(P)
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    blank = lambda: O.Pages(*(torch.zeros(1, nkv, P, 128) for _ in range(2)), *(torch.ones(1, nkv) for _ in range(2)))  # noqa: E731
+    once, steps = blank(), blank()
+    O.append(once, qkv, nq, nkv, table, [P], [0, P], cos, sin)
+    for t in range(P):
+        O.append(steps, qkv[t:t + 1], nq, nkv, table, [t + 1], [0, 1], cos, sin)
+    assert torch.equal(once.ks, steps.ks) and torch.equal(once.vs, steps.vs)
+    for a, b in ((once.k, steps.k), (once.v, steps.v)):
+        normal = a.abs() >= 2.0 ** -6
+        assert torch.equal(a[normal], b[normal])
+        assert float((a - b).abs().max()) <= 2.0 ** -9
+
+
+def test_oracle_rounding_is_torch_rounding():
+    x = torch.cat([torch.linspace(-448, 448, 40001), torch.linspace(-0.05, 0.05, 40001)])
+    assert torch.equal(O.e4m3_round(x.double()).float(), x.to(torch.float8_e4m3fn).float())
