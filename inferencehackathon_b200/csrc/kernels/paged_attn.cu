@@ -24,6 +24,7 @@ constexpr int PD_WARPS = 4;
 constexpr int PD_UNIT = 64;                  // keys per unit: 16 per warp
 constexpr int PD_REC = PG_HD + 4;            // record of a row: 128 channels, m, l, 2 pad
 constexpr float PD_OFF = 6.f;                // log2 of what a probability is scaled by (fp16 keeps more small ones)
+constexpr float PD_NONE = 1e30f;             // OFF - running maximum before the first key
 constexpr float PD_LAZY = 8.f;               // the running maximum may be passed by 2^8 before the accumulators are rescaled
 
 template <bool F16>
@@ -55,21 +56,8 @@ __device__ __forceinline__ float2 pd_unpack(unsigned v) {
   if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
   else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
-// (x, y) -> packed heads and packed remainders
-template <bool F16>
-__device__ __forceinline__ void pd_split(float x, float y, unsigned& hi, unsigned& lo) {
-  hi = pd_pack<F16>(x, y);
-  const float2 h = pd_unpack<F16>(hi);
-  lo = pd_pack<F16>(x - h.x, y - h.y);
-}
-__device__ __forceinline__ unsigned pd_cvt(unsigned pair) {     // two e4m3 bytes -> two fp16
-  const __half2 h = cvt_e4m3x2(static_cast<unsigned short>(pair));
-  return *reinterpret_cast<const unsigned*>(&h);
-}
-__device__ __forceinline__ uint4 pd_ldg(const void* p) {        // cache rows are read once: no L1 allocation
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+__device__ __forceinline__ void pd_cvt4(unsigned w, unsigned& lo, unsigned& hi) {     // four e4m3 bytes -> two pairs of fp16
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 __device__ __forceinline__ float pd_ex2(float x) {
   float y;
@@ -78,20 +66,30 @@ __device__ __forceinline__ float pd_ex2(float x) {
 }
 __device__ __forceinline__ unsigned pd_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// A page scale as a power of two's exponent, inside the range that append writes (a scale of 0 reads as the least one).
-__device__ __forceinline__ float pd_log2_scale(float s) { return log2f(fminf(fmaxf(s, 8.673617379884035e-19f), 1.152921504606847e18f)); }
+// log2 of a page scale inside the range that append writes (a scale of 0 reads as the least one): the exponent from the bits, exact
+// for powers of two, and the logarithm of the mantissa for other scales (lg2.approx on [1, 2): within 2^-22).
+__device__ __forceinline__ float pd_log2_scale(float s) {
+  const unsigned u = __float_as_uint(fminf(fmaxf(s, 8.673617379884035e-19f), 1.152921504606847e18f));
+  float f;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(__uint_as_float((u & 0x7fffffu) | 0x3f800000u)));
+  return static_cast<float>(static_cast<int>(u >> 23) - 127) + f;
+}
 
 // ---- work items ------------------------------------------------------------------------------------------------------------
+// An item costs its units and PD_START more (loading Q, filling the ring, adding the warps up): ranges are cut on that cost, so a CTA
+// with many short items gets fewer keys. Positions inside an item: [0, PD_START) start-up, then the units.
+constexpr int PD_START = 3;
+
 struct PdWork {
   int tiles, units, items;       // of one sequence: row tiles, units per item, items = nkv * tiles
-  long long total;               // items * units
+  long long total;               // cost: items * (units + PD_START)
 };
 __device__ __forceinline__ PdWork pd_work(const IhbPaged& c, const PgSeq& s, int G, int RT) {
   PdWork w;
   w.tiles = (s.n * G + RT - 1) / RT;
   w.units = s.n > 0 ? (s.len + PD_UNIT - 1) / PD_UNIT : 0;
   w.items = w.units > 0 ? w.tiles * c.nkv : 0;
-  w.total = static_cast<long long>(w.items) * w.units;
+  w.total = static_cast<long long>(w.items) * (w.units + PD_START);
   return w;
 }
 __device__ __forceinline__ long long warp_incl_scan_ll(long long v, int lane) {
@@ -102,7 +100,7 @@ __device__ __forceinline__ long long warp_incl_scan_ll(long long v, int lane) {
   }
   return v;
 }
-// Units of the whole batch (whole warp).
+// Cost of the whole batch (whole warp).
 __device__ __forceinline__ long long pd_total(const IhbPaged& c, int G, int RT, int lane) {
   long long sum = 0;
   for (int b = lane; b < c.B; b += 32) sum += pd_work(c, pg_seq(c, b), G, RT).total;
@@ -110,7 +108,7 @@ __device__ __forceinline__ long long pd_total(const IhbPaged& c, int G, int RT, 
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
-// The sequence that holds unit u (whole warp, u < total); `before`: units ahead of it.
+// The sequence that holds position u (whole warp, u < total); `before`: cost ahead of it.
 __device__ __forceinline__ int pd_find(const IhbPaged& c, int G, int RT, int lane, long long u, long long& before) {
   long long at = 0;
   for (int b0 = 0; b0 < c.B; b0 += 32) {
@@ -128,7 +126,7 @@ __device__ __forceinline__ int pd_find(const IhbPaged& c, int G, int RT, int lan
   before = at;
   return c.B;
 }
-// Ranges: CTA i of `parts` takes units [i * total / parts, (i + 1) * total / parts).
+// Ranges: CTA i of `parts` takes positions [i * total / parts, (i + 1) * total / parts).
 __device__ __forceinline__ int pd_parts(long long total, int grid) { return static_cast<int>(total < grid ? total : grid); }
 __device__ __forceinline__ long long pd_cut(long long total, int parts, int i) { return total * i / parts; }
 
@@ -136,6 +134,11 @@ __device__ __forceinline__ void pd_store(const IhbPagedAttn& a, int t, int h, in
   const size_t o = static_cast<size_t>(t) * a.out_stride_t + static_cast<size_t>(h) * a.out_stride_h + ch;
   if (a.out_bf16) reinterpret_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16(v);
   else reinterpret_cast<float*>(a.out)[o] = v;
+}
+__device__ __forceinline__ void pd_store4(const IhbPagedAttn& a, int t, int h, int ch, float4 v) {
+  const size_t o = static_cast<size_t>(t) * a.out_stride_t + static_cast<size_t>(h) * a.out_stride_h + ch;
+  if (a.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o) = make_uint2(pd_pack<false>(v.x, v.y), pd_pack<false>(v.z, v.w));
+  else *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o) = v;
 }
 // (m, l) of a finished row -> natural log of its denominator
 template <bool KV8>
@@ -151,22 +154,52 @@ __device__ __forceinline__ bool pd_sees(const IhbPagedAttn& a, const PgSeq& s, i
   return j < 0 || (j < a.mask_stride && a.mask[static_cast<size_t>(s.t0 + i) * a.mask_stride + j] != 0);
 }
 
-template <int NT, bool KV8, bool QF32>
-__global__ void __launch_bounds__(PD_WARPS * 32, NT == 1 ? 4 : (QF32 ? 2 : 3)) paged_rows_kernel(const __grid_constant__ IhbPagedAttn a, int grid) {
-  constexpr int RT = 8 * NT;
-  constexpr bool PSPLIT = QF32 || !KV8;      // probabilities as head + remainder: fp32 results, and bf16 would round them by 2^-9
-  constexpr int KW = KV8 ? 2 : 4;            // 16-byte loads per key of a thread's 32 channels
-  __shared__ __align__(16) float o_s[PD_WARPS][RT][PG_HD + 4];
-  __shared__ float m_s[PD_WARPS][RT], l_s[PD_WARPS][RT];
+// Shared memory of a CTA: ST key steps per warp in flight (16 rows of K, 16 of V, the page's scales), the Q fragments of the row
+// tile; the four warps' results take the place of the steps at the end of an item.
+template <int NT, bool KV8, int QT>
+struct PdSmem {
+  static constexpr int ROWB = KV8 ? PG_HD : 2 * PG_HD;
+  static constexpr int STEP = 2 * 16 * ROWB + 16;
+  static constexpr int PER_SM = KV8 ? 4 : (NT == 2 && QT > 1 ? 2 : 3);          // CTAs per SM that ring and registers leave room for
+  static constexpr int ST = KV8 || PER_SM == 2 ? 3 : 2;
+  static constexpr int QB = QT * NT * 8 * 32 * 8;
+  static constexpr int STEPS = PD_WARPS * ST * STEP, OUT = PD_WARPS * 8 * NT * (PG_HD + 4) * 4;
+  static constexpr int BYTES = QB + (STEPS > OUT ? STEPS : OUT);
+};
+
+__device__ __forceinline__ void pd_cp16(uint32_t dst, const void* src, bool ok) {       // zeros when !ok: src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pd_cp4(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void pd_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void pd_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// 16-byte chunk `ch` of row r: the chunks that the eight lanes of one shared-memory phase read lie in different banks
+__device__ __forceinline__ int pd_kswz(int r, int ch) { return ch ^ ((r & 1) << 2); }
+__device__ __forceinline__ int pd_vswz(int r, int ch) { return ch ^ (((r >> 1) & 3) << 1); }
+
+// QT / PT: 16-bit terms that a query element / a probability is split into.
+template <int NT, bool KV8, int QT, int PT>
+__global__ void __launch_bounds__(PD_WARPS * 32, PdSmem<NT, KV8, QT>::PER_SM) paged_rows_kernel(const __grid_constant__ IhbPagedAttn a, int grid) {
+  using SM = PdSmem<NT, KV8, QT>;
+  constexpr int RT = 8 * NT, ST = SM::ST, ROWB = SM::ROWB;
+  extern __shared__ __align__(128) unsigned char pd_sm[];
+  __shared__ float m_s[PD_WARPS][RT], l_s[PD_WARPS][RT], rowf_s[RT];
+  uint2* qf = reinterpret_cast<uint2*>(pd_sm);                                   // [QT][NT][8][32]
+  float (*o_s)[RT][PG_HD + 4] = reinterpret_cast<float (*)[RT][PG_HD + 4]>(pd_sm + SM::QB);
   const IhbPaged& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
   const int G = a.nq / c.nkv;
+  unsigned char* ring = pd_sm + SM::QB + warp * ST * SM::STEP;
   pdl_launch_dependents();                   // the folding kernel waits for this one's end; it may be scheduled from here on
 
   // entries without a cached row: zeros
   for (int b = blockIdx.x; b < c.B; b += grid) {
     const PgSeq s = pg_seq(c, b);
+    if (s.n > a.max_q && tid == 0) set_error(c.err, ERR_BAD_ARGS);      // more tokens than the caller planned for
     if (s.len > 0 || s.n == 0) continue;
     for (int i = 0; i < s.n; ++i)
       for (int h = 0; h < a.nq; ++h) pd_store(a, s.t0 + i, h, tid, 0.f);
@@ -184,7 +217,6 @@ __global__ void __launch_bounds__(PD_WARPS * 32, NT == 1 ? 4 : (QF32 ? 2 : 3)) p
   PgSeq s = pg_seq(c, b);
   PdWork w = pd_work(c, s, G, RT);
   const int psh = __ffs(c.page) - 1;
-  const float sm = a.scale * PG_LOG2E;
 
   while (u < u_end) {
     while (u - before >= w.total) {           // next sequence with work
@@ -193,17 +225,60 @@ __global__ void __launch_bounds__(PD_WARPS * 32, NT == 1 ? 4 : (QF32 ? 2 : 3)) p
       s = pg_seq(c, b);
       w = pd_work(c, s, G, RT);
     }
-    const int item = static_cast<int>((u - before) / w.units), unit0 = static_cast<int>((u - before) % w.units);
-    const int n_units = static_cast<int>(min(static_cast<long long>(w.units - unit0), u_end - u));
+    const int span = w.units + PD_START, item = static_cast<int>((u - before) / span), at = static_cast<int>((u - before) % span);
+    const int taken = static_cast<int>(min(static_cast<long long>(span - at), u_end - u));
+    const int unit0 = max(at - PD_START, 0), n_units = at + taken - PD_START - unit0;
+    if (n_units <= 0) {                       // only start-up cost of the item lies in this range
+      u += taken;
+      continue;
+    }
     const int kvh = item / w.tiles, row0 = (item % w.tiles) * RT;
     const int* table = c.block_table + static_cast<size_t>(b) * c.table_stride;
 
-    // ---- Q^T fragments: row g of each group of 8, the channels that this thread takes of every key ----
-    unsigned qh[NT][8][2], ql[QF32 ? NT : 1][8][2];
-    float rowf[NT][2];                        // what a score of rows 2 t4, 2 t4 + 1 is multiplied by
+    // keys that any row of the tile sees lie below key_end; below key_all every row sees them
+    const int i_last = min((row0 + RT - 1) / G, s.n - 1);
+    const int seen_end = a.mask != nullptr ? s.len : min(s.len, s.base + i_last + 1);
+    const int key_end = min(seen_end, (unit0 + n_units) * PD_UNIT);
+    const int key_all = min(s.len, a.mask != nullptr ? s.base : s.base + row0 / G + 1);
+
+    auto page_of = [&](int key) -> int { return key < key_end ? table[key >> psh] : -1; };
+    // lane's first chunk in the pages' rows: chunk `lane`, then every 32nd (two or four rows on)
+    constexpr int CPR = ROWB / 16;            // chunks per row
+    const int lr = lane / CPR, lc = lane % CPR;
+    const size_t in_page = static_cast<size_t>(kvh) * c.page * ROWB + lane * 16;
+    const char* k0 = reinterpret_cast<const char*>(c.k) + in_page;
+    const char* v0 = reinterpret_cast<const char*>(c.v) + in_page;
+    const unsigned page_bytes = static_cast<unsigned>(c.nkv * c.page) * ROWB;
+    auto issue = [&](int key, int page, int slot) {       // the 16 keys from `key` on into one step of the ring
+      const bool ok = key < key_end && static_cast<unsigned>(page) < static_cast<unsigned>(c.n_pages);
+      const unsigned pg = ok ? page : 0;
+      const size_t off = static_cast<size_t>(pg) * page_bytes + (ok ? (key & (c.page - 1)) * ROWB : 0);
+      unsigned char* st = ring + slot * SM::STEP;
+      const uint32_t kd = smem_u32(st), vd = kd + 16 * ROWB;
+      const bool all = key + 16 <= s.len;     // rows behind the sequence may hold anything, and 0 * NaN is NaN: zeros instead
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + nt * 8 + g, i = r / G;
+      for (int i = 0; i < ROWB / 32; ++i) {
+        const int r = lr + i * (32 / CPR);
+        pd_cp16(kd + r * ROWB + pd_kswz(r, lc) * 16, k0 + off + i * 512, ok);
+        pd_cp16(vd + r * ROWB + pd_vswz(r, lc) * 16, v0 + off + i * 512, ok && (all || key + r < s.len));
+      }
+      if (KV8 && lane < 2) pd_cp4(kd + 32 * ROWB + lane * 4, (lane ? c.v_scale : c.k_scale) + static_cast<size_t>(pg) * c.nkv + kvh, ok);
+      if (lane == 2) *reinterpret_cast<int*>(st + 32 * ROWB + 8) = ok || key >= key_end;
+    };
+
+    int key = unit0 * PD_UNIT + warp * 16;
+    int page_next = page_of(key);
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) {
+      const int page = page_next;
+      page_next = page_of(key + (i + 1) * PD_UNIT);
+      issue(key + i * PD_UNIT, page, i);
+      pd_commit();
+    }
+
+    // ---- Q^T fragments, one group of 8 rows per warp: row g, the channels that lane t4 takes of every key ----
+    if (warp < NT) {
+      const int r = row0 + warp * 8 + g, i = r / G;
       const bool ok = i < s.n;
       const size_t off = ok ? static_cast<size_t>(s.t0 + i) * a.q_stride_t + static_cast<size_t>(kvh * G + r % G) * a.q_stride_h : 0;
       float x[32];
@@ -238,116 +313,100 @@ __global__ void __launch_bounds__(PD_WARPS * 32, NT == 1 ? 4 : (QF32 ? 2 : 3)) p
 #pragma unroll
         for (int j = 0; j < 32; ++j) x[j] *= inv;
       }
+      if (t4 == 0) rowf_s[warp * 8 + g] = a.scale * PG_LOG2E * f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
+      for (int t = 0; t < QT; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if constexpr (QF32) pd_split<KV8>(x[4 * k + 2 * h], x[4 * k + 2 * h + 1], qh[nt][k][h], ql[nt][k][h]);
-          else qh[nt][k][h] = pd_pack<KV8>(x[4 * k + 2 * h], x[4 * k + 2 * h + 1]);
+        for (int k = 0; k < 8; ++k) {
+          unsigned q2[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float& y0 = x[4 * k + 2 * h];
+            float& y1 = x[4 * k + 2 * h + 1];
+            q2[h] = pd_pack<KV8>(y0, y1);
+            const float2 v = pd_unpack<KV8>(q2[h]);
+            y0 -= v.x;
+            y1 -= v.y;
+          }
+          qf[((t * NT + warp) * 8 + k) * 32 + lane] = make_uint2(q2[0], q2[1]);
         }
-      rowf[nt][0] = sm * __shfl_sync(0xffffffffu, f, (2 * t4) * 4);
-      rowf[nt][1] = sm * __shfl_sync(0xffffffffu, f, (2 * t4 + 1) * 4);
     }
+    __syncthreads();
 
     float o[NT][8][4];
-    float m[NT][2], l[NT][2];
+    constexpr float OFF = KV8 ? PD_OFF : 0.f;
+    float mo[NT][2], l[NT][2], rowf[NT][2];   // mo: OFF - running maximum
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        mo[nt][r] = PD_NONE;
+        l[nt][r] = 0.f;
+        rowf[nt][r] = rowf_s[nt * 8 + 2 * t4 + r];
+      }
     }
-    // keys that any row of the tile sees lie below key_end; below key_all every row sees them
-    const int i_last = min((row0 + RT - 1) / G, s.n - 1);
-    const int seen_end = a.mask != nullptr ? s.len : min(s.len, s.base + i_last + 1);
-    const int key_end = min(seen_end, (unit0 + n_units) * PD_UNIT);
-    const int key_all = min(s.len, a.mask != nullptr ? s.base : s.base + row0 / G + 1);
 
-    uint4 kr[2][KW], vr[4][KV8 ? 1 : 2];
-    float ksc = 1.f, vsc = 1.f, ksn = 1.f, vsn = 1.f;
-    int pg_next;                              // page of the step after the one whose rows are being loaded
-    auto page_of = [&](int key) -> int {
-      if (key >= key_end) return -2;
-      const int p = table[key >> psh];
-      return p;
-    };
-    auto load_k = [&](int key, int page) {
-      const bool ok = key < key_end && page >= 0 && page < c.n_pages;
-      const size_t hr = (static_cast<size_t>(ok ? page : 0) * c.nkv + kvh) * c.page + (ok ? (key & (c.page - 1)) : 0);
-      const char* base = reinterpret_cast<const char*>(c.k) + hr * (KV8 ? PG_HD : 2 * PG_HD);
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < KW; ++j)
-          kr[h][j] = ok ? pd_ldg(base + (g + 8 * h) * (KV8 ? PG_HD : 2 * PG_HD) + j * 64 + t4 * 16) : make_uint4(0, 0, 0, 0);
-      if constexpr (KV8) {
-        const size_t si = static_cast<size_t>(ok ? page : 0) * c.nkv + kvh;
-        ksn = ok ? c.k_scale[si] : 0.f;
-        vsn = ok ? c.v_scale[si] : 0.f;
-      }
-    };
-    auto load_v = [&](int key, int page) {
-      const bool ok = key < key_end && page >= 0 && page < c.n_pages;
-      const size_t hr = (static_cast<size_t>(ok ? page : 0) * c.nkv + kvh) * c.page + (ok ? (key & (c.page - 1)) : 0);
-      const char* base = reinterpret_cast<const char*>(c.v) + hr * (KV8 ? PG_HD : 2 * PG_HD);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int kk = 2 * t4 + (i & 1) + 8 * (i >> 1);
-        const bool in = ok && key + kk < s.len;   // rows behind the sequence may hold anything: 0 * NaN is NaN
-#pragma unroll
-        for (int j = 0; j < (KV8 ? 1 : 2); ++j)
-          vr[i][j] = in ? pd_ldg(base + kk * (KV8 ? PG_HD : 2 * PG_HD) + j * 128 + g * 16) : make_uint4(0, 0, 0, 0);
-      }
-    };
-
-    int key = unit0 * PD_UNIT + warp * 16;
-    int page = page_of(key);
-    load_k(key, page);
-    load_v(key, page);
-    pg_next = page_of(key + PD_UNIT);
+    int slot = 0;
     for (; key < key_end; key += PD_UNIT) {
-      const bool bad_page = page < 0 || page >= c.n_pages;
+      pd_wait<ST - 2>();                      // this step's copies have landed (those of the lane; the others' after the barrier)
+      __syncwarp();
+      {
+        const int page = page_next, nslot = slot == 0 ? ST - 1 : slot - 1;       // the step that was read last
+        page_next = page_of(key + ST * PD_UNIT);
+        issue(key + (ST - 1) * PD_UNIT, page, nslot);
+        pd_commit();
+      }
+      const unsigned char* st = ring + slot * SM::STEP;
+      slot = slot == ST - 1 ? 0 : slot + 1;
+      const float2 sc = *reinterpret_cast<const float2*>(st + 32 * ROWB);
+      const bool bad_page = *reinterpret_cast<const int*>(st + 32 * ROWB + 8) == 0;
       if (bad_page && lane == 0) set_error(c.err, ERR_BAD_ARGS);
-      ksc = ksn;
-      vsc = vsn;
       // ---- S^T: 16 keys x RT rows ----
       float d[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) d[nt][0] = d[nt][1] = d[nt][2] = d[nt][3] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        unsigned af[4];
-        if constexpr (KV8) {
-          const unsigned w0 = pd_word(kr[0][k >> 2], k & 3), w1 = pd_word(kr[1][k >> 2], k & 3);
-          af[0] = pd_cvt(w0 & 0xffffu); af[1] = pd_cvt(w1 & 0xffffu);
-          af[2] = pd_cvt(w0 >> 16);     af[3] = pd_cvt(w1 >> 16);
-        } else {
-          af[0] = pd_word(kr[0][k >> 1], (k & 1) * 2);     af[1] = pd_word(kr[1][k >> 1], (k & 1) * 2);
-          af[2] = pd_word(kr[0][k >> 1], (k & 1) * 2 + 1); af[3] = pd_word(kr[1][k >> 1], (k & 1) * 2 + 1);
-        }
+      for (int k4 = 0; k4 < ROWB / 64; ++k4) {      // one 16-byte chunk of keys g and g + 8
+        const uint4 x0 = *reinterpret_cast<const uint4*>(st + g * ROWB + pd_kswz(g, k4 * 4 + t4) * 16);
+        const uint4 x1 = *reinterpret_cast<const uint4*>(st + (g + 8) * ROWB + pd_kswz(g + 8, k4 * 4 + t4) * 16);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          pd_mma<KV8>(d[nt], af, qh[nt][k][0], qh[nt][k][1]);
-          if constexpr (QF32) pd_mma<KV8>(d[nt], af, ql[nt][k][0], ql[nt][k][1]);
+        for (int kk = 0; kk < (KV8 ? 4 : 2); ++kk) {
+          const int k = k4 * (KV8 ? 4 : 2) + kk;
+          unsigned af[4];
+          if constexpr (KV8) {
+            pd_cvt4(pd_word(x0, kk), af[0], af[2]);
+            pd_cvt4(pd_word(x1, kk), af[1], af[3]);
+          } else {
+            af[0] = pd_word(x0, 2 * kk);     af[1] = pd_word(x1, 2 * kk);
+            af[2] = pd_word(x0, 2 * kk + 1); af[3] = pd_word(x1, 2 * kk + 1);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+              const uint2 q2 = qf[((t * NT + nt) * 8 + k) * 32 + lane];
+              pd_mma<KV8>(d[nt], af, q2.x, q2.y);
+            }
         }
       }
-      const int page_now = pg_next;
-      load_k(key + PD_UNIT, page_now);        // the next step's K while this step's softmax and V product run
-      pg_next = page_of(key + 2 * PD_UNIT);
       // ---- softmax: rows 2 t4, 2 t4 + 1, keys g, g + 8 ----
-      const float ev = KV8 ? pd_log2_scale(vsc) : 0.f;
+      const float ev = KV8 ? pd_log2_scale(sc.y) : 0.f;
       const bool edge = bad_page || key + 16 > key_all;
       bool grow = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        const float f0 = KV8 ? rowf[nt][0] * sc.x : rowf[nt][0], f1 = KV8 ? rowf[nt][1] * sc.x : rowf[nt][1];
+        d[nt][0] = fmaf(d[nt][0], f0, ev);
+        d[nt][1] = fmaf(d[nt][1], f1, ev);
+        d[nt][2] = fmaf(d[nt][2], f0, ev);
+        d[nt][3] = fmaf(d[nt][3], f1, ev);
+        if (edge)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float f = KV8 ? rowf[nt][j & 1] * ksc : rowf[nt][j & 1];
-          d[nt][j] = fmaf(d[nt][j], f, ev);
-          if (edge && (bad_page || !pd_sees(a, s, (row0 + nt * 8 + 2 * t4 + (j & 1)) / G, key + g + 8 * (j >> 1)))) d[nt][j] = -INFINITY;
-        }
-        grow |= fmaxf(d[nt][0], d[nt][2]) > m[nt][0] + PD_LAZY || fmaxf(d[nt][1], d[nt][3]) > m[nt][1] + PD_LAZY;
+          for (int j = 0; j < 4; ++j)
+            if (bad_page || !pd_sees(a, s, (row0 + nt * 8 + 2 * t4 + (j & 1)) / G, key + g + 8 * (j >> 1))) d[nt][j] = -INFINITY;
+        grow |= fmaxf(d[nt][0], d[nt][2]) + mo[nt][0] > PD_LAZY + OFF || fmaxf(d[nt][1], d[nt][3]) + mo[nt][1] > PD_LAZY + OFF;
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -358,62 +417,66 @@ __global__ void __launch_bounds__(PD_WARPS * 32, NT == 1 ? 4 : (QF32 ? 2 : 3)) p
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float mn = fmaxf(m[nt][r], mx);
-            const float f = m[nt][r] == -INFINITY ? 0.f : pd_ex2(m[nt][r] - mn);
-            m[nt][r] = mn;
+            if (mx == -INFINITY) continue;
+            const float was = mo[nt][r];
+            mo[nt][r] = fminf(was, OFF - mx);
+            const float f = was == PD_NONE ? 0.f : pd_ex2(mo[nt][r] - was);
             l[nt][r] *= f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) { o[nt][j][r] *= f; o[nt][j][r + 2] *= f; }
           }
       }
       const float lf = KV8 ? pd_ex2(-ev) : 1.f;
-      unsigned ph[NT][2], pl[PSPLIT ? NT : 1][2];
+      unsigned ph[NT][PT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float p[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float mr = m[nt][j & 1] == -INFINITY ? 0.f : m[nt][j & 1];     // nothing seen yet: every score is -inf (or NaN)
-          p[j] = pd_ex2(d[nt][j] - mr + (KV8 ? PD_OFF : 0.f));
+          p[j] = pd_ex2(d[nt][j] + mo[nt][j & 1]);      // nothing seen yet: every score is -inf (or NaN), and so is the sum
         }
         l[nt][0] += (p[0] + p[2]) * lf;
         l[nt][1] += (p[1] + p[3]) * lf;
-        if constexpr (PSPLIT) {
-          unsigned h0, h1, r0, r1;
-          pd_split<KV8>(p[0], p[1], h0, r0);
-          pd_split<KV8>(p[2], p[3], h1, r1);
-          ph[nt][0] = pd_movt(h0); ph[nt][1] = pd_movt(h1);
-          pl[nt][0] = pd_movt(r0); pl[nt][1] = pd_movt(r1);
-        } else {
-          ph[nt][0] = pd_movt(pd_pack<KV8>(p[0], p[1]));
-          ph[nt][1] = pd_movt(pd_pack<KV8>(p[2], p[3]));
-        }
+#pragma unroll
+        for (int t = 0; t < PT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned x = pd_pack<KV8>(p[2 * h], p[2 * h + 1]);
+            ph[nt][t][h] = pd_movt(x);
+            if (t + 1 < PT) {
+              const float2 v = pd_unpack<KV8>(x);
+              p[2 * h] -= v.x;
+              p[2 * h + 1] -= v.y;
+            }
+          }
       }
-      // ---- a value that is not finite in a row that not every query sees: those who see it get it, the others nothing ----
-      if (key + 16 > key_all && key < seen_end) {
-        bool odd = false;
+      // ---- V rows 2 t4, 2 t4 + 1, + 8, + 9: 16 channels ----
+      const unsigned char* vst = st + 16 * ROWB;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+      for (int jv = 0; jv < (KV8 ? 1 : 2); ++jv) {
+        uint4 vr[4];
 #pragma unroll
-          for (int j = 0; j < (KV8 ? 1 : 2); ++j)
+        for (int i = 0; i < 4; ++i) {
+          const int r = 2 * t4 + (i & 1) + 8 * (i >> 1);
+          vr[i] = *reinterpret_cast<const uint4*>(vst + r * ROWB + pd_vswz(r, jv * 8 + g) * 16);
+        }
+        // a value that is not finite in a row that not every query sees: those who see it get it, the others nothing
+        if (key + 16 > key_all) {
+          bool odd = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const unsigned x = pd_word(vr[i][j], q);
+              const unsigned x = pd_word(vr[i], q);
               if constexpr (KV8) odd |= ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u);
               else odd |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
             }
-        if (__any_sync(0xffffffffu, odd)) {
-          for (int kk = 0; kk < 16; ++kk) {
-            const int src = (lane & ~3) | ((kk & 7) >> 1), i = (kk & 1) + 2 * (kk >> 3);
-#pragma unroll
-            for (int j = 0; j < (KV8 ? 1 : 2); ++j)
+          if (__any_sync(0xffffffffu, odd)) {
+            for (int kk = 0; kk < 16; ++kk) {
+              const unsigned* xr = reinterpret_cast<const unsigned*>(vst + kk * ROWB + pd_vswz(kk, jv * 8 + g) * 16);
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                unsigned mine = 0;
-#pragma unroll
-                for (int ii = 0; ii < 4; ++ii)
-                  if (ii == i) mine = pd_word(vr[ii][j], q);
-                const unsigned x = __shfl_sync(0xffffffffu, mine, src);
+                const unsigned x = xr[q];
                 float v[4];
                 if constexpr (KV8) {
                   const float4 f = e4m3x4_to_float4(x);
@@ -428,23 +491,14 @@ __global__ void __launch_bounds__(PD_WARPS * 32, NT == 1 ? 4 : (QF32 ? 2 : 3)) p
                   for (int r = 0; r < 2; ++r) {
                     if (!pd_sees(a, s, (row0 + nt * 8 + 2 * t4 + r) / G, key + kk)) continue;
 #pragma unroll
-                    for (int e = 0; e < (KV8 ? 4 : 2); ++e) {
-                      if (fabsf(v[e]) <= 3.4028235e38f) continue;     // finite
-                      constexpr int M2 = KV8 ? 2 : 1;
-                      const int mt = KV8 ? q * M2 + (e >> 1) : j * 4 + q;
-#pragma unroll
-                      for (int jj = 0; jj < 8; ++jj)
-                        if (jj == mt) o[nt][jj][r + 2 * (e & 1)] += v[e];
-                    }
+                    for (int e = 0; e < (KV8 ? 4 : 2); ++e)
+                      if (!(fabsf(v[e]) <= 3.4028235e38f)) o[nt][KV8 ? 2 * q + (e >> 1) : jv * 4 + q][r + 2 * (e & 1)] += v[e];
                   }
               }
-          }
-          // and out of the product
+            }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < (KV8 ? 1 : 2); ++j) {
-              unsigned x[4] = {vr[i][j].x, vr[i][j].y, vr[i][j].z, vr[i][j].w};
+            for (int i = 0; i < 4; ++i) {     // and out of the product
+              unsigned x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 if constexpr (KV8) {
@@ -456,35 +510,33 @@ __global__ void __launch_bounds__(PD_WARPS * 32, NT == 1 ? 4 : (QF32 ? 2 : 3)) p
                   if ((x[q] & 0x7f800000u) == 0x7f800000u) x[q] &= 0x0000ffffu;
                 }
               }
-              vr[i][j] = make_uint4(x[0], x[1], x[2], x[3]);
+              vr[i] = make_uint4(x[0], x[1], x[2], x[3]);
             }
+          }
+        }
+        // ---- O^T += V^T P^T: tiles of 16 channels ----
+#pragma unroll
+        for (int jj = 0; jj < (KV8 ? 8 : 4); ++jj) {
+          const int j = KV8 ? jj : jv * 4 + jj;
+          unsigned af[4];
+          if constexpr (KV8) {
+            const unsigned sel = (jj & 1) ? 0x7362u : 0x5140u;
+            pd_cvt4(__byte_perm(pd_word(vr[0], jj >> 1), pd_word(vr[1], jj >> 1), sel), af[0], af[1]);
+            pd_cvt4(__byte_perm(pd_word(vr[2], jj >> 1), pd_word(vr[3], jj >> 1), sel), af[2], af[3]);
+          } else {
+            const unsigned w0 = pd_word(vr[0], jj), w1 = pd_word(vr[1], jj), w2 = pd_word(vr[2], jj), w3 = pd_word(vr[3], jj);
+            af[0] = __byte_perm(w0, w1, 0x5410); af[1] = __byte_perm(w0, w1, 0x7632);
+            af[2] = __byte_perm(w2, w3, 0x5410); af[3] = __byte_perm(w2, w3, 0x7632);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int t = 0; t < PT; ++t) pd_mma<KV8>(o[nt][j], af, ph[nt][t][0], ph[nt][t][1]);
         }
       }
-      // ---- O^T += V^T P^T: 8 tiles of 16 channels ----
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        unsigned af[4];
-        if constexpr (KV8) {
-          const unsigned sel = (j & 1) ? 0x7362u : 0x5140u;
-          const unsigned x = __byte_perm(pd_word(vr[0][0], j >> 1), pd_word(vr[1][0], j >> 1), sel);
-          const unsigned y = __byte_perm(pd_word(vr[2][0], j >> 1), pd_word(vr[3][0], j >> 1), sel);
-          af[0] = pd_cvt(x & 0xffffu); af[1] = pd_cvt(x >> 16);
-          af[2] = pd_cvt(y & 0xffffu); af[3] = pd_cvt(y >> 16);
-        } else {
-          const unsigned w0 = pd_word(vr[0][j >> 2], j & 3), w1 = pd_word(vr[1][j >> 2], j & 3);
-          const unsigned w2 = pd_word(vr[2][j >> 2], j & 3), w3 = pd_word(vr[3][j >> 2], j & 3);
-          af[0] = __byte_perm(w0, w1, 0x5410); af[1] = __byte_perm(w0, w1, 0x7632);
-          af[2] = __byte_perm(w2, w3, 0x5410); af[3] = __byte_perm(w2, w3, 0x7632);
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          pd_mma<KV8>(o[nt][j], af, ph[nt][0], ph[nt][1]);
-          if constexpr (PSPLIT) pd_mma<KV8>(o[nt][j], af, pl[nt][0], pl[nt][1]);
-        }
-      }
-      load_v(key + PD_UNIT, page_now);
-      page = page_now;
     }
+    pd_wait<0>();
+    __syncthreads();                           // every warp is done with its steps: their place takes the results
 
     // ---- the four warps' results ----
 #pragma unroll
@@ -496,7 +548,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32, NT == 1 ? 4 : (QF32 ? 2 : 3)) p
         t += __shfl_xor_sync(0xffffffffu, t, 8);
         t += __shfl_xor_sync(0xffffffffu, t, 16);
         const int row = nt * 8 + 2 * t4 + r;
-        if (g == 0) { m_s[warp][row] = m[nt][r]; l_s[warp][row] = t; }
+        if (g == 0) { m_s[warp][row] = mo[nt][r] == PD_NONE ? -INFINITY : OFF - mo[nt][r]; l_s[warp][row] = t; }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int ch = KV8 ? g * 16 + 2 * j : (j >> 2) * 64 + g * 8 + (j & 3) * 2;
@@ -506,108 +558,159 @@ __global__ void __launch_bounds__(PD_WARPS * 32, NT == 1 ? 4 : (QF32 ? 2 : 3)) p
     __syncthreads();
     const bool whole = n_units == w.units;
     float* rec = reinterpret_cast<float*>(a.scratch) + (static_cast<size_t>(blockIdx.x) * 2 + (u == u_first ? 0 : 1)) * RT * PD_REC;
-    for (int row = 0; row < RT; ++row) {
-      float M = fmaxf(fmaxf(m_s[0][row], m_s[1][row]), fmaxf(m_s[2][row], m_s[3][row])), L = 0.f, acc = 0.f;
-      if (M > -INFINITY) {
 #pragma unroll
-        for (int x = 0; x < PD_WARPS; ++x) {
-          const float f = m_s[x][row] == -INFINITY ? 0.f : pd_ex2(m_s[x][row] - M);
-          L += f * l_s[x][row];
-          acc += f == 0.f ? 0.f : f * o_s[x][row][tid];
-        }
-      } else {                                 // nothing seen, or nothing but NaN
+    for (int x = 0; x < RT / PD_WARPS; ++x) {   // a warp per row, four channels per lane
+      const int row = x * PD_WARPS + warp, i = (row0 + row) / G;
+      if (whole && i >= s.n) break;
+      const float M = fmaxf(fmaxf(m_s[0][row], m_s[1][row]), fmaxf(m_s[2][row], m_s[3][row]));
+      float L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int x = 0; x < PD_WARPS; ++x) { L += l_s[x][row]; acc += o_s[x][row][tid]; }
+      for (int y = 0; y < PD_WARPS; ++y) {      // M = -inf: nothing seen, or nothing but NaN
+        const float f = M == -INFINITY ? 1.f : (m_s[y][row] == -INFINITY ? 0.f : pd_ex2(m_s[y][row] - M));
+        L += f * l_s[y][row];
+        if (f == 0.f) continue;
+        const float4 v = *reinterpret_cast<const float4*>(&o_s[y][row][lane * 4]);
+        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
       }
       if (whole) {
-        const int i = (row0 + row) / G;
-        if (i < s.n) {
-          const int hd = kvh * G + (row0 + row) % G;
-          pd_store(a, s.t0 + i, hd, tid, L == 0.f ? acc * 0.f : acc / L);
-          if (tid == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(s.t0 + i) * a.nq + hd] = pd_lse<KV8>(M, L);
-        }
+        const int hd = kvh * G + (row0 + row) % G;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        pd_store4(a, s.t0 + i, hd, lane * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        if (lane == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(s.t0 + i) * a.nq + hd] = pd_lse<KV8>(M, L);
       } else {
-        rec[row * PD_REC + tid] = acc;
-        if (tid == 0) { rec[row * PD_REC + PG_HD] = M; rec[row * PD_REC + PG_HD + 1] = L; }
+        *reinterpret_cast<float4*>(rec + row * PD_REC + lane * 4) = acc;
+        if (lane == 0) *reinterpret_cast<float2*>(rec + row * PD_REC + PG_HD) = make_float2(M, L);
       }
     }
     __syncthreads();
-    u += n_units;
+    u += taken;
   }
 }
 
-// Folds the records of the items that a range end cut. Block i looks at the cut before range i: it owns the item if that cut is the
-// first one inside it. 128 threads: one channel each.
-template <bool KV8>
-__global__ void __launch_bounds__(128) paged_fold_kernel(const __grid_constant__ IhbPagedAttn a, int grid, int RT) {
+// Folds the records of the items that a range end cut. Block (item, group of rows); WPR warps share the pieces of a row, a lane
+// holds four channels. All that depends on lengths alone is worked out while the main kernel still runs.
+template <bool KV8, int WPR>
+__global__ void __launch_bounds__(WPR == 1 ? 128 : WPR * 32) paged_fold_kernel(const __grid_constant__ IhbPagedAttn a, int grid, int RT) {
+  __shared__ __align__(16) float red[WPR][PG_HD + 4];
   const IhbPaged& c = a.c;
-  const int tid = threadIdx.x, lane = tid & 31, G = a.nq / c.nkv;
-  const long long total = pd_total(c, G, RT, lane);
-  const int parts = pd_parts(total, grid), i0 = blockIdx.x + 1;
-  if (i0 >= parts) { pdl_wait(); return; }
-  const long long cut = pd_cut(total, parts, i0);
-  long long before;
-  const int b = pd_find(c, G, RT, lane, cut, before);
-  const PgSeq s = pg_seq(c, b);
-  const PdWork w = pd_work(c, s, G, RT);
-  const int item = static_cast<int>((cut - before) / w.units);
-  const long long lo = before + static_cast<long long>(item) * w.units, hi = lo + w.units;
-  pdl_wait();
-  if (cut == lo || pd_cut(total, parts, i0 - 1) > lo) return;   // not inside an item, or an earlier cut is
-  int last = i0;                                                // ranges i0 - 1 .. last have a piece
-  while (last + 1 < parts && pd_cut(total, parts, last + 1) < hi) ++last;
-  const int kvh = item / w.tiles, row0 = (item % w.tiles) * RT;
-  const float* recs = reinterpret_cast<const float*>(a.scratch);
-  // the first range's piece is its last segment (slot 1 unless the range began inside this item or at its start)
-  const int first_slot = pd_cut(total, parts, i0 - 1) == lo ? 0 : 1;
-  for (int row = blockIdx.y; row < RT; row += gridDim.y) {
-    const int i = (row0 + row) / G;
-    if (i >= s.n) break;
-    float M = -INFINITY;
-    for (int x = i0 - 1; x <= last; ++x) M = fmaxf(M, recs[((static_cast<size_t>(x) * 2 + (x == i0 - 1 ? first_slot : 0)) * RT + row) * PD_REC + PG_HD]);
-    float L = 0.f, acc = 0.f;
-#pragma unroll 4
-    for (int x = i0 - 1; x <= last; ++x) {
-      const float* r = recs + ((static_cast<size_t>(x) * 2 + (x == i0 - 1 ? first_slot : 0)) * RT + row) * PD_REC;
-      const float mx = r[PG_HD];
-      const float f = M == -INFINITY ? 1.f : (mx == -INFINITY ? 0.f : pd_ex2(mx - M));
-      const float v = r[tid];
-      L += f * r[PG_HD + 1];
-      acc += f == 0.f ? 0.f : f * v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.nq / c.nkv;
+  // the item of this block: sequences in order, their items in order
+  int left = blockIdx.x, b = -1;
+  long long lo = 0, total = 0;
+  for (int b0 = 0; b0 < c.B; b0 += 32) {
+    PdWork w = {0, 0, 0, 0};
+    if (b0 + lane < c.B) w = pd_work(c, pg_seq(c, b0 + lane), G, RT);
+    const long long run = warp_incl_scan_ll(w.total, lane);
+    if (b < 0) {
+      const int incl = warp_incl_scan(w.items, lane);
+      const unsigned hit = __ballot_sync(0xffffffffu, incl > left);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        b = b0 + src;
+        left -= __shfl_sync(0xffffffffu, incl - w.items, src);
+        lo = total + __shfl_sync(0xffffffffu, run - w.total, src);
+      } else {
+        left -= __shfl_sync(0xffffffffu, incl, 31);
+      }
     }
-    const int hd = kvh * G + (row0 + row) % G;
-    pd_store(a, s.t0 + i, hd, tid, L == 0.f ? acc * 0.f : acc / L);
-    if (tid == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(s.t0 + i) * a.nq + hd] = pd_lse<KV8>(M, L);
+    total += __shfl_sync(0xffffffffu, run, 31);
   }
+  int first = 0, last = 0, row0 = 0, kvh = 0;
+  size_t slot0 = 0;
+  PgSeq s = {0, 0, 0, 0};
+  if (b >= 0) {
+    s = pg_seq(c, b);
+    const PdWork w = pd_work(c, s, G, RT);
+    lo += static_cast<long long>(left) * (w.units + PD_START);
+    const long long hi = lo + w.units + PD_START, key0 = lo + PD_START;
+    const int parts = pd_parts(total, grid);
+    first = static_cast<int>(key0 * parts / total);            // the range that holds the item's first unit
+    while (first + 1 < parts && pd_cut(total, parts, first + 1) <= key0) ++first;
+    while (first > 0 && pd_cut(total, parts, first) > key0) --first;
+    last = static_cast<int>((hi - 1) * parts / total);         // the range that holds its last unit
+    while (last + 1 < parts && pd_cut(total, parts, last + 1) < hi) ++last;
+    while (last > first && pd_cut(total, parts, last) >= hi) --last;
+    kvh = left / w.tiles;
+    row0 = (left % w.tiles) * RT;
+    slot0 = pd_cut(total, parts, first) >= lo ? 0 : 1;         // the first piece is its range's last segment: slot 1, or 0 if the only one
+  }
+  pdl_wait();
+  if (b < 0 || first == last) return;                          // one range had all of it and has written the result
+  const int row = WPR == 1 ? blockIdx.y * 4 + warp : blockIdx.y, i = (row0 + row) / G;
+  if (row >= RT || i >= s.n) return;
+  const float* r0 = reinterpret_cast<const float*>(a.scratch) + ((static_cast<size_t>(first) * 2 + slot0) * RT + row) * PD_REC;
+  const float* r1 = reinterpret_cast<const float*>(a.scratch) + (static_cast<size_t>(first) * 2 * RT + row) * PD_REC;   // slot 0 of the others
+  const size_t step = static_cast<size_t>(2) * RT * PD_REC;
+  const int n = last - first + 1;
+  float M = -INFINITY;
+  for (int x = lane; x < n; x += 32) M = fmaxf(M, (x == 0 ? r0 : r1 + x * step)[PG_HD]);
+  M = warp_max(M);
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int x = WPR == 1 ? 0 : warp; x < n; x += WPR) {
+    const float* r = x == 0 ? r0 : r1 + x * step;
+    const float2 ml = *reinterpret_cast<const float2*>(r + PG_HD);
+    const float4 v = *reinterpret_cast<const float4*>(r + lane * 4);
+    const float f = M == -INFINITY ? 1.f : (ml.x == -INFINITY ? 0.f : pd_ex2(ml.x - M));      // M = -inf: nothing seen, or only NaN
+    L += f * ml.y;
+    if (f != 0.f) { acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w; }
+  }
+  if (WPR > 1) {
+    *reinterpret_cast<float4*>(&red[warp][lane * 4]) = acc;
+    if (lane == 0) red[warp][PG_HD] = L;
+    __syncthreads();
+    if (warp) return;
+#pragma unroll
+    for (int x = 1; x < WPR; ++x) {
+      const float4 v = *reinterpret_cast<const float4*>(&red[x][lane * 4]);
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+      L += red[x][PG_HD];
+    }
+  }
+  const int hd = kvh * G + (row0 + row) % G;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  pd_store4(a, s.t0 + i, hd, lane * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+  if (lane == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(s.t0 + i) * a.nq + hd] = pd_lse<KV8>(M, L);
 }
 
 struct PdPlan {
-  int nt, grid;
+  int nt, per_sm, grid;
 };
 static PdPlan pd_plan(const IhbPagedAttn& a) {
   PdPlan p;
   const int G = a.nq / a.c.nkv;
   p.nt = static_cast<long long>(a.max_q) * G <= 8 ? 1 : 2;
-  const bool f32 = !a.q_bf16;
-  p.grid = 148 * (p.nt == 1 ? 4 : (f32 ? 2 : 3));             // what is resident at once
+  const bool kv8 = a.c.k_scale != nullptr;
+  p.per_sm = kv8 ? 4 : (p.nt == 2 && !a.q_bf16 ? 2 : 3);       // what is resident at once (PdSmem::PER_SM)
+  p.grid = 148 * p.per_sm;
   return p;
 }
 
-template <int NT, bool KV8, bool QF32>
+template <int NT, bool KV8, int QT, int PT>
 static cudaError_t pd_launch(const IhbPagedAttn& a, const PdPlan& p, cudaStream_t stream) {
-  paged_rows_kernel<NT, KV8, QF32><<<p.grid, PD_WARPS * 32, 0, stream>>>(a, p.grid);
-  cudaError_t e = cudaGetLastError();
+  using SM = PdSmem<NT, KV8, QT>;
+  cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<NT, KV8, QT, PT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES);
   if (e != cudaSuccess) return e;
+  paged_rows_kernel<NT, KV8, QT, PT><<<p.grid, PD_WARPS * 32, SM::BYTES, stream>>>(a, p.grid);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int G = a.nq / a.c.nkv, RT = 8 * NT;
+  const long long items = static_cast<long long>(a.c.B) * a.c.nkv * ((static_cast<long long>(a.max_q) * G + RT - 1) / RT);
+  if (items > 0x7fffffffll) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(p.grid - 1, 4);
-  cfg.blockDim = dim3(128);
+  // few items: many pieces each, eight warps share a row's; many items: two or three pieces each, a warp takes a row
+  const bool wide = items * 8 <= p.grid;
+  cfg.gridDim = dim3(static_cast<unsigned>(items), wide ? RT : RT / 4);
+  cfg.blockDim = dim3(wide ? 256 : 128);
   cfg.stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_fold_kernel<KV8>, a, p.grid, 8 * NT);
+  return wide ? cudaLaunchKernelEx(&cfg, paged_fold_kernel<KV8, 8>, a, p.grid, RT) : cudaLaunchKernelEx(&cfg, paged_fold_kernel<KV8, 1>, a, p.grid, RT);
 }
 
 }  // namespace ihb
@@ -634,10 +737,12 @@ extern "C" int ihb_paged_attention(const IhbPagedAttn* p, cudaStream_t stream) {
   if (!paged_attn_ok(a) || a.scratch == nullptr) return cudaErrorInvalidValue;
   const PdPlan pl = pd_plan(a);
   const bool kv8 = a.c.k_scale != nullptr, f32 = !a.q_bf16;
+  // terms of q / of the probabilities. e4m3 pages (fp16 products): bf16 queries are exact in one, fp32 ones take two (22 bits);
+  // bf16 pages: probabilities in one term would be off by 2^-9, in two by 2^-17; fp32 in and out takes three of both
   if (pl.nt == 1) {
-    if (kv8) return f32 ? pd_launch<1, true, true>(a, pl, stream) : pd_launch<1, true, false>(a, pl, stream);
-    return f32 ? pd_launch<1, false, true>(a, pl, stream) : pd_launch<1, false, false>(a, pl, stream);
+    if (kv8) return f32 ? pd_launch<1, true, 2, 2>(a, pl, stream) : pd_launch<1, true, 1, 1>(a, pl, stream);
+    return f32 ? pd_launch<1, false, 3, 3>(a, pl, stream) : pd_launch<1, false, 1, 2>(a, pl, stream);
   }
-  if (kv8) return f32 ? pd_launch<2, true, true>(a, pl, stream) : pd_launch<2, true, false>(a, pl, stream);
-  return f32 ? pd_launch<2, false, true>(a, pl, stream) : pd_launch<2, false, false>(a, pl, stream);
+  if (kv8) return f32 ? pd_launch<2, true, 2, 2>(a, pl, stream) : pd_launch<2, true, 1, 1>(a, pl, stream);
+  return f32 ? pd_launch<2, false, 3, 3>(a, pl, stream) : pd_launch<2, false, 1, 2>(a, pl, stream);
 }
