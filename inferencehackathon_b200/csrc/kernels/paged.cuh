@@ -61,4 +61,52 @@ __device__ __forceinline__ unsigned char pg_e4m3(float x) {
   return static_cast<unsigned char>(__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3));
 }
 
+// ---- attention ------------------------------------------------------------------------------------------------------------------
+constexpr float PD_OFF = 6.f;                // e4m3 pages: log2 of what a probability is scaled by (fp16 keeps more small ones)
+constexpr float PD_LAZY = 8.f;               // the running maximum may be passed by 2^8 before the accumulators are rescaled
+constexpr int PD_REC = PG_HD + 4;            // record of a row in a cut item: 128 channels, m, l, 2 pad
+
+template <bool F16>
+__device__ __forceinline__ unsigned pd_pack(float lo, float hi) {
+  if constexpr (F16) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
+  }
+}
+template <bool F16>
+__device__ __forceinline__ float2 pd_unpack(unsigned v) {
+  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ void pd_cvt4(unsigned w, unsigned& lo, unsigned& hi) {     // four e4m3 bytes -> two pairs of fp16
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ float pd_ex2(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// log2 of a page scale inside the range that append writes (a scale of 0 reads as the least one): the exponent from the bits, exact
+// for powers of two, and the logarithm of the mantissa for other scales (lg2.approx on [1, 2): within 2^-22).
+__device__ __forceinline__ float pd_log2_scale(float s) {
+  const unsigned u = __float_as_uint(fminf(fmaxf(s, 8.673617379884035e-19f), 1.152921504606847e18f));
+  float f;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(__uint_as_float((u & 0x7fffffu) | 0x3f800000u)));
+  return static_cast<float>(static_cast<int>(u >> 23) - 127) + f;
+}
+
+__device__ __forceinline__ void pd_store4(const IhbPagedAttn& a, int t, int h, int ch, float4 v) {
+  const size_t o = static_cast<size_t>(t) * a.out_stride_t + static_cast<size_t>(h) * a.out_stride_h + ch;
+  if (a.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o) = make_uint2(pd_pack<false>(v.x, v.y), pd_pack<false>(v.z, v.w));
+  else *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o) = v;
+}
+// (m, l) of a finished row -> natural log of its denominator
+template <bool KV8>
+__device__ __forceinline__ float pd_lse(float m, float l) {
+  return l > 0.f ? (m - (KV8 ? PD_OFF : 0.f) + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
+}
+
 }  // namespace ihb

@@ -17,15 +17,13 @@
 // ragged batches and single long sequences load every SM the same. Lengths are read on the device. An item cut by a range end
 // leaves one record (O, m, l) per piece, folded by a second kernel in a fixed order: results do not depend on timing.
 #include "paged.cuh"
+#include "paged_tiles.h"
 
 namespace ihb {
 
 constexpr int PD_WARPS = 4;
 constexpr int PD_UNIT = 64;                  // keys per unit: 16 per warp
-constexpr int PD_REC = PG_HD + 4;            // record of a row: 128 channels, m, l, 2 pad
-constexpr float PD_OFF = 6.f;                // log2 of what a probability is scaled by (fp16 keeps more small ones)
 constexpr float PD_NONE = 1e30f;             // OFF - running maximum before the first key
-constexpr float PD_LAZY = 8.f;               // the running maximum may be passed by 2^8 before the accumulators are rescaled
 
 template <bool F16>
 __device__ __forceinline__ void pd_mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
@@ -41,39 +39,7 @@ __device__ __forceinline__ unsigned pd_movt(unsigned x) {       // transpose of 
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-template <bool F16>
-__device__ __forceinline__ unsigned pd_pack(float lo, float hi) {
-  if constexpr (F16) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const unsigned*>(&v);
-  } else {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const unsigned*>(&v);
-  }
-}
-template <bool F16>
-__device__ __forceinline__ float2 pd_unpack(unsigned v) {
-  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-  else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-}
-__device__ __forceinline__ void pd_cvt4(unsigned w, unsigned& lo, unsigned& hi) {     // four e4m3 bytes -> two pairs of fp16
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-}
-__device__ __forceinline__ float pd_ex2(float x) {
-  float y;
-  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ unsigned pd_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
-// log2 of a page scale inside the range that append writes (a scale of 0 reads as the least one): the exponent from the bits, exact
-// for powers of two, and the logarithm of the mantissa for other scales (lg2.approx on [1, 2): within 2^-22).
-__device__ __forceinline__ float pd_log2_scale(float s) {
-  const unsigned u = __float_as_uint(fminf(fmaxf(s, 8.673617379884035e-19f), 1.152921504606847e18f));
-  float f;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(f) : "f"(__uint_as_float((u & 0x7fffffu) | 0x3f800000u)));
-  return static_cast<float>(static_cast<int>(u >> 23) - 127) + f;
-}
 
 // ---- work items ------------------------------------------------------------------------------------------------------------
 // An item costs its units and PD_START more (loading Q, filling the ring, adding the warps up): ranges are cut on that cost, so a CTA
@@ -135,17 +101,6 @@ __device__ __forceinline__ void pd_store(const IhbPagedAttn& a, int t, int h, in
   if (a.out_bf16) reinterpret_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16(v);
   else reinterpret_cast<float*>(a.out)[o] = v;
 }
-__device__ __forceinline__ void pd_store4(const IhbPagedAttn& a, int t, int h, int ch, float4 v) {
-  const size_t o = static_cast<size_t>(t) * a.out_stride_t + static_cast<size_t>(h) * a.out_stride_h + ch;
-  if (a.out_bf16) *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o) = make_uint2(pd_pack<false>(v.x, v.y), pd_pack<false>(v.z, v.w));
-  else *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o) = v;
-}
-// (m, l) of a finished row -> natural log of its denominator
-template <bool KV8>
-__device__ __forceinline__ float pd_lse(float m, float l) {
-  return l > 0.f ? (m - (KV8 ? PD_OFF : 0.f) + log2f(l)) * 0.6931471805599453f : (l == 0.f ? -INFINITY : l);
-}
-
 // Does row i of the call's tokens (of a sequence with s.n) see key p?
 __device__ __forceinline__ bool pd_sees(const IhbPagedAttn& a, const PgSeq& s, int i, int p) {
   if (i >= s.n || p >= s.len) return false;
@@ -726,8 +681,12 @@ static bool paged_attn_ok(const IhbPagedAttn& a) {
          a.q_stride_t % 8 == 0 && a.q_stride_h % 8 == 0;
 }
 
+// Which kernel: tiles of 128 rows on tcgen05 where a sequence may have more rows ((token, head) pairs) than two small tiles hold
+static bool use_tiles(const IhbPagedAttn& a) { return a.q_bf16 && static_cast<long long>(a.max_q) * (a.nq / a.c.nkv) > 32; }
+
 extern "C" size_t ihb_paged_attention_scratch(const IhbPagedAttn* a) {
   if (a->c.nkv < 1 || a->nq % a->c.nkv) return 0;
+  if (use_tiles(*a)) return paged_tiles_scratch(*a);
   const PdPlan p = pd_plan(*a);
   return static_cast<size_t>(p.grid) * 2 * 8 * p.nt * PD_REC * sizeof(float);
 }
@@ -735,6 +694,7 @@ extern "C" size_t ihb_paged_attention_scratch(const IhbPagedAttn* a) {
 extern "C" int ihb_paged_attention(const IhbPagedAttn* p, cudaStream_t stream) {
   const IhbPagedAttn& a = *p;
   if (!paged_attn_ok(a) || a.scratch == nullptr) return cudaErrorInvalidValue;
+  if (use_tiles(a)) return paged_tiles_launch(a, stream);
   const PdPlan pl = pd_plan(a);
   const bool kv8 = a.c.k_scale != nullptr, f32 = !a.q_bf16;
   // terms of q / of the probabilities. e4m3 pages (fp16 products): bf16 queries are exact in one, fp32 ones take two (22 bits);

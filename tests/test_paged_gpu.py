@@ -154,19 +154,20 @@ def test_append_reports_bad_pages_and_positions():
 
 
 # ---- attention ------------------------------------------------------------------------------------------------------------
-def _tol(ref, q, ref_pages, scale, cache, io, out_io):
+def _tol(ref, q, ref_pages, scale, cache, io, out_io, tiles=False):
     """What the roundings allow, relative to the largest |v| that is seen (a probability that is off by a relative d moves the
     output by at most d of that on both sides of the quotient, hence the 2):
       scores      q in two terms: fp16 pairs for e4m3 pages (22 bits), bf16 pairs for bf16 pages (16 bits; bf16 q is exact in
                   both), times |q| |k| scale; fp32 sums of 128 terms and the exponent's fp32 rounding at |s| <= 64: 2^-18
-      P           fp16 (2^-11, bf16 q over e4m3 pages), fp16 pairs (2^-22) or bf16 pairs (2^-16)
+      P           fp16 (2^-11, bf16 q over e4m3 pages), fp16 pairs (2^-22) or bf16 pairs (2^-16); bf16 q in the kernel of 128-row
+                  tiles over bf16 pages: one bf16 (2^-8)
       sums        fp32 over up to 2^12 terms: 2^-18 with room; ex2 2^-22
     and half a step of the output type."""
     vmax = float(torch.nan_to_num((ref_pages.v * (1.0 if ref_pages.vs is None else ref_pages.vs[:, :, None, None]))).abs().max())
     smax = float(q.double().norm(dim=-1).max()) * scale * float(
         torch.nan_to_num((ref_pages.k * (1.0 if ref_pages.ks is None else ref_pages.ks[:, :, None, None]))).norm(dim=-1).max())
     e_s = 0.0 if io == "bf16" else (2.0 ** -22 if cache == "fp8" else 2.0 ** -16)
-    e_p = 2.0 ** -16 if cache == "bf16" else (2.0 ** -11 if io == "bf16" else 2.0 ** -22)
+    e_p = (2.0 ** -8 if tiles and io == "bf16" else 2.0 ** -16) if cache == "bf16" else (2.0 ** -11 if io == "bf16" else 2.0 ** -22)
     return vmax * 2 * (e_s * smax + e_p + 2.0 ** -18 + 2.0 ** -18) + ref.abs() * torch.finfo(_io(out_io)).eps / 2
 
 
@@ -231,7 +232,7 @@ def test_attention(lens, news, nq, nkv, page, cache, io, masked):
     ref, ref_lse = O.attention(ref_pages, q[:T], table, lens, cu, nkv, mask)
     out, lse = _run_attn(k, v, ks, vs, table, q, cu, mask, lens, news)
     assert bool((out[T:] == 7.0).all()) and bool((lse[T:] == 7.0).all())
-    tol = _tol(ref, q[:T], ref_pages, 128 ** -0.5, cache, io, io)
+    tol = _tol(ref, q[:T], ref_pages, 128 ** -0.5, cache, io, io, tiles=max(news) * (nq // nkv) > 32)
     far = (out[:T].double().cpu() - ref).abs()
     assert bool((far <= tol).all()), (float(far.max()), float(tol.max()))
     got = lse[:T].double().cpu()
@@ -242,6 +243,34 @@ def test_attention(lens, news, nq, nkv, page, cache, io, masked):
         (ref_pages.k * (1.0 if ref_pages.ks is None else ref_pages.ks[:, :, None, None]))).norm(dim=-1).max())
     e_s = 0.0 if io == "bf16" else (2.0 ** -22 if cache == "fp8" else 2.0 ** -16)
     assert float((got - ref_lse)[~empty].abs().max()) <= e_s * smax + 2.0 ** -17
+
+
+CHUNKS = [
+    ([1500, 300, 129], [600, 129, 100], 8, 1, 64),
+    ([513, 0, 1], [513, 0, 1], 6, 2, 16),                        # odd group, from the first token
+    ([2000], [17], 64, 4, 128),                                  # two tiles of a verify window
+    ([5000, 128, 640], [8, 8, 8], 16, 1, 32),                    # one full tile: both groups share its key blocks
+    ([384, 384], [128, 256], 2, 1, 128),
+]
+
+
+@pytest.mark.parametrize("lens,news,nq,nkv,page", CHUNKS)
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("io", ["bf16", "fp32"])
+def test_attention_chunks(lens, news, nq, nkv, page, cache, io):
+    """Windows of several tiles and key blocks, cut over the GPU."""
+    k, v, ks, vs, table, q, cu, _ = _attn_case(lens, news, nq, nkv, page, cache, io, sum(lens))
+    T = sum(news)
+    ref_pages = O.Pages(k, v, ks, vs)
+    ref, ref_lse = O.attention(ref_pages, q[:T], table, lens, cu, nkv)
+    out, lse = _run_attn(k, v, ks, vs, table, q, cu, None, lens, news)
+    assert bool((out[T:] == 7.0).all())
+    tol = _tol(ref, q[:T], ref_pages, 128 ** -0.5, cache, io, io, tiles=True)
+    far = (out[:T].double().cpu() - ref).abs()
+    assert bool((far <= tol).all()), (float(far.max()), float(tol.max()))
+    assert float((lse[:T].double().cpu() - ref_lse).abs().max()) <= 2e-4
+    again, _ = _run_attn(k, v, ks, vs, table, q, cu, None, lens, news)
+    assert torch.equal(out, again)
 
 
 @pytest.mark.parametrize("cache", ["fp8", "bf16"])
@@ -259,11 +288,12 @@ def test_attention_long_contexts_are_cut_over_the_gpu(cache):
 
 
 @pytest.mark.parametrize("cache", ["fp8", "bf16"])
-@pytest.mark.parametrize("news", [[6], [40]])
-def test_what_a_token_does_not_see_never_reaches_it(cache, news):
+@pytest.mark.parametrize("news", [[6], [40], [150]])
+@pytest.mark.parametrize("io", ["fp32", "bf16"])
+def test_what_a_token_does_not_see_never_reaches_it(cache, news, io):
     """NaN (and infinities, in bf16 pages) in rows of the call that only later tokens see, and a token that sees nothing."""
     lens, nq, nkv, page = [news[0] + 30], 8, 2, 16
-    k, v, ks, vs, table, q, cu, _ = _attn_case(lens, news, nq, nkv, page, cache, "fp32", 4)
+    k, v, ks, vs, table, q, cu, _ = _attn_case(lens, news, nq, nkv, page, cache, io, 4)
     n = news[0]
     clean = O.attention(O.Pages(k, v, ks, vs), q[:n], table, lens, cu, nkv)[0]
     row = lens[0] - 2                                                                     # the last but one token's row
@@ -274,7 +304,7 @@ def test_what_a_token_does_not_see_never_reaches_it(cache, news):
         v[g, 1, r, 6] = float("inf")
     out, _ = _run_attn(k, v, ks, vs, table, q, cu, None, lens, news)
     got = out[:n].double().cpu()
-    tol = _tol(clean, q[:n], O.Pages(k, v, ks, vs), 128 ** -0.5, cache, "fp32", "fp32")
+    tol = _tol(clean, q[:n], O.Pages(k, v, ks, vs), 128 ** -0.5, cache, io, io, tiles=n * 4 > 32)
     assert bool(((got - clean).abs() <= tol)[: n - 2].all())                              # earlier tokens: untouched
     assert bool(torch.isnan(got[n - 2:, :4]).all())                                       # who sees the key: NaN everywhere
     assert bool(torch.isnan(got[n - 2:, 4:, 5]).all())                                    # who sees the value: in its channel
@@ -283,7 +313,7 @@ def test_what_a_token_does_not_see_never_reaches_it(cache, news):
     other = [c for c in range(128) if c not in (5, 6)]
     assert bool(((got - clean).abs() <= tol)[n - 2:, 4:][..., other].all())
     # with a mask that shows a token nothing and no rows ahead of the call: zeros
-    k, v, ks, vs, table, q, cu, _ = _attn_case(news, news, nq, nkv, page, cache, "fp32", 6)
+    k, v, ks, vs, table, q, cu, _ = _attn_case(news, news, nq, nkv, page, cache, io, 6)
     mask = torch.eye(n + 1, dtype=torch.bool)
     mask[2] = False
     out, lse = _run_attn(k, v, ks, vs, table, q, cu, mask, news, news)
