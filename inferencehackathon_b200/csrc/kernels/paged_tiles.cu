@@ -21,23 +21,38 @@
 namespace ihb {
 
 constexpr int PT_M = 128, PT_KB = 128;
-constexpr int PT_THREADS = 416;
+constexpr int PT_THREADS = 512;
+// Registers: 512 threads start with 128 each (all of the SM's); the loader and the issuer's group give theirs to the softmax groups, which
+// then hold a row's 128 scores: 256 x 184 + 128 x 72 + 128 x 72 = 512 x 128.
+constexpr int PT_REGS = 128, PT_REGS_SOFTMAX = 184, PT_REGS_LOAD = 72, PT_REGS_MMA = 72;
+static_assert(256 * PT_REGS_SOFTMAX + 128 * PT_REGS_LOAD + 128 * PT_REGS_MMA <= PT_THREADS * PT_REGS, "more registers than the block has");
 constexpr int PT_MMA_WARP = 12;
 constexpr int PT_HALF = 16384;                 // 128 rows x 128 bytes: one swizzled half (64 channels) of a tile
 constexpr int PT_TILE = 2 * PT_HALF;
 constexpr int PT_HDR = 2048;                // barriers; m and l of the second group at 1024 and 1536
-constexpr int PT_SMEM = PT_HDR + 6 * PT_TILE + 1024;      // Q x 2, K x 2, V x 2, alignment
+constexpr int PT_RAW = 128 * PG_HD;             // e4m3 bytes of a key block's K or V
+template <bool KV8>
+constexpr int pt_smem() { return 1024 + PT_HDR + 6 * PT_TILE + (KV8 ? 2 * PT_RAW : 0); }
 constexpr int PT_MAX_GRID = 148;              // one CTA per SM
 constexpr int PT_START = 256;                  // start-up cost of an item, in keys
 
+constexpr int PT_SEGS = 4;
+// A piece of an item: rows [row0, row0 + rows) of a sequence's KV head, key blocks [blk0, blk1) of nblk.
+struct PtSeg {
+  int b, kvh, row0, rows, blk0, blk1, nblk, first_in_range;
+  int seen_end;                                // keys that any of the rows sees lie below it
+  PgSeq s;
+  int last;                                    // no segment: the end
+};
+
 struct PtHdr {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t q_full[2], q_free, s_full[2], p_ready[2], pv_done[2];
+  uint64_t q_full[2], q_free, s_full[2], p_ready[2], pv_done[2], hand[2];
   uint32_t tmem;
   int abort_flag;
   int odd;                                     // V rows of the call's own tokens that are not finite were seen (set by the loader)
-  int b0;
-  long long before, total;
+  uint64_t seg_full[PT_SEGS], seg_free[PT_SEGS];
+  PtSeg seg[PT_SEGS];
 };
 
 // ---- work items ----------------------------------------------------------------------------------------------------------------
@@ -63,17 +78,12 @@ __device__ __forceinline__ PtWork pt_work(const IhbPagedAttn& p, const PgSeq& s,
 }
 __device__ __forceinline__ long long pt_prefix(const PtWork& w, long long j) { return j * w.a + w.d * (j * (j + 1) / 2); }
 
-struct PtSeg {
-  int kvh, row0, rows, blk0, blk1, nblk;       // rows [row0, row0 + rows) of the sequence's KV head, key blocks [blk0, blk1) of nblk
-  bool first_in_range;
-};
-// The segments of a CTA's range, in order; every role of the CTA walks them alike.
+// The segments of a CTA's range, in order.
 struct PtIter {
   long long u, u_end, u0, before;
   int b;
   PgSeq s;
   PtWork w;
-  int seen_end;
   __device__ __forceinline__ void start(const IhbPagedAttn& p, int G, int RT, long long total, long long before_, int b_, int grid) {
     u0 = u = total * blockIdx.x / grid;
     u_end = total * (blockIdx.x + 1) / grid;
@@ -84,7 +94,7 @@ struct PtIter {
       w = pt_work(p, s, G, RT);
     }
   }
-  // false at the end. Segments without a key block are passed over but for `cont` (see below).
+  // false at the end. A segment without a key block is only reported in the middle of an item (for the descriptor).
   __device__ __forceinline__ bool next(const IhbPagedAttn& p, int G, int RT, PtSeg& g) {
     while (u < u_end) {
       long long all = w.head * p.c.nkv;
@@ -109,16 +119,19 @@ struct PtIter {
       }
       const long long lo = pt_prefix(w, j), len = w.a + w.d * (j + 1);
       const long long v0 = q - lo, v1 = min(len, v0 + (u_end - u));
+      g.b = b;
+      g.s = s;
+      g.last = 0;
       g.row0 = static_cast<int>(j) * RT;
       g.rows = min(RT, s.n * G - g.row0);
       const int i_last = (g.row0 + g.rows - 1) / G;
-      seen_end = p.mask != nullptr ? s.len : min(s.len, s.base + i_last + 1);
-      g.nblk = max(1, (seen_end + PT_KB - 1) / PT_KB);
+      g.seen_end = p.mask != nullptr ? s.len : min(s.len, s.base + i_last + 1);
+      g.nblk = max(1, (g.seen_end + PT_KB - 1) / PT_KB);
       g.blk0 = static_cast<int>(v0 * g.nblk / len);
       g.blk1 = static_cast<int>(v1 * g.nblk / len);
       g.first_in_range = u == u0;
       u += v1 - v0;
-      if (g.blk0 < g.blk1 || g.blk0 > 0) return true;       // (an empty piece in the middle of an item is reported, see the descriptor)
+      if (g.blk0 < g.blk1 || g.blk0 > 0) return true;
     }
     return false;
   }
@@ -146,6 +159,27 @@ __device__ __forceinline__ void pt_ld32(uint32_t t, float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+// Four of them in flight: pt_ld32_issue x 4, pt_wait_ld, pt_pin x 4 (ties the registers' first use to the wait).
+__device__ __forceinline__ void pt_ld32_issue(uint32_t t, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+        "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]),
+        "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void pt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pt_pin(float* v) {
+  asm volatile(""
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
+                 "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
+                 "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+                 "+f"(v[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void pt_st32(uint32_t t, const float (&v)[32]) {
   __syncwarp();
   asm volatile(
@@ -165,6 +199,10 @@ __device__ __forceinline__ void pt_st16(uint32_t t, const unsigned (&v)[16]) {
       : "memory");
 }
 __device__ __forceinline__ void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void pt_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void pt_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // D[tmem] += A[tmem] * B[shared]
 __device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -185,6 +223,15 @@ __device__ __forceinline__ uint64_t pt_desc_mn(const void* tile) {
 // offset of a 16-byte chunk (8 channels) of row r in a swizzled tile
 __device__ __forceinline__ int pt_at(int r, int ch) { return (ch >> 3) * PT_HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4); }
 
+// Shared memory by 32-bit address: the aligned base is a computed pointer, which the compiler would access as generic memory.
+__device__ __forceinline__ uint4 pt_lds(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void pt_sts(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 // Does a row see key p? vis: keys below it are seen; mrow: the row's mask over the call's tokens, or NULL.
 __device__ __forceinline__ bool pt_sees(const IhbPagedAttn& a, const PgSeq& s, const unsigned char* mrow, int vis, int p) {
   if (p < vis) return true;
@@ -209,6 +256,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
   uint8_t* sq = smem + PT_HDR;
   uint8_t* sk = sq + 2 * PT_TILE;
   uint8_t* sv = sk + 2 * PT_TILE;
+  uint8_t* raw = sv + 2 * PT_TILE;             // e4m3 pages: two batches of bytes on their way to the tiles
   constexpr int RT = 2 * PT_M;
   const IhbPaged& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -225,39 +273,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       mbar_init(&sh.p_ready[i], 128); mbar_init(&sh.pv_done[i], 1);
     }
     mbar_init(&sh.q_free, 1);
+    mbar_init(&sh.hand[0], 128);
+    mbar_init(&sh.hand[1], 128);
+    for (int i = 0; i < PT_SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_free[i], 13); }
     sh.abort_flag = 0;
     sh.odd = 0;
     fence_mbar_init();
   }
   if (warp == PT_MMA_WARP) tmem_alloc(&sh.tmem, 512);
-  if (warp == 8) {                             // the sequence in which this CTA's range begins
-    long long total = 0;
-    for (int b = lane; b < c.B; b += 32) total += pt_work(a, pg_seq(c, b), G, RT).head * c.nkv;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const long long u = total * blockIdx.x / grid;
-    long long at = 0, before = 0;
-    int found = 0;
-    for (int b0 = 0; b0 < c.B; b0 += 32) {
-      long long t = 0;
-      if (b0 + lane < c.B) t = pt_work(a, pg_seq(c, b0 + lane), G, RT).head * c.nkv;
-      long long incl = t;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, at + incl > u);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        before = at + __shfl_sync(0xffffffffu, incl - t, src);
-        found = b0 + src;
-        break;
-      }
-      at += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    if (lane == 0) { sh.b0 = found; sh.before = before; sh.total = total; }
-  }
   // entries without a cached row: zeros
   for (int b = blockIdx.x; b < c.B; b += grid) {
     const PgSeq s = pg_seq(c, b);
@@ -275,70 +298,68 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   volatile int* abort_flag = &sh.abort_flag;
-  PtIter it;
-  it.start(a, G, RT, sh.total, sh.before, sh.b0, grid);
-  PtSeg sg;
+  // The next segment: every role reads the scheduler's records in order, and gives a record back (free_seg) when done with it.
+  unsigned n_seg = 0;
+  auto next_seg = [&]() -> const PtSeg* {
+    if (!tc_wait(&sh.seg_full[n_seg % PT_SEGS], (n_seg / PT_SEGS) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT)) return nullptr;
+    const PtSeg* g = &sh.seg[n_seg % PT_SEGS];
+    return g->last ? nullptr : g;
+  };
   bool ok = true;
 
   if (warp < 8) {
+    pt_regs_inc<PT_REGS_SOFTMAX>();
     // =============================== softmax groups ===============================================================================
     const int wg = warp >> 2, quarter = warp & 3, r_tile = quarter * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t t_s = lane_base + wg * 128, t_o = lane_base + 256 + wg * 128;
     constexpr float OFF = KV8 ? PD_OFF : 0.f;
-    unsigned n_blk = 0, n_seg = 0;             // blocks and segments this group has been through: barrier phases
-    PtDesc desc = {0, 0, 0, 0, 0, 0, 0, 0};
-    while (it.next(a, G, RT, sg)) {
-      const PgSeq& s = it.s;
-      if (sg.blk0 > 0) {
-        desc.cont = sg.blk0 < sg.blk1 ? 2 : 1;
-        desc.ends = sg.blk1 == sg.nblk;
-      }
-      if (sg.blk0 == sg.blk1) continue;
+    unsigned n_blk = 0, n_hand = 0;            // blocks this group has been through, segments that both groups shared: barrier phases
+    while (const PtSeg* gp = next_seg()) {
+      const PtSeg& sg = *gp;
+      const PgSeq& s = sg.s;
       const bool pair = sg.rows > PT_M;        // two tiles; else both groups have the same rows and every other key block
       const bool whole = sg.blk0 == 0 && sg.blk1 == sg.nblk;
-      const int slot = sg.first_in_range ? 0 : 1;
-      if (!whole && sg.blk0 == 0) {
-        desc.tail = 1; desc.slot = slot; desc.b = it.b; desc.kvh = sg.kvh; desc.row0 = sg.row0; desc.rows = sg.rows;
-      }
       const int r = (pair ? wg * PT_M : 0) + r_tile;                    // row of the item
       const bool live = r < sg.rows;
       const int tok = live ? (sg.row0 + r) / G : 0, head = sg.kvh * G + (live ? (sg.row0 + r) % G : 0);
-      const int vis = !live ? max(it.seen_end, 0) : (a.mask != nullptr ? max(s.base, 0) : min(max(s.base + tok + 1, 0), s.len));   // keys [0, vis) are seen
+      const int vis = !live ? max(sg.seen_end, 0) : (a.mask != nullptr ? max(s.base, 0) : min(max(s.base + tok + 1, 0), s.len));   // keys [0, vis) are seen
       const unsigned char* mrow = a.mask != nullptr && live ? a.mask + static_cast<size_t>(s.t0 + tok) * a.mask_stride : nullptr;
-      const int* table = c.block_table + static_cast<size_t>(it.b) * c.table_stride;
+      const int* table = c.block_table + static_cast<size_t>(sg.b) * c.table_stride;
       // ---- Q: one row per thread ----
       float rowf = a.scale * PG_LOG2E;
       if (ok && n_seg > 0) ok = tc_wait(&sh.q_free, (n_seg - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+      if (ok && n_hand > 0) ok = tc_wait(&sh.hand[1], (n_hand - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
       {
-        uint8_t* dst = sq + wg * PT_TILE;
+        const uint32_t dst = smem_u32(sq) + wg * PT_TILE;
         const size_t off = static_cast<size_t>(s.t0 + tok) * a.q_stride_t + static_cast<size_t>(head) * a.q_stride_h;
-        float inv = 1.f;
+        uint4 v[16];
+#pragma unroll
+        for (int ch = 0; ch < 16; ++ch) {
+          v[ch] = make_uint4(0, 0, 0, 0);
+          if (live) v[ch] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + off + ch * 8);
+        }
         if constexpr (KV8) {                   // |q| of the row into [1, 2): a power of two, exact
           float mx = 0.f;
-          if (live)
-            for (int ch = 0; ch < 16; ++ch) {
-              const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + off + ch * 8);
-              const unsigned x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
-            }
-          const int e = min(max(static_cast<int>(__float_as_uint(mx) >> 23) - 127, -100), 100);
-          rowf *= __uint_as_float(static_cast<unsigned>(127 + e) << 23);
-          inv = __uint_as_float(static_cast<unsigned>(127 - e) << 23);
-        }
-#pragma unroll 4
-        for (int ch = 0; ch < 16; ++ch) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (live) v = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + off + ch * 8);
-          if constexpr (KV8) {
-            unsigned x[4] = {v.x, v.y, v.z, v.w};
+          for (int ch = 0; ch < 16; ++ch) {
+            const unsigned x[4] = {v[ch].x, v[ch].y, v[ch].z, v[ch].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
+          }
+          const int e2 = min(max(static_cast<int>(__float_as_uint(mx) >> 23) - 127, -100), 100);
+          rowf *= __uint_as_float(static_cast<unsigned>(127 + e2) << 23);
+          const float inv = __uint_as_float(static_cast<unsigned>(127 - e2) << 23);
+#pragma unroll
+          for (int ch = 0; ch < 16; ++ch) {
+            unsigned x[4] = {v[ch].x, v[ch].y, v[ch].z, v[ch].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = pd_pack<true>(__uint_as_float(x[e] << 16) * inv, __uint_as_float(x[e] & 0xffff0000u) * inv);
-            v = make_uint4(x[0], x[1], x[2], x[3]);
+            v[ch] = make_uint4(x[0], x[1], x[2], x[3]);
           }
-          *reinterpret_cast<uint4*>(dst + pt_at(r_tile, ch)) = v;
         }
+#pragma unroll
+        for (int ch = 0; ch < 16; ++ch) pt_sts(dst + pt_at(r_tile, ch), v[ch]);
         fence_proxy_async_smem();
         mbar_arrive(&sh.q_full[wg]);
       }
@@ -346,14 +367,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       const int step = pair ? 1 : 2;
       auto page_at = [&](int blk) -> int {
         const int key = blk * PT_KB + (lane & 7) * 16;
-        return blk < sg.blk1 && key < it.seen_end ? table[key >> psh] : 0;
+        return blk < sg.blk1 && key < sg.seen_end ? table[key >> psh] : 0;
       };
       auto scales_at = [&](int blk, int page, float& ks, float& vs) {
         const bool good = static_cast<unsigned>(page) < static_cast<unsigned>(c.n_pages);
         ks = good ? 1.f : -1.f;                // negative: not seen
         vs = 1.f;
         if (KV8 && good && blk < sg.blk1) {
-          ks = c.k_scale[static_cast<size_t>(page) * c.nkv + sg.kvh];
+          ks = fmaxf(c.k_scale[static_cast<size_t>(page) * c.nkv + sg.kvh], 1e-30f);      // (0 would turn a masked -inf into NaN)
           vs = c.v_scale[static_cast<size_t>(page) * c.nkv + sg.kvh];
         }
       };
@@ -371,30 +392,52 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         const bool bad = __any_sync(0xffffffffu, ks_raw < 0.f);
         if (bad && lane == 0) set_error(c.err, ERR_BAD_ARGS);
         const bool edge = __any_sync(0xffffffffu, key0 + PT_KB > vis) || bad;
-        if (ok) ok = tc_wait(&sh.s_full[wg], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
-        tc_fence_after();
-        // ---- maximum ----
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          float v[32];
-          pt_ld32(t_s + q * 32, v);
+        unsigned seen[4] = {~0u, ~0u, ~0u, ~0u};      // bit e of word q: the row sees key q * 32 + e of the block
+        if (edge) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float kf = __shfl_sync(0xffffffffu, ks_raw, 2 * q + h), ev = KV8 ? __shfl_sync(0xffffffffu, ev_l, 2 * q + h) : 0.f;
-            const int kc = key0 + q * 32 + h * 16;
-            if (edge) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                if (kf < 0.f || !pt_sees(a, s, mrow, vis, kc + e)) v[h * 16 + e] = -INFINITY;
-              }
+          for (int q = 0; q < 4; ++q) {
+            const int kc = key0 + q * 32, n = min(max(vis - kc, 0), 32);
+            unsigned w = n == 32 ? ~0u : (1u << n) - 1u;
+            if (mrow != nullptr && n < 32)
+              for (int e = n; e < 32; ++e)
+                if (pt_sees(a, s, mrow, vis, kc + e)) w |= 1u << e;
+            if (bad) {
+              if (__shfl_sync(0xffffffffu, ks_raw, 2 * q) < 0.f) w &= 0xffff0000u;
+              if (__shfl_sync(0xffffffffu, ks_raw, 2 * q + 1) < 0.f) w &= 0x0000ffffu;
             }
-            float x = v[h * 16];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) x = fmaxf(x, v[h * 16 + e]);
-            if (x != -INFINITY) mx = fmaxf(mx, fmaf(x, kf * rowf, ev));
+            seen[q] = w;
           }
         }
+        if (ok) ok = tc_wait(&sh.s_full[wg], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+        tc_fence_after();
+        __syncwarp();
+        float v[PT_KB];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) pt_ld32_issue(t_s + q * 32, v + q * 32);
+        pt_wait_ld();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) pt_pin(v + q * 32);
+        if (edge) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen[q] & (1u << e))) v[q * 32 + e] = -INFINITY;
+        }
+        // ---- maximum ----
+        float mx = -INFINITY, kf[8], ev[8];    // factor of the scores and log2 of the V scale, per 16 keys
+#pragma unroll
+        for (int h = 0; h < 8; ++h) {
+          kf[h] = KV8 ? __shfl_sync(0xffffffffu, ks_raw, h) * rowf : rowf;
+          ev[h] = KV8 ? __shfl_sync(0xffffffffu, ev_l, h) : 0.f;
+          float x0 = v[h * 16], x1 = v[h * 16 + 1];
+#pragma unroll
+          for (int e = 2; e < 16; e += 2) { x0 = fmaxf(x0, v[h * 16 + e]); x1 = fmaxf(x1, v[h * 16 + e + 1]); }
+          x0 = fmaxf(x0, x1);
+          if (KV8) mx = fmaxf(mx, fmaf(x0, kf[h], ev[h]));
+          else mx = fmaxf(mx, x0);
+        }
+        if (!KV8) mx *= rowf;
         // ---- rescale when the maximum has grown enough ----
         if (__any_sync(0xffffffffu, mx > m + PD_LAZY)) {
           const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : pd_ex2(m - mn);
@@ -404,44 +447,38 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             if (ok) ok = tc_wait(&sh.pv_done[wg], (n_blk - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
             tc_fence_after();
 #pragma unroll 1
-            for (int q = 0; q < 4; ++q) {
-              float v[32];
-              pt_ld32(t_o + q * 32, v);
+            for (int q = 0; q < 8; ++q) {
+              float x[16];
+              __syncwarp();
+              tmem_ld16(t_o + q * 16, x);
+              unsigned y[16];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] *= f;
-              pt_st32(t_o + q * 32, v);
+              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(x[e] * f);
+              pt_st16(t_o + q * 16, y);
             }
           }
         }
         have = true;
         // ---- probabilities, in the place of the scores ----
         const float mo = OFF - (m == -INFINITY ? 0.f : m);
-#pragma unroll 1
+#pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float v[32];
-          pt_ld32(t_s + q * 32, v);
           unsigned pk[16];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float kf = __shfl_sync(0xffffffffu, ks_raw, 2 * q + h), ev = KV8 ? __shfl_sync(0xffffffffu, ev_l, 2 * q + h) : 0.f;
-            const float f = kf * rowf, add = ev + mo;
-            const int kc = key0 + q * 32 + h * 16;
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[h * 16 + e] = fmaf(v[h * 16 + e], f, add);
-            if (edge) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                if (kf < 0.f || !pt_sees(a, s, mrow, vis, kc + e)) v[h * 16 + e] = -INFINITY;
-              }
-            }
+          for (int h = 2 * q; h < 2 * q + 2; ++h) {
+            const float add = KV8 ? ev[h] + mo : mo;
+            float s0 = 0.f, s1 = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              const float p0 = pd_ex2(v[h * 16 + e]), p1 = pd_ex2(v[h * 16 + e + 1]);
-              sum += p0 + p1;
-              pk[h * 8 + e / 2] = pd_pack<KV8>(p0, p1);
+              float& x0 = v[h * 16 + e];
+              float& x1 = v[h * 16 + e + 1];
+              x0 = pd_ex2(fmaf(x0, kf[h], add));        // a masked score stays -inf: its factor is positive
+              x1 = pd_ex2(fmaf(x1, kf[h], add));
+              s0 += x0;
+              s1 += x1;
+              pk[(h & 1) * 8 + e / 2] = pd_pack<KV8>(x0, x1);
             }
-            l += KV8 ? sum * pd_ex2(-ev) : sum;
+            l += KV8 ? (s0 + s1) * pd_ex2(-ev[h]) : s0 + s1;
           }
           pt_st16(t_s + q * 16, pk);
         }
@@ -454,7 +491,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       if (have && ok) ok = tc_wait(&sh.pv_done[wg], (n_blk - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
       tc_fence_after();
       float f0 = 1.f, f1 = 0.f;
-      float* xs = reinterpret_cast<float*>(sq);
+      const uint32_t xs = smem_u32(sq) + r_tile * 512;                   // the row's place
       if (!pair) {                             // the second group hands its result over through the place of Q, which no product reads now
         float* xm = reinterpret_cast<float*>(smem + 1024);
         float* xl = reinterpret_cast<float*>(smem + 1536);
@@ -469,11 +506,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
               pt_ld32(t_o + q * 32, v);
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<float4*>(xs + r_tile * 128 + (((q * 8 + e) ^ (lane & 7)) << 2)) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                pt_sts(xs + (((q * 8 + e) ^ (lane & 7)) << 4), make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
             }
           }
         }
-        named_bar_sync(1, 256);
+        if (wg == 1) mbar_arrive(&sh.hand[0]);
+        else if (ok) ok = tc_wait(&sh.hand[0], n_hand & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
         if (wg == 0 && sg.blk1 - sg.blk0 > 1) {
           const float m1 = xm[r_tile], M = fmaxf(m, m1);
           f0 = M == -INFINITY ? 1.f : (m == -INFINITY ? 0.f : pd_ex2(m - M));       // M = -inf: nothing seen, or nothing but NaN
@@ -484,6 +522,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       }
       if (pair || wg == 0) {
         const bool odd = *reinterpret_cast<volatile int*>(&sh.odd) != 0;
+        const int slot = sg.first_in_range ? 0 : 1;
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
         float* rec = recs + ((static_cast<size_t>(blockIdx.x) * 2 + slot) * rec_rows + r) * PD_REC;
 #pragma unroll 1
@@ -493,18 +532,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           if (f1 != 0.f) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const float4 x = *reinterpret_cast<const float4*>(xs + r_tile * 128 + (((q * 8 + e) ^ (lane & 7)) << 2));
-              v[4 * e] = v[4 * e] * f0 + x.x * f1;
-              v[4 * e + 1] = v[4 * e + 1] * f0 + x.y * f1;
-              v[4 * e + 2] = v[4 * e + 2] * f0 + x.z * f1;
-              v[4 * e + 3] = v[4 * e + 3] * f0 + x.w * f1;
+              const uint4 x = pt_lds(xs + (((q * 8 + e) ^ (lane & 7)) << 4));
+              v[4 * e] = v[4 * e] * f0 + __uint_as_float(x.x) * f1;
+              v[4 * e + 1] = v[4 * e + 1] * f0 + __uint_as_float(x.y) * f1;
+              v[4 * e + 2] = v[4 * e + 2] * f0 + __uint_as_float(x.z) * f1;
+              v[4 * e + 3] = v[4 * e + 3] * f0 + __uint_as_float(x.w) * f1;
             }
           } else if (f0 != 1.f) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] *= f0;
           }
           if (odd && live)                     // values that are not finite, left out of the products: added where they are seen
-            for (int key = max(max(s.base, 0), sg.blk0 * PT_KB); key < min(it.seen_end, sg.blk1 * PT_KB); ++key) {
+            for (int key = max(max(s.base, 0), sg.blk0 * PT_KB); key < min(sg.seen_end, sg.blk1 * PT_KB); ++key) {
               const int pg = table[key >> psh];
               if (!pt_sees(a, s, mrow, vis, key) || static_cast<unsigned>(pg) >= static_cast<unsigned>(c.n_pages)) continue;
               const size_t row = (static_cast<size_t>(pg) * c.nkv + sg.kvh) * c.page + (key & (c.page - 1));
@@ -520,7 +559,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             for (int e = 0; e < 32; ++e) v[e] *= inv;
             if (a.out_bf16) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
+              for (int e = 0; e < 8; ++e)      // (strides of out are multiples of four elements)
                 *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o + 4 * e) =
                     make_uint2(pd_pack<false>(v[4 * e], v[4 * e + 1]), pd_pack<false>(v[4 * e + 2], v[4 * e + 3]));
             } else {
@@ -537,108 +576,153 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         if (live && !whole && r < rec_rows) *reinterpret_cast<float2*>(rec + PG_HD) = make_float2(m, l);
       }
       tc_fence_before();
-      if (!pair) named_bar_sync(1, 256);       // the place of Q is free again
+      if (!pair) {
+        if (wg == 0) mbar_arrive(&sh.hand[1]);                           // the place of Q is free again
+        ++n_hand;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
       ++n_seg;
     }
-    if (tid == 0) descs[blockIdx.x] = desc;
   } else if (warp < PT_MMA_WARP) {
+    pt_regs_dec<PT_REGS_LOAD>();
     // =============================== loader ===========================================================================================
-    // batches of eight 16-byte chunks per thread: K, V (e4m3) or K rows 0-63, 64-127, V rows 0-63, 64-127 (bf16); two batches in registers
-    constexpr int NB = KV8 ? 2 : 4;
+    // Batches: K, V, K, V ... of the key blocks, copied 16 bytes at a time by cp.async (rows that nobody sees: zeros). A thread works
+    // on the chunks that it copied itself, so a batch needs no barrier among the loader's threads. Two batches are under way:
+    // e4m3 bytes land in `raw` and go from there, as fp16, into the tile; bf16 rows land in the tile.
     const int lt = tid - 256;
-    const int lrow = KV8 ? lt >> 3 : lt >> 4, lch = KV8 ? lt & 7 : lt & 15;
+    constexpr int CPR = KV8 ? 8 : 16, N = KV8 ? 8 : 16, RSTEP = 128 / CPR;      // chunks per row, chunks per thread, rows between them
+    const int lrow = lt / CPR, lch = lt % CPR;
     unsigned gk = 0;                           // blocks so far
-    while (it.next(a, G, RT, sg)) {
-      if (sg.blk0 == sg.blk1) continue;
-      const PgSeq& s = it.s;
-      const int* table = c.block_table + static_cast<size_t>(it.b) * c.table_stride;
-      auto load = [&](uint4 (&buf)[8], int blk, int t) {
-        const char* base = reinterpret_cast<const char*>(t < NB / 2 ? c.k : c.v);
-        const int r0 = lrow + (KV8 ? 0 : (t & 1) * 64);
-        int page[8];
+    while (const PtSeg* gp = next_seg()) {
+      const int blk0 = gp->blk0, nb = 2 * (gp->blk1 - blk0), seen_end = gp->seen_end, base = gp->s.base;
+      const int* table = c.block_table + static_cast<size_t>(gp->b) * c.table_stride;
+      const size_t head_off = static_cast<size_t>(gp->kvh) * c.page * (PG_HD * (KV8 ? 1 : 2)) + lch * 16;
+      const unsigned page_bytes = static_cast<unsigned>(c.nkv * c.page) * (PG_HD * (KV8 ? 1 : 2));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
+      ++n_seg;
+      // pages of the block's eight groups of 16 keys: looked up while the block before is on its way, -1: nobody sees them
+      int page[8];
+      auto lookup = [&](int blk) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int key = blk * PT_KB + r0 + i * (KV8 ? 16 : 8);
-          page[i] = key < it.seen_end ? table[key >> psh] : -1;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = blk * PT_KB + r0 + i * (KV8 ? 16 : 8);
-          buf[i] = make_uint4(0, 0, 0, 0);
-          if (static_cast<unsigned>(page[i]) < static_cast<unsigned>(c.n_pages))
-            buf[i] = *reinterpret_cast<const uint4*>(base + ((static_cast<size_t>(page[i]) * c.nkv + sg.kvh) * c.page + (key & (c.page - 1))) * (KV8 ? PG_HD : 2 * PG_HD) + lch * 16);
+          const int key = blk * PT_KB + i * 16;
+          page[i] = key < seen_end ? __ldg(table + (key >> psh)) : -1;
         }
       };
-      auto store = [&](uint4 (&buf)[8], int blk, int t, int st) {
-        uint8_t* dst = (t < NB / 2 ? sk : sv) + st * PT_TILE;
-        const int r0 = lrow + (KV8 ? 0 : (t & 1) * 64);
-        if (t >= NB / 2 && blk * PT_KB + PT_KB > s.base) {        // rows of the call's own tokens: not every row sees them
-          bool hit = false;
+      auto issue = [&](int n) {                // batch n of the segment
+        const int blk = blk0 + (n >> 1);
+        const char* src0 = reinterpret_cast<const char*>((n & 1) ? c.v : c.k) + head_off;
+        const unsigned g = gk + (n >> 1);
+        const uint32_t dst = smem_u32(KV8 ? raw + (n & 1) * PT_RAW + lt * 16 : ((n & 1) ? sv : sk) + (g & 1) * PT_TILE + pt_at(lrow, lch));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (blk * PT_KB + r0 + i * (KV8 ? 16 : 8) < s.base) continue;
-            unsigned x[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
-            bool bad = false;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if constexpr (KV8) bad |= (((x[q] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;
-              else bad |= (x[q] & 0x7f80u) == 0x7f80u || (x[q] & 0x7f800000u) == 0x7f800000u;
-            }
-            if (!bad) continue;
-            hit = true;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if constexpr (KV8) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (((x[q] >> (8 * e)) & 0x7fu) == 0x7fu) x[q] &= ~(0xffu << (8 * e));
-              } else {
-                if ((x[q] & 0x7f80u) == 0x7f80u) x[q] &= 0xffff0000u;
-                if ((x[q] & 0x7f800000u) == 0x7f800000u) x[q] &= 0x0000ffffu;
-              }
-            }
-            buf[i] = make_uint4(x[0], x[1], x[2], x[3]);
-          }
-          if (hit) *reinterpret_cast<volatile int*>(&sh.odd) = 1;
+        for (int i = 0; i < N; ++i) {
+          const int key = blk * PT_KB + lrow + i * RSTEP, pg = page[KV8 ? i : i >> 1];
+          const bool good = key < seen_end && static_cast<unsigned>(pg) < static_cast<unsigned>(c.n_pages);
+          const char* src = src0 + (good ? static_cast<size_t>(pg) * page_bytes + (key & (c.page - 1)) * (PG_HD * (KV8 ? 1 : 2)) : 0);
+          // (RSTEP is 16 or 8 rows: the swizzle of a thread's rows is the same)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * (KV8 ? 2048 : RSTEP * 128)), "l"(src), "r"(good ? 16 : 0));
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if ((n & 1) && n + 1 < nb) lookup(blk + 1);
+      };
+      // what is not finite in rows of the call's own tokens (not every row sees them) is taken out; true: there was something
+      auto clean = [&](uint4& y) -> bool {
+        unsigned x[4] = {y.x, y.y, y.z, y.w};
+        bool bad = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = r0 + i * (KV8 ? 16 : 8);
-          if constexpr (KV8) {                 // 16 bytes are two chunks of eight fp16; the halves of a row start with different ones:
-            uint4 lo, hi;                      // the eight lanes of a phase then write to different banks
-            pd_cvt4(buf[i].x, lo.x, lo.y);
-            pd_cvt4(buf[i].y, lo.z, lo.w);
-            pd_cvt4(buf[i].z, hi.x, hi.y);
-            pd_cvt4(buf[i].w, hi.z, hi.w);
-            const int swap = lch >> 2;
-            *reinterpret_cast<uint4*>(dst + pt_at(row, 2 * lch + swap)) = swap ? hi : lo;
-            *reinterpret_cast<uint4*>(dst + pt_at(row, 2 * lch + 1 - swap)) = swap ? lo : hi;
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (KV8) bad |= (((x[q] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;
+          else bad |= (x[q] & 0x7f80u) == 0x7f80u || (x[q] & 0x7f800000u) == 0x7f800000u;
+        }
+        if (!bad) return false;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if constexpr (KV8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (((x[q] >> (8 * e)) & 0x7fu) == 0x7fu) x[q] &= ~(0xffu << (8 * e));
           } else {
-            *reinterpret_cast<uint4*>(dst + pt_at(row, lch)) = buf[i];
+            if ((x[q] & 0x7f80u) == 0x7f80u) x[q] &= 0xffff0000u;
+            if ((x[q] & 0x7f800000u) == 0x7f800000u) x[q] &= 0x0000ffffu;
           }
         }
+        y = make_uint4(x[0], x[1], x[2], x[3]);
+        return true;
       };
-      uint4 buf[2][8];
-      load(buf[0], sg.blk0, 0);
-      load(buf[1], sg.blk0, 1);
-      for (int blk = sg.blk0; blk < sg.blk1; ++blk, ++gk) {
-        const int st = gk & 1;
-        const unsigned par = ((gk >> 1) & 1u) ^ 1u;
+      auto wait_empty = [&](int n) {
+        const unsigned g = gk + (n >> 1);
+        if (g >= 2 && ok) ok = tc_wait((n & 1) ? &sh.v_empty[g & 1] : &sh.k_empty[g & 1], ((g >> 1) & 1u) ^ 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
+      };
+      auto finish = [&](int n) {               // batch n has landed
+        const int blk = blk0 + (n >> 1);
+        const unsigned g = gk + (n >> 1);
+        const uint32_t dst = smem_u32((n & 1) ? sv : sk) + (g & 1) * PT_TILE;
+        const bool window = (n & 1) && blk * PT_KB + PT_KB > base;
+        bool hit = false;
+        if constexpr (KV8) {
+          const uint32_t src = smem_u32(raw) + (n & 1) * PT_RAW + lt * 16;
+          // 16 bytes are two chunks of eight fp16; the halves of a row start with different ones: the eight lanes of a phase then write
+          // to different banks. The swizzle of a thread's rows (16 apart) is the same.
+          const int swap = lch >> 2;
+          const uint32_t d0 = dst + pt_at(lrow, 2 * lch + swap), d1 = dst + pt_at(lrow, 2 * lch + 1 - swap);
+          uint4 x[N];
 #pragma unroll
-        for (int t = 0; t < NB; ++t) {
-          if (t == 0 && gk >= 2 && ok) ok = tc_wait(&sh.k_empty[st], par, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
-          if (t == NB / 2 && gk >= 2 && ok) ok = tc_wait(&sh.v_empty[st], par, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
-          store(buf[t & 1], blk, t, st);
-          if (t == NB / 2 - 1 || t == NB - 1) {
-            fence_proxy_async_smem();
-            mbar_arrive(t < NB / 2 ? &sh.k_full[st] : &sh.v_full[st]);
+          for (int i = 0; i < N; ++i) x[i] = pt_lds(src + i * 2048);
+          if (window)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              if (blk * PT_KB + lrow + i * RSTEP >= base) hit |= clean(x[i]);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            uint4 lo, hi;
+            pd_cvt4(x[i].x, lo.x, lo.y);
+            pd_cvt4(x[i].y, lo.z, lo.w);
+            pd_cvt4(x[i].z, hi.x, hi.y);
+            pd_cvt4(x[i].w, hi.z, hi.w);
+            pt_sts(d0 + i * RSTEP * 128, swap ? hi : lo);
+            pt_sts(d1 + i * RSTEP * 128, swap ? lo : hi);
           }
-          if (t + 2 < NB) load(buf[t & 1], blk, t + 2);
-          else if (blk + 1 < sg.blk1) load(buf[t & 1], blk + 1, t + 2 - NB);
+        } else if (window) {
+          for (int i = 0; i < N; ++i) {
+            const uint32_t p = dst + pt_at(lrow, lch) + i * RSTEP * 128;
+            uint4 x = pt_lds(p);
+            if (blk * PT_KB + lrow + i * RSTEP >= base && clean(x)) { pt_sts(p, x); hit = true; }
+          }
         }
+        if (hit) *reinterpret_cast<volatile int*>(&sh.odd) = 1;
+        fence_proxy_async_smem();
+        mbar_arrive((n & 1) ? &sh.v_full[g & 1] : &sh.k_full[g & 1]);
+      };
+      lookup(blk0);
+      if constexpr (KV8) {
+        issue(0);
+        issue(1);
+        for (int n = 0; n < nb; ++n) {
+          if (n + 1 < nb) asm volatile("cp.async.wait_group 1;" ::: "memory");
+          else asm volatile("cp.async.wait_group 0;" ::: "memory");
+          wait_empty(n);
+          finish(n);
+          if (n + 2 < nb) issue(n + 2);
+        }
+      } else {
+        for (int n = 0; n < nb; ++n) {
+          wait_empty(n);
+          issue(n);
+          if (n > 0) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            finish(n - 1);
+          }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        finish(nb - 1);
       }
+      gk += nb >> 1;
     }
-  } else if (lane == 0) {
+  } else {
+    pt_regs_dec<PT_REGS_MMA>();
+    if (warp == PT_MMA_WARP && lane == 0) {
     // =============================== MMA issuer =========================================================================================
     constexpr uint32_t idesc = (1u << 4) | (KV8 ? 0u : ((1u << 7) | (1u << 10))) | (static_cast<uint32_t>(PT_KB >> 3) << 17) | (static_cast<uint32_t>(PT_M >> 4) << 24);
     constexpr uint32_t idesc_v = idesc | (1u << 16);                   // V: MN-major
@@ -657,10 +741,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         pt_mma_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, pt_desc_mn(sv + (gk & 1) * PT_TILE) + k * (2048 >> 4), idesc_v, !first || k > 0);
       tc_commit(&sh.pv_done[w]);
     };
-    unsigned gk = 0, n_seg = 0, n_p[2] = {0, 0};
+    unsigned gk = 0, n_p[2] = {0, 0};
     auto full = [&](uint64_t* bar, unsigned g) { return tc_wait(&bar[g & 1], (g >> 1) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT); };
-    while (ok && it.next(a, G, RT, sg)) {
-      if (sg.blk0 == sg.blk1) continue;
+    while (const PtSeg* gp = ok ? next_seg() : nullptr) {
+      const PtSeg& sg = *gp;
       const int nb = sg.blk1 - sg.blk0, ahead = sg.rows > PT_M ? 1 : 2;   // pair: both groups take block j; else group j & 1 does
       ok = tc_wait(&sh.q_full[0], n_seg & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT) &&
            tc_wait(&sh.q_full[1], n_seg & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
@@ -689,7 +773,64 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         }
       }
       tc_commit(&sh.q_free);
+      mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
       ++n_seg;
+    }
+    } else if (warp == PT_MMA_WARP + 1) {
+      // =============================== scheduler ==========================================================================================
+      long long total = 0;
+      for (int b = lane; b < c.B; b += 32) total += pt_work(a, pg_seq(c, b), G, RT).head * c.nkv;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      const long long u = total * blockIdx.x / grid;
+      long long at = 0, before = 0;
+      int found = 0;
+      for (int b0 = 0; b0 < c.B; b0 += 32) {   // the sequence in which this CTA's range begins
+        long long t = 0;
+        if (b0 + lane < c.B) t = pt_work(a, pg_seq(c, b0 + lane), G, RT).head * c.nkv;
+        long long incl = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, at + incl > u);
+        if (hit) {
+          const int src = __ffs(hit) - 1;
+          before = at + __shfl_sync(0xffffffffu, incl - t, src);
+          found = b0 + src;
+          break;
+        }
+        at += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (lane == 0) {
+        PtDesc desc = {0, 0, 0, 0, 0, 0, 0, 0};
+        PtIter it;
+        it.start(a, G, RT, total, before, found, grid);
+        for (bool more = true; more && ok;) {
+          PtSeg g;
+          g.last = 0;
+          more = it.next(a, G, RT, g);
+          if (more) {
+            if (g.blk0 > 0) {
+              desc.cont = g.blk0 < g.blk1 ? 2 : 1;
+              desc.ends = g.blk1 == g.nblk;
+            }
+            if (g.blk0 == g.blk1) continue;
+            if (g.blk0 == 0 && g.blk1 < g.nblk) {
+              desc.tail = 1; desc.slot = g.first_in_range ? 0 : 1; desc.b = g.b; desc.kvh = g.kvh; desc.row0 = g.row0; desc.rows = g.rows;
+            }
+          } else {
+            g.last = 1;
+            descs[blockIdx.x] = desc;
+          }
+          const unsigned i = n_seg % PT_SEGS;
+          if (n_seg >= PT_SEGS) ok = tc_wait(&sh.seg_free[i], ((n_seg / PT_SEGS) & 1u) ^ 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
+          sh.seg[i] = g;
+          mbar_arrive(&sh.seg_full[i]);
+          ++n_seg;
+        }
+      }
     }
   }
   tc_fence_before();
@@ -760,9 +901,15 @@ size_t paged_tiles_scratch(const IhbPagedAttn& a) {
 template <bool KV8>
 static cudaError_t pt_launch(const IhbPagedAttn& a, cudaStream_t stream) {
   const int grid = PT_MAX_GRID, rec_rows = pt_rec_rows(a);             // one CTA per SM
-  cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, PT_SMEM);
+  static const int regs = [] {                 // the register split draws on what the block is launched with
+    cudaFuncAttributes f;
+    return cudaFuncGetAttributes(&f, paged_tiles_kernel<KV8>) == cudaSuccess ? f.numRegs : 0;
+  }();
+  if (regs < PT_REGS) return cudaErrorInvalidConfiguration;
+  constexpr int bytes = pt_smem<KV8>();
+  cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  paged_tiles_kernel<KV8><<<grid, PT_THREADS, PT_SMEM, stream>>>(a, grid, rec_rows);
+  paged_tiles_kernel<KV8><<<grid, PT_THREADS, bytes, stream>>>(a, grid, rec_rows);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
