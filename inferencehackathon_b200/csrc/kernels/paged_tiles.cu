@@ -5,8 +5,10 @@
 // A CTA takes up to 256 rows ((token, query head) pairs of one sequence and KV head) as two tiles of 128 and walks key blocks of 128:
 //   warps 0-3, 4-7   one softmax group per tile, a thread per row: scores from tensor memory, running maximum and sum in registers,
 //                    probabilities (16 bits) back into tensor memory in the place of the scores
-//   warps 8-11       loader: page lookups, 16-byte loads one block ahead in registers, e4m3 -> fp16, swizzled tiles in shared memory
-//   warp 12          issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as an MN-major operand: the
+//   warps 8-11       bring V: page lookups, 16-byte asynchronous copies, e4m3 -> fp16 on the way into the swizzled tile
+//   warps 14, 15     bring K, and the page scales. e4m3 K needs no conversion: a bf16 query row, scaled by a power of two, is the sum of two
+//                    e4m3 rows (8 significant bits: 4 + 4), so S = Qhi K^T + Qlo K^T runs on e4m3 products, which are twice as fast
+//   warp 13          lays out the segments; warp 12 issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as an MN-major operand: the
 //                    rows of the cache are used as they lie, no transpose)
 // While one group computes its softmax the tensor cores work for the other. A sequence with at most 128 rows gives both groups the
 // same rows: they take the even and the odd key blocks, and their results are added up at the end.
@@ -22,17 +24,13 @@ namespace ihb {
 
 constexpr int PT_M = 128, PT_KB = 128;
 constexpr int PT_THREADS = 512;
-// Registers: 512 threads start with 128 each (all of the SM's); the loader and the issuer's group give theirs to the softmax groups, which
-// then hold a row's 128 scores: 256 x 184 + 128 x 72 + 128 x 72 = 512 x 128.
-constexpr int PT_REGS = 128, PT_REGS_SOFTMAX = 184, PT_REGS_LOAD = 72, PT_REGS_MMA = 72;
-static_assert(256 * PT_REGS_SOFTMAX + 128 * PT_REGS_LOAD + 128 * PT_REGS_MMA <= PT_THREADS * PT_REGS, "more registers than the block has");
 constexpr int PT_MMA_WARP = 12;
 constexpr int PT_HALF = 16384;                 // 128 rows x 128 bytes: one swizzled half (64 channels) of a tile
 constexpr int PT_TILE = 2 * PT_HALF;
-constexpr int PT_HDR = 2048;                // barriers; m and l of the second group at 1024 and 1536
+constexpr int PT_HDR = 3072;                   // barriers and segments; m and l of the second group at 1024 and 1536; page scales at 2048
 constexpr int PT_RAW = 128 * PG_HD;             // e4m3 bytes of a key block's K or V
 template <bool KV8>
-constexpr int pt_smem() { return 1024 + PT_HDR + 6 * PT_TILE + (KV8 ? 2 * PT_RAW : 0); }
+constexpr int pt_smem() { return PT_HDR + 6 * PT_TILE + (KV8 ? 2 * PT_RAW : 0); }
 constexpr int PT_MAX_GRID = 148;              // one CTA per SM
 constexpr int PT_START = 256;                  // start-up cost of an item, in keys
 
@@ -45,8 +43,12 @@ struct PtSeg {
   int last;                                    // no segment: the end
 };
 
+template <bool KV8>
+constexpr int pt_k_stages() { return KV8 ? 4 : 2; }             // of 16 / 32 KB
+constexpr int PT_SC = 8;                       // blocks whose page scales are kept: more than are ever under way
+
 struct PtHdr {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t k_full[4], k_empty[4], v_full[2], v_empty[2];
   uint64_t q_full[2], q_free, s_full[2], p_ready[2], pv_done[2], hand[2];
   uint32_t tmem;
   int abort_flag;
@@ -159,27 +161,6 @@ __device__ __forceinline__ void pt_ld32(uint32_t t, float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-// Four of them in flight: pt_ld32_issue x 4, pt_wait_ld, pt_pin x 4 (ties the registers' first use to the wait).
-__device__ __forceinline__ void pt_ld32_issue(uint32_t t, float* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
-      "%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
-        "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]),
-        "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-      : "r"(t)
-      : "memory");
-}
-__device__ __forceinline__ void pt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void pt_pin(float* v) {
-  asm volatile(""
-               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
-                 "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
-                 "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
-                 "+f"(v[31])
-               :
-               : "memory");
-}
 __device__ __forceinline__ void pt_st32(uint32_t t, const float (&v)[32]) {
   __syncwarp();
   asm volatile(
@@ -199,34 +180,163 @@ __device__ __forceinline__ void pt_st16(uint32_t t, const unsigned (&v)[16]) {
       : "memory");
 }
 __device__ __forceinline__ void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void pt_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void pt_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-// D[tmem] += A[tmem] * B[shared]
-__device__ __forceinline__ void pt_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(acc)
-      : "memory");
+// Eight products, D[tmem] (+)= A B. PT_QK16: 16 channels each, both operands in shared memory (K-major, two swizzled halves); PT_QK8: e4m3, 32
+// channels each, first Q's heads, then its remainders (a half further on) with the same K; PT_PV: 16 keys each, A in tensor memory (8
+// columns per step), B in shared memory, MN-major. The issuing thread shares its scheduler with softmax warps, so the descriptors'
+// high words are constants and a step costs one or two additions.
+enum { PT_QK16, PT_QK8, PT_PV };
+template <int KIND>
+__device__ __forceinline__ void pt_mma8(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  // high word: stride offset 1024 bytes, version 1, 128-byte swizzle
+  if constexpr (KIND == PT_PV)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 b, {%2, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t"
+        "add.u32 x, %1, 8;\n\tadd.u32 y, %2, 128;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
+        "add.u32 x, %1, 16;\n\tadd.u32 y, %2, 256;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
+        "add.u32 x, %1, 24;\n\tadd.u32 y, %2, 384;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
+        "add.u32 x, %1, 32;\n\tadd.u32 y, %2, 512;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
+        "add.u32 x, %1, 40;\n\tadd.u32 y, %2, 640;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
+        "add.u32 x, %1, 48;\n\tadd.u32 y, %2, 768;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
+        "add.u32 x, %1, 56;\n\tadd.u32 y, %2, 896;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t}"
+        ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(acc), "n"(0x40004040)
+        : "memory");
+  else if constexpr (KIND == PT_QK8)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t"
+        "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 1024;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {%2, %5};\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 1026;\n\tadd.u32 y, %2, 2;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 1028;\n\tadd.u32 y, %2, 4;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 1030;\n\tadd.u32 y, %2, 6;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, 1;\n\t}"
+        ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(acc), "n"(0x40004040)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t"
+        "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 1024;\n\tadd.u32 y, %2, 1024;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 1026;\n\tadd.u32 y, %2, 1026;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 1028;\n\tadd.u32 y, %2, 1028;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t"
+        "add.u32 x, %1, 1030;\n\tadd.u32 y, %2, 1030;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n\t}"
+        ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(acc), "n"(0x40004040)
+        : "memory");
 }
-// Shared-memory descriptor of an MN-major operand, 128-byte swizzle: rows of 64 MN elements (128 bytes), one per K; the next 64 MN
-// elements PT_HALF bytes on (leading offset), groups of 8 K 1024 bytes apart (stride offset).
-__device__ __forceinline__ uint64_t pt_desc_mn(const void* tile) {
-  uint64_t d = (static_cast<uint64_t>(smem_u32(tile)) >> 4) & 0x3FFFull;
-  d |= static_cast<uint64_t>(PT_HALF >> 4) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
-  d |= 1ull << 46;
-  d |= 2ull << 61;
-  return d;
-}
+// Low words of the descriptors: start address; leading offset 16 bytes (K-major: unused) or PT_HALF (MN-major: rows of 64 MN elements, one
+// per K, the next 64 a half further on; the stride offset is then that of 8 K).
+__device__ __forceinline__ uint32_t pt_lo_k(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ uint32_t pt_lo_mn(uint32_t addr) { return ((addr >> 4) & 0x3FFFu) | (static_cast<uint32_t>(PT_HALF >> 4) << 16); }
 // offset of a 16-byte chunk (8 channels) of row r in a swizzled tile
 __device__ __forceinline__ int pt_at(int r, int ch) { return (ch >> 3) * PT_HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4); }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pt_pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void pt_unpair(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t pt_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pt_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float pt_max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ void pt_mask32(float* v, unsigned seen) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (!(seen & (1u << e))) v[e] = -INFINITY;
+}
+// What one of NTH loader threads copies of a key block: RPT rows of one of its groups of 16 keys (one page: one lookup), COLS 16-byte chunks
+// of each. A warp's copies cover whole rows.
+template <bool KV8, int NTH>
+struct PtRows {
+  static constexpr int ROWB = KV8 ? PG_HD : 2 * PG_HD, TPG = NTH / 8, COLS = KV8 || TPG == 16 ? 1 : 2, CPT = ROWB / 16 / COLS, RPT = 16 * CPT / TPG;
+  int grp, row, ch, key0, end, blk, psh, in_page;
+  unsigned page_bytes;
+  const char* src;
+  const int* table;
+  int page;                                    // of the next block's group, looked up while the block before is on its way
+  __device__ __forceinline__ PtRows(const IhbPaged& c, int t, int psh_) : grp(t / TPG), row((t % TPG) / CPT * RPT), ch(t % CPT), psh(psh_), in_page(c.page - 1) {
+    page_bytes = static_cast<unsigned>(c.nkv * c.page) * ROWB;
+  }
+  __device__ __forceinline__ void start(const IhbPaged& c, const void* base, const PtSeg& g) {
+    key0 = g.blk0 * PT_KB + grp * 16;
+    end = min(g.seen_end, g.blk1 * PT_KB);     // keys from here on: zeros
+    blk = 0;
+    src = reinterpret_cast<const char*>(base) + static_cast<size_t>(g.kvh) * c.page * ROWB + ch * 16;
+    table = c.block_table + static_cast<size_t>(g.b) * c.table_stride;
+    lookup();
+  }
+  __device__ __forceinline__ void lookup() {
+    const int key = key0 + blk * PT_KB;
+    page = key < end ? __ldg(table + (key >> psh)) : -1;
+  }
+  static __device__ __forceinline__ void copy(uint32_t d, const char* p, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(p), "r"(n));
+  }
+  // Copies the next block. TILE: row r's chunk to its place in the swizzled tile at dst; else chunk i to dst + i * 2048 (the thread's own).
+  template <bool TILE>
+  __device__ __forceinline__ void issue(uint32_t dst, int n_pages) {
+    const int key = key0 + blk * PT_KB + row;
+    const bool good = static_cast<unsigned>(page) < static_cast<unsigned>(n_pages);
+    const int live = good ? min(max(end - key, 0), RPT) : 0;
+    const char* p = src + (good ? static_cast<size_t>(page) * page_bytes + (key & in_page) * ROWB : 0);
+    const int r0 = grp * 16 + row;             // a multiple of 8: the swizzle of row r0 + i is that of i
+    const uint32_t d = TILE ? dst + r0 * 128 + (ch << 4 & 127) + (ch >> 3) * PT_HALF : dst;
+    if (live == RPT) {
+#pragma unroll
+      for (int i = 0; i < RPT; ++i)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) copy(TILE ? (d ^ ((i & 7) << 4)) + i * 128 + c * PT_HALF : d + i * 2048, p + i * ROWB + c * 128, 16);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < RPT; ++i)
+        for (int c = 0; c < COLS; ++c)
+          copy(TILE ? (d ^ ((i & 7) << 4)) + i * 128 + c * PT_HALF : d + i * 2048, i < live ? p + i * ROWB + c * 128 : src, i < live ? 16 : 0);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ++blk;
+    lookup();
+  }
+};
+// Takes what is not finite out of 16 bytes of V; true: there was something.
+template <bool KV8>
+__device__ __noinline__ bool pt_clean(uint4& y) {
+  unsigned x[4] = {y.x, y.y, y.z, y.w};
+  bool bad = false;
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (KV8) {
+      for (int e = 0; e < 4; ++e)
+        if (((x[q] >> (8 * e)) & 0x7fu) == 0x7fu) { x[q] &= ~(0xffu << (8 * e)); bad = true; }
+    } else {
+      if ((x[q] & 0x7f80u) == 0x7f80u) { x[q] &= 0xffff0000u; bad = true; }
+      if ((x[q] & 0x7f800000u) == 0x7f800000u) { x[q] &= 0x0000ffffu; bad = true; }
+    }
+  }
+  y = make_uint4(x[0], x[1], x[2], x[3]);
+  return bad;
+}
 // Shared memory by 32-bit address: the aligned base is a computed pointer, which the compiler would access as generic memory.
 __device__ __forceinline__ uint4 pt_lds(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 pt_lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
 __device__ __forceinline__ void pt_sts(uint32_t a, uint4 v) {
@@ -250,13 +360,15 @@ __device__ __forceinline__ float pt_v_at(const IhbPaged& c, size_t row, int ch) 
 
 template <bool KV8>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid_constant__ IhbPagedAttn a, int grid, int rec_rows) {
-  extern __shared__ uint8_t pt_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];            // (checked below: the swizzle goes by address)
   PtHdr& sh = *reinterpret_cast<PtHdr*>(smem);
   uint8_t* sq = smem + PT_HDR;
+  // per block and 16 keys: factor of the scores (negative: no such page), log2 of the V scale, 1 / V scale; .w of the first: a page is missing
+  float4* sc = reinterpret_cast<float4*>(smem + 2048);         // [PT_SC][8]
   uint8_t* sk = sq + 2 * PT_TILE;
   uint8_t* sv = sk + 2 * PT_TILE;
-  uint8_t* raw = sv + 2 * PT_TILE;             // e4m3 pages: two batches of bytes on their way to the tiles
+  uint8_t* raw = sv + 2 * PT_TILE;             // e4m3 pages: the bytes of two V blocks on their way to the tiles
+  constexpr int KS = pt_k_stages<KV8>(), K_BYTES = 2 * PT_TILE / KS;
   constexpr int RT = 2 * PT_M;
   const IhbPaged& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -267,15 +379,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
 
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.k_full[i], 128); mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.k_full[2 * i], 64); mbar_init(&sh.k_full[2 * i + 1], 64);
+      mbar_init(&sh.k_empty[2 * i], 1); mbar_init(&sh.k_empty[2 * i + 1], 1);
       mbar_init(&sh.v_full[i], 128); mbar_init(&sh.v_empty[i], 1);
-      mbar_init(&sh.q_full[i], 128); mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.q_full[i], 128); mbar_init(&sh.s_full[i], 2);
       mbar_init(&sh.p_ready[i], 128); mbar_init(&sh.pv_done[i], 1);
     }
     mbar_init(&sh.q_free, 1);
     mbar_init(&sh.hand[0], 128);
     mbar_init(&sh.hand[1], 128);
-    for (int i = 0; i < PT_SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_free[i], 13); }
+    for (int i = 0; i < PT_SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_free[i], 15); }
     sh.abort_flag = 0;
     sh.odd = 0;
     fence_mbar_init();
@@ -293,6 +406,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       if (lane == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(s.t0) * a.nq + i] = -INFINITY;
     }
   }
+  if (tid == 0 && (smem_u32(smem) & 1023u)) { set_error(c.err, ERR_BAD_ARGS); sh.abort_flag = 1; }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -308,13 +422,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
   bool ok = true;
 
   if (warp < 8) {
-    pt_regs_inc<PT_REGS_SOFTMAX>();
     // =============================== softmax groups ===============================================================================
     const int wg = warp >> 2, quarter = warp & 3, r_tile = quarter * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     const uint32_t t_s = lane_base + wg * 128, t_o = lane_base + 256 + wg * 128;
     constexpr float OFF = KV8 ? PD_OFF : 0.f;
-    unsigned n_blk = 0, n_hand = 0;            // blocks this group has been through, segments that both groups shared: barrier phases
+    unsigned g0 = 0, n_blk = 0, n_hand = 0;            // blocks of earlier segments; blocks this group has been through, segments that both groups shared: barrier phases
     while (const PtSeg* gp = next_seg()) {
       const PtSeg& sg = *gp;
       const PgSeq& s = sg.s;
@@ -339,7 +452,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           v[ch] = make_uint4(0, 0, 0, 0);
           if (live) v[ch] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + off + ch * 8);
         }
-        if constexpr (KV8) {                   // |q| of the row into [1, 2): a power of two, exact
+        if constexpr (KV8) {                   // |q| of the row below 256 by a power of two, then an e4m3 head and an e4m3 remainder
           float mx = 0.f;
 #pragma unroll
           for (int ch = 0; ch < 16; ++ch) {
@@ -347,49 +460,42 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
 #pragma unroll
             for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
           }
-          const int e2 = min(max(static_cast<int>(__float_as_uint(mx) >> 23) - 127, -100), 100);
-          rowf *= __uint_as_float(static_cast<unsigned>(127 + e2) << 23);
+          const int e2 = min(max(static_cast<int>(__float_as_uint(mx) >> 23) - 127 - 7, -100), 100);
+          rowf *= mx <= 3.4028235e38f ? __uint_as_float(static_cast<unsigned>(127 + e2) << 23) : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
           const float inv = __uint_as_float(static_cast<unsigned>(127 - e2) << 23);
 #pragma unroll
-          for (int ch = 0; ch < 16; ++ch) {
-            unsigned x[4] = {v[ch].x, v[ch].y, v[ch].z, v[ch].w};
+          for (int ch = 0; ch < 8; ++ch) {
+            const unsigned x[8] = {v[2 * ch].x, v[2 * ch].y, v[2 * ch].z, v[2 * ch].w, v[2 * ch + 1].x, v[2 * ch + 1].y, v[2 * ch + 1].z, v[2 * ch + 1].w};
+            unsigned hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = pd_pack<true>(__uint_as_float(x[e] << 16) * inv, __uint_as_float(x[e] & 0xffff0000u) * inv);
-            v[ch] = make_uint4(x[0], x[1], x[2], x[3]);
+            for (int e = 0; e < 4; ++e) {
+              const float y0 = __uint_as_float(x[2 * e] << 16) * inv, y1 = __uint_as_float(x[2 * e] & 0xffff0000u) * inv;
+              const float y2 = __uint_as_float(x[2 * e + 1] << 16) * inv, y3 = __uint_as_float(x[2 * e + 1] & 0xffff0000u) * inv;
+              hi[e] = static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y0, y1), __NV_SATFINITE, __NV_E4M3)) |
+                      static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y2, y3), __NV_SATFINITE, __NV_E4M3)) << 16;
+              const float4 h = e4m3x4_to_float4(hi[e]);
+              lo[e] = static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y0 - h.x, y1 - h.y), __NV_SATFINITE, __NV_E4M3)) |
+                      static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y2 - h.z, y3 - h.w), __NV_SATFINITE, __NV_E4M3)) << 16;
+            }
+            pt_sts(dst + pt_at(r_tile, ch), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            pt_sts(dst + PT_HALF + pt_at(r_tile, ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
           }
-        }
+        } else {
 #pragma unroll
-        for (int ch = 0; ch < 16; ++ch) pt_sts(dst + pt_at(r_tile, ch), v[ch]);
+          for (int ch = 0; ch < 16; ++ch) pt_sts(dst + pt_at(r_tile, ch), v[ch]);
+        }
         fence_proxy_async_smem();
         mbar_arrive(&sh.q_full[wg]);
       }
-      // ---- page scales: lane i (0 .. 7) looks after the 16 keys i of a block, one block ahead ----
-      const int step = pair ? 1 : 2;
-      auto page_at = [&](int blk) -> int {
-        const int key = blk * PT_KB + (lane & 7) * 16;
-        return blk < sg.blk1 && key < sg.seen_end ? table[key >> psh] : 0;
-      };
-      auto scales_at = [&](int blk, int page, float& ks, float& vs) {
-        const bool good = static_cast<unsigned>(page) < static_cast<unsigned>(c.n_pages);
-        ks = good ? 1.f : -1.f;                // negative: not seen
-        vs = 1.f;
-        if (KV8 && good && blk < sg.blk1) {
-          ks = fmaxf(c.k_scale[static_cast<size_t>(page) * c.nkv + sg.kvh], 1e-30f);      // (0 would turn a masked -inf into NaN)
-          vs = c.v_scale[static_cast<size_t>(page) * c.nkv + sg.kvh];
-        }
-      };
-      int blk = sg.blk0 + (pair ? 0 : wg);
-      float ks_n, vs_n;
-      scales_at(blk, page_at(blk), ks_n, vs_n);
-      int page_n = page_at(blk + step);
+      const int step = pair ? 1 : 2, blk_end = sg.blk1, blk_first = sg.blk0;
       float m = -INFINITY, l = 0.f;
       bool have = false;                       // O holds something
-      for (; blk < sg.blk1; blk += step) {
-        const float ks_raw = ks_n, ev_l = KV8 ? pd_log2_scale(vs_n) : 0.f;          // of the lane's 16 keys
-        scales_at(blk + step, page_n, ks_n, vs_n);
-        page_n = page_at(blk + 2 * step);
+      for (int blk = blk_first + (pair ? 0 : wg); blk < blk_end; blk += step) {
+        if (ok) ok = tc_wait(&sh.s_full[wg], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+        tc_fence_after();
+        const float4* sb = sc + ((g0 + blk - blk_first) % PT_SC) * 8;
         const int key0 = blk * PT_KB;
-        const bool bad = __any_sync(0xffffffffu, ks_raw < 0.f);
+        const bool bad = sb[0].w != 0.f;
         if (bad && lane == 0) set_error(c.err, ERR_BAD_ARGS);
         const bool edge = __any_sync(0xffffffffu, key0 + PT_KB > vis) || bad;
         unsigned seen[4] = {~0u, ~0u, ~0u, ~0u};      // bit e of word q: the row sees key q * 32 + e of the block
@@ -402,40 +508,33 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
               for (int e = n; e < 32; ++e)
                 if (pt_sees(a, s, mrow, vis, kc + e)) w |= 1u << e;
             if (bad) {
-              if (__shfl_sync(0xffffffffu, ks_raw, 2 * q) < 0.f) w &= 0xffff0000u;
-              if (__shfl_sync(0xffffffffu, ks_raw, 2 * q + 1) < 0.f) w &= 0x0000ffffu;
+              if (sb[2 * q].x < 0.f) w &= 0xffff0000u;
+              if (sb[2 * q + 1].x < 0.f) w &= 0x0000ffffu;
             }
             seen[q] = w;
           }
         }
-        if (ok) ok = tc_wait(&sh.s_full[wg], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
-        tc_fence_after();
-        __syncwarp();
-        float v[PT_KB];
+        // ---- maximum. Both passes read the scores from tensor memory, 32 at a time, in short loops: unrolled over the row's 128 scores the
+        // kernel's hot code is several times the first instruction cache, and every warp of the SM pays for it ----
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          float v[32];
+          pt_ld32(t_s + q * 32, v);
+          if (edge) pt_mask32(v, q < 2 ? (q ? seen[1] : seen[0]) : (q == 2 ? seen[2] : seen[3]));
 #pragma unroll
-        for (int q = 0; q < 4; ++q) pt_ld32_issue(t_s + q * 32, v + q * 32);
-        pt_wait_ld();
+          for (int h = 0; h < 2; ++h) {
+            float x = pt_max3(v[h * 16], v[h * 16 + 1], v[h * 16 + 2]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) pt_pin(v + q * 32);
-        if (edge) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(seen[q] & (1u << e))) v[q * 32 + e] = -INFINITY;
-        }
-        // ---- maximum ----
-        float mx = -INFINITY, kf[8], ev[8];    // factor of the scores and log2 of the V scale, per 16 keys
-#pragma unroll
-        for (int h = 0; h < 8; ++h) {
-          kf[h] = KV8 ? __shfl_sync(0xffffffffu, ks_raw, h) * rowf : rowf;
-          ev[h] = KV8 ? __shfl_sync(0xffffffffu, ev_l, h) : 0.f;
-          float x0 = v[h * 16], x1 = v[h * 16 + 1];
-#pragma unroll
-          for (int e = 2; e < 16; e += 2) { x0 = fmaxf(x0, v[h * 16 + e]); x1 = fmaxf(x1, v[h * 16 + e + 1]); }
-          x0 = fmaxf(x0, x1);
-          if (KV8) mx = fmaxf(mx, fmaf(x0, kf[h], ev[h]));
-          else mx = fmaxf(mx, x0);
+            for (int e = 3; e < 15; e += 2) x = pt_max3(x, v[h * 16 + e], v[h * 16 + e + 1]);
+            x = fmaxf(x, v[h * 16 + 15]);
+            if (KV8) {
+              const float2 ke = *reinterpret_cast<const float2*>(&sb[2 * q + h]);
+              mx = fmaxf(mx, fmaf(x, fabsf(ke.x) * rowf, ke.y));
+            } else {
+              mx = fmaxf(mx, x);
+            }
+          }
         }
         if (!KV8) mx *= rowf;
         // ---- rescale when the maximum has grown enough ----
@@ -461,26 +560,33 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         have = true;
         // ---- probabilities, in the place of the scores ----
         const float mo = OFF - (m == -INFINITY ? 0.f : m);
-#pragma unroll
+#pragma unroll 1
         for (int q = 0; q < 4; ++q) {
+          float v[32];
+          pt_ld32(t_s + q * 32, v);
+          if (edge) pt_mask32(v, q < 2 ? (q ? seen[1] : seen[0]) : (q == 2 ? seen[2] : seen[3]));
           unsigned pk[16];
 #pragma unroll
-          for (int h = 2 * q; h < 2 * q + 2; ++h) {
-            const float add = KV8 ? ev[h] + mo : mo;
-            float s0 = 0.f, s1 = 0.f;
+          for (int h = 0; h < 2; ++h) {
+            float4 ke = make_float4(1.f, 0.f, 1.f, 0.f);
+            if (KV8) ke = sb[2 * q + h];
+            const float f = KV8 ? fabsf(ke.x) * rowf : rowf, add = KV8 ? ke.y + mo : mo;
+            const uint64_t f2 = pt_pair(f, f), add2 = pt_pair(add, add);
+            uint64_t sum = 0;                  // (0.f, 0.f)
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              float& x0 = v[h * 16 + e];
-              float& x1 = v[h * 16 + e + 1];
-              x0 = pd_ex2(fmaf(x0, kf[h], add));        // a masked score stays -inf: its factor is positive
-              x1 = pd_ex2(fmaf(x1, kf[h], add));
-              s0 += x0;
-              s1 += x1;
-              pk[(h & 1) * 8 + e / 2] = pd_pack<KV8>(x0, x1);
+              float p0, p1;
+              pt_unpair(pt_fma2(pt_pair(v[h * 16 + e], v[h * 16 + e + 1]), f2, add2), p0, p1);      // a masked score stays -inf: f > 0
+              p0 = pd_ex2(p0);
+              p1 = pd_ex2(p1);
+              sum = pt_add2(sum, pt_pair(p0, p1));
+              pk[h * 8 + e / 2] = pd_pack<KV8>(p0, p1);
             }
-            l += KV8 ? (s0 + s1) * pd_ex2(-ev[h]) : s0 + s1;
+            float s0, s1;
+            pt_unpair(sum, s0, s1);
+            l += KV8 ? (s0 + s1) * ke.z : s0 + s1;
           }
-          pt_st16(t_s + q * 16, pk);
+          pt_st16(t_s + q * 16, pk);           // (the scores that these columns held have been read)
         }
         pt_wait_st();
         tc_fence_before();
@@ -580,198 +686,214 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         if (wg == 0) mbar_arrive(&sh.hand[1]);                           // the place of Q is free again
         ++n_hand;
       }
+      g0 += blk_end - blk_first;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
       ++n_seg;
     }
   } else if (warp < PT_MMA_WARP) {
-    pt_regs_dec<PT_REGS_LOAD>();
     // =============================== loader ===========================================================================================
-    // Batches: K, V, K, V ... of the key blocks, copied 16 bytes at a time by cp.async (rows that nobody sees: zeros). A thread works
-    // on the chunks that it copied itself, so a batch needs no barrier among the loader's threads. Two batches are under way:
-    // e4m3 bytes land in `raw` and go from there, as fp16, into the tile; bf16 rows land in the tile.
+    // V blocks, copied 16 bytes at a time by cp.async (rows that nobody sees: zeros). A thread works on the chunks that it copied itself, so a
+    // block needs no barrier among the loader's threads. Two blocks are under way: e4m3 bytes land in `raw` and go from there, as fp16,
+    // into the tile; bf16 rows land in the tile.
     const int lt = tid - 256;
-    constexpr int CPR = KV8 ? 8 : 16, N = KV8 ? 8 : 16, RSTEP = 128 / CPR;      // chunks per row, chunks per thread, rows between them
-    const int lrow = lt / CPR, lch = lt % CPR;
+    using Rows = PtRows<KV8, 128>;
+    Rows rows(c, lt, psh);
     unsigned gk = 0;                           // blocks so far
     while (const PtSeg* gp = next_seg()) {
-      const int blk0 = gp->blk0, nb = 2 * (gp->blk1 - blk0), seen_end = gp->seen_end, base = gp->s.base;
-      const int* table = c.block_table + static_cast<size_t>(gp->b) * c.table_stride;
-      const size_t head_off = static_cast<size_t>(gp->kvh) * c.page * (PG_HD * (KV8 ? 1 : 2)) + lch * 16;
-      const unsigned page_bytes = static_cast<unsigned>(c.nkv * c.page) * (PG_HD * (KV8 ? 1 : 2));
+      const int nb = gp->blk1 - gp->blk0, base = gp->s.base, first = gp->blk0 * PT_KB;
+      rows.start(c, c.v, *gp);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
       ++n_seg;
-      // pages of the block's eight groups of 16 keys: looked up while the block before is on its way, -1: nobody sees them
-      int page[8];
-      auto lookup = [&](int blk) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = blk * PT_KB + i * 16;
-          page[i] = key < seen_end ? __ldg(table + (key >> psh)) : -1;
-        }
-      };
-      auto issue = [&](int n) {                // batch n of the segment
-        const int blk = blk0 + (n >> 1);
-        const char* src0 = reinterpret_cast<const char*>((n & 1) ? c.v : c.k) + head_off;
-        const unsigned g = gk + (n >> 1);
-        const uint32_t dst = smem_u32(KV8 ? raw + (n & 1) * PT_RAW + lt * 16 : ((n & 1) ? sv : sk) + (g & 1) * PT_TILE + pt_at(lrow, lch));
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int key = blk * PT_KB + lrow + i * RSTEP, pg = page[KV8 ? i : i >> 1];
-          const bool good = key < seen_end && static_cast<unsigned>(pg) < static_cast<unsigned>(c.n_pages);
-          const char* src = src0 + (good ? static_cast<size_t>(pg) * page_bytes + (key & (c.page - 1)) * (PG_HD * (KV8 ? 1 : 2)) : 0);
-          // (RSTEP is 16 or 8 rows: the swizzle of a thread's rows is the same)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * (KV8 ? 2048 : RSTEP * 128)), "l"(src), "r"(good ? 16 : 0));
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if ((n & 1) && n + 1 < nb) lookup(blk + 1);
-      };
-      // what is not finite in rows of the call's own tokens (not every row sees them) is taken out; true: there was something
-      auto clean = [&](uint4& y) -> bool {
-        unsigned x[4] = {y.x, y.y, y.z, y.w};
-        bool bad = false;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if constexpr (KV8) bad |= (((x[q] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u;
-          else bad |= (x[q] & 0x7f80u) == 0x7f80u || (x[q] & 0x7f800000u) == 0x7f800000u;
-        }
-        if (!bad) return false;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if constexpr (KV8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (((x[q] >> (8 * e)) & 0x7fu) == 0x7fu) x[q] &= ~(0xffu << (8 * e));
-          } else {
-            if ((x[q] & 0x7f80u) == 0x7f80u) x[q] &= 0xffff0000u;
-            if ((x[q] & 0x7f800000u) == 0x7f800000u) x[q] &= 0x0000ffffu;
-          }
-        }
-        y = make_uint4(x[0], x[1], x[2], x[3]);
-        return true;
-      };
       auto wait_empty = [&](int n) {
-        const unsigned g = gk + (n >> 1);
-        if (g >= 2 && ok) ok = tc_wait((n & 1) ? &sh.v_empty[g & 1] : &sh.k_empty[g & 1], ((g >> 1) & 1u) ^ 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
+        const unsigned g = gk + n;
+        if (g >= 2 && ok) ok = tc_wait(&sh.v_empty[g & 1], ((g >> 1) & 1u) ^ 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
       };
-      auto finish = [&](int n) {               // batch n has landed
-        const int blk = blk0 + (n >> 1);
-        const unsigned g = gk + (n >> 1);
-        const uint32_t dst = smem_u32((n & 1) ? sv : sk) + (g & 1) * PT_TILE;
-        const bool window = (n & 1) && blk * PT_KB + PT_KB > base;
+      auto finish = [&](int n) {               // block n has landed
+        const unsigned g = gk + n;
+        const int r0 = rows.grp * 16 + rows.row, key = first + n * PT_KB + r0;
+        const uint32_t dst = smem_u32(sv) + (g & 1) * PT_TILE + r0 * 128;
+        // rows of the call's own tokens, which not every row sees: what is not finite is taken out here and added where it is seen
+        const bool window = first + n * PT_KB + PT_KB > base;
         bool hit = false;
         if constexpr (KV8) {
           const uint32_t src = smem_u32(raw) + (n & 1) * PT_RAW + lt * 16;
-          // 16 bytes are two chunks of eight fp16; the halves of a row start with different ones: the eight lanes of a phase then write
-          // to different banks. The swizzle of a thread's rows (16 apart) is the same.
-          const int swap = lch >> 2;
-          const uint32_t d0 = dst + pt_at(lrow, 2 * lch + swap), d1 = dst + pt_at(lrow, 2 * lch + 1 - swap);
-          uint4 x[N];
-#pragma unroll
-          for (int i = 0; i < N; ++i) x[i] = pt_lds(src + i * 2048);
           if (window)
+#pragma unroll 1
+            for (int i = 0; i < Rows::RPT; ++i)
+              if (key + i >= base) {
+                uint4 x = pt_lds(src + i * 2048);
+                if (pt_clean<true>(x)) { pt_sts(src + i * 2048, x); hit = true; }
+              }
+          // 16 bytes are two chunks of eight fp16; the halves of a row start with different ones: the eight lanes of a phase then write
+          // to different banks
+          const int swap = rows.ch >> 2;
+          const uint32_t d0 = dst + swap * PT_HALF + (((2 * rows.ch + swap) & 7) << 4), d1 = dst + swap * PT_HALF + (((2 * rows.ch + 1 - swap) & 7) << 4);
+          uint2 x[Rows::RPT], y[Rows::RPT];
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-              if (blk * PT_KB + lrow + i * RSTEP >= base) hit |= clean(x[i]);
+          for (int i = 0; i < Rows::RPT; ++i) {
+            x[i] = pt_lds8(src + i * 2048 + swap * 8);
+            y[i] = pt_lds8(src + i * 2048 + 8 - swap * 8);
+          }
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            uint4 lo, hi;
-            pd_cvt4(x[i].x, lo.x, lo.y);
-            pd_cvt4(x[i].y, lo.z, lo.w);
-            pd_cvt4(x[i].z, hi.x, hi.y);
-            pd_cvt4(x[i].w, hi.z, hi.w);
-            pt_sts(d0 + i * RSTEP * 128, swap ? hi : lo);
-            pt_sts(d1 + i * RSTEP * 128, swap ? lo : hi);
+          for (int i = 0; i < Rows::RPT; ++i) {
+            uint4 a0, a1;
+            pd_cvt4(x[i].x, a0.x, a0.y);
+            pd_cvt4(x[i].y, a0.z, a0.w);
+            pd_cvt4(y[i].x, a1.x, a1.y);
+            pd_cvt4(y[i].y, a1.z, a1.w);
+            pt_sts((d0 ^ ((i & 7) << 4)) + i * 128, a0);
+            pt_sts((d1 ^ ((i & 7) << 4)) + i * 128, a1);
           }
         } else if (window) {
-          for (int i = 0; i < N; ++i) {
-            const uint32_t p = dst + pt_at(lrow, lch) + i * RSTEP * 128;
-            uint4 x = pt_lds(p);
-            if (blk * PT_KB + lrow + i * RSTEP >= base && clean(x)) { pt_sts(p, x); hit = true; }
-          }
+#pragma unroll 1
+          for (int i = 0; i < Rows::RPT; ++i)
+            if (key + i >= base) {
+              const uint32_t p = ((dst + (rows.ch >> 3) * PT_HALF + ((rows.ch & 7) << 4)) ^ ((i & 7) << 4)) + i * 128;
+              uint4 x = pt_lds(p);
+              if (pt_clean<false>(x)) { pt_sts(p, x); hit = true; }
+            }
         }
         if (hit) *reinterpret_cast<volatile int*>(&sh.odd) = 1;
         fence_proxy_async_smem();
-        mbar_arrive((n & 1) ? &sh.v_full[g & 1] : &sh.k_full[g & 1]);
+        mbar_arrive(&sh.v_full[g & 1]);
       };
-      lookup(blk0);
-      if constexpr (KV8) {
-        issue(0);
-        issue(1);
-        for (int n = 0; n < nb; ++n) {
+      // e4m3: the bytes of block n + 2 are on their way while block n is converted; bf16: the rows of block n while block n - 1 is handed over
+      constexpr int AHEAD = KV8 ? 2 : 0, LAG = KV8 ? 0 : 1;
+#pragma unroll 1
+      for (int n = -AHEAD; n < nb + LAG; ++n) {
+        if (!KV8 && n < nb) wait_empty(n);
+        const int f = n - LAG;
+        if (KV8 && f >= 0) {
           if (n + 1 < nb) asm volatile("cp.async.wait_group 1;" ::: "memory");
           else asm volatile("cp.async.wait_group 0;" ::: "memory");
-          wait_empty(n);
-          finish(n);
-          if (n + 2 < nb) issue(n + 2);
+          wait_empty(f);
+          finish(f);
         }
-      } else {
-        for (int n = 0; n < nb; ++n) {
-          wait_empty(n);
-          issue(n);
-          if (n > 0) {
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            finish(n - 1);
-          }
+        if (n + AHEAD < nb) {
+          if constexpr (KV8) rows.template issue<false>(smem_u32(raw) + ((n + AHEAD) & 1) * PT_RAW + lt * 16, c.n_pages);
+          else rows.template issue<true>(smem_u32(sv) + ((gk + n) & 1) * PT_TILE, c.n_pages);
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        finish(nb - 1);
+        if (!KV8 && f >= 0) {
+          if (n < nb) asm volatile("cp.async.wait_group 1;" ::: "memory");
+          else asm volatile("cp.async.wait_group 0;" ::: "memory");
+          finish(f);
+        }
       }
-      gk += nb >> 1;
+      gk += nb;
     }
   } else {
-    pt_regs_dec<PT_REGS_MMA>();
+    if (warp >= PT_MMA_WARP + 2) {
+      // =============================== K and the page scales ==============================================================================
+      constexpr int LAG = KS / 2;              // blocks under way
+      const int lt = tid - (PT_MMA_WARP + 2) * 32;
+      PtRows<KV8, 64> rows(c, lt, psh);
+      unsigned gk = 0;
+      while (const PtSeg* gp = next_seg()) {
+        const int nb = gp->blk1 - gp->blk0, kvh = gp->kvh, first = gp->blk0 * PT_KB;
+        rows.start(c, c.k, *gp);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
+        ++n_seg;
+        // lane i (0 .. 7) of warp 14 looks after the scales of the block's 16 keys i
+        float ks = 1.f, vs = 1.f;
+        auto page_at = [&](int n) {
+          const int key = first + n * PT_KB + (lane & 7) * 16;
+          return key < rows.end ? __ldg(rows.table + (key >> psh)) : 0;
+        };
+        int pg_next = page_at(0);
+        auto load_scales = [&](int n) {
+          const int key = first + n * PT_KB + (lane & 7) * 16, pg = pg_next;
+          pg_next = page_at(n + 1);
+          ks = vs = 1.f;
+          if (key < rows.end) {
+            if (static_cast<unsigned>(pg) >= static_cast<unsigned>(c.n_pages)) {
+              ks = -1.f;
+            } else if (KV8) {
+              ks = fmaxf(__ldg(c.k_scale + static_cast<size_t>(pg) * c.nkv + kvh), 1e-30f);      // (0 would turn a masked -inf into NaN)
+              vs = __ldg(c.v_scale + static_cast<size_t>(pg) * c.nkv + kvh);
+            }
+          }
+        };
+        auto store_scales = [&](int n) {
+          const unsigned any = __ballot_sync(0xffffffffu, ks < 0.f);
+          const float ev = KV8 ? pd_log2_scale(vs) : 0.f;
+          if (lane < 8) sc[((gk + n) % PT_SC) * 8 + lane] = make_float4(ks, ev, KV8 ? pd_ex2(-ev) : 1.f, any ? 1.f : 0.f);
+          if (any && lane == 0) set_error(c.err, ERR_BAD_ARGS);
+        };
+        auto finish = [&](int n) {
+          fence_proxy_async_smem();
+          mbar_arrive(&sh.k_full[(gk + n) % KS]);
+        };
+#pragma unroll 1
+        for (int n = 0; n < nb + LAG; ++n) {
+          const unsigned g = gk + n;
+          if (n < nb) {
+            if (g >= KS && ok) ok = tc_wait(&sh.k_empty[g % KS], ((g / KS) & 1u) ^ 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
+            rows.template issue<true>(smem_u32(sk) + (g % KS) * K_BYTES, c.n_pages);
+          } else {
+            asm volatile("cp.async.commit_group;" ::: "memory");       // (an empty group: the count below stays the same)
+          }
+          if (warp == PT_MMA_WARP + 2) {
+            if (n > 0 && n <= nb) store_scales(n - 1);
+            if (n < nb) load_scales(n);
+          }
+          if (n >= LAG) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
+            finish(n - LAG);
+          }
+        }
+        gk += nb;
+      }
+    } else
     if (warp == PT_MMA_WARP && lane == 0) {
     // =============================== MMA issuer =========================================================================================
     constexpr uint32_t idesc = (1u << 4) | (KV8 ? 0u : ((1u << 7) | (1u << 10))) | (static_cast<uint32_t>(PT_KB >> 3) << 17) | (static_cast<uint32_t>(PT_M >> 4) << 24);
     constexpr uint32_t idesc_v = idesc | (1u << 16);                   // V: MN-major
+    const uint32_t q_lo = pt_lo_k(smem_u32(sq)), k_lo = pt_lo_k(smem_u32(sk)), v_lo = pt_lo_mn(smem_u32(sv));
     auto qk = [&](int w, unsigned gk) {
       tc_fence_after();
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        tc_mma<1>(tmem + w * 128, smem_desc_sw128(sq + w * PT_TILE + (k >> 2) * PT_HALF) + 2 * (k & 3),
-                  smem_desc_sw128(sk + (gk & 1) * PT_TILE + (k >> 2) * PT_HALF) + 2 * (k & 3), idesc, k > 0);
+      pt_mma8<KV8 ? PT_QK8 : PT_QK16>(tmem + w * 128, q_lo + w * (PT_TILE >> 4), k_lo + (gk % KS) * (K_BYTES >> 4), idesc, 0);
       tc_commit(&sh.s_full[w]);
+      mbar_arrive(&sh.s_full[w]);              // hands on what the loader wrote beside the tile (the wait on k_full came before)
     };
     auto pv = [&](int w, unsigned gk, bool first) {
       tc_fence_after();
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        pt_mma_ts(tmem + 256 + w * 128, tmem + w * 128 + k * 8, pt_desc_mn(sv + (gk & 1) * PT_TILE) + k * (2048 >> 4), idesc_v, !first || k > 0);
+      pt_mma8<PT_PV>(tmem + 256 + w * 128, tmem + w * 128, v_lo + (gk & 1) * (PT_TILE >> 4), idesc_v, !first);
       tc_commit(&sh.pv_done[w]);
     };
-    unsigned gk = 0, n_p[2] = {0, 0};
-    auto full = [&](uint64_t* bar, unsigned g) { return tc_wait(&bar[g & 1], (g >> 1) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT); };
+    unsigned gk = 0, n_p = 0;                  // blocks so far; bit w: phase of p_ready[w]
+    auto full_k = [&](unsigned g) { return tc_wait(&sh.k_full[g % KS], (g / KS) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT); };
+    auto full_v = [&](unsigned g) { return tc_wait(&sh.v_full[g & 1], (g >> 1) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT); };
     while (const PtSeg* gp = ok ? next_seg() : nullptr) {
       const PtSeg& sg = *gp;
       const int nb = sg.blk1 - sg.blk0, ahead = sg.rows > PT_M ? 1 : 2;   // pair: both groups take block j; else group j & 1 does
       ok = tc_wait(&sh.q_full[0], n_seg & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT) &&
            tc_wait(&sh.q_full[1], n_seg & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
-      for (int j = 0; j < min(ahead, nb) && ok; ++j) {
-        ok = full(sh.k_full, gk + j);
-        if (!ok) break;
-        qk(j, gk + j);
-        if (ahead == 1) qk(1, gk + j);
-        tc_commit(&sh.k_empty[(gk + j) & 1]);
-      }
-      for (int j = 0; j < nb && ok; ++j, ++gk) {
-        ok = full(sh.v_full, gk);
-        for (int w = ahead == 1 ? 0 : (j & 1); ok && w < (ahead == 1 ? 2 : (j & 1) + 1); ++w) {
-          const bool last = ahead == 2 || w == 1;
-          ok = tc_wait(&sh.p_ready[w], n_p[w] & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+      // step i: O += P V of block j - ahead, then S of block j, for group w (one instance of either product: code that is rarely run is fetched
+      // from far, and the other warps' code is large)
+      const int steps = ahead == 1 ? 2 * (nb + 1) : nb + 2;
+#pragma unroll 1
+      for (int i = 0; i < steps && ok; ++i) {
+        const int j = ahead == 1 ? i >> 1 : i, w = i & 1, jp = j - ahead;
+        const bool opens = ahead == 2 || w == 0, closes = ahead == 2 || w == 1;     // the block's first / last use
+        if (jp >= 0 && jp < nb) {
+          if (opens) ok = full_v(gk + jp);
+          if (ok) ok = tc_wait(&sh.p_ready[w], (n_p >> w) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
           if (!ok) break;
-          ++n_p[w];
-          pv(w, gk, j < ahead);
-          if (last) tc_commit(&sh.v_empty[gk & 1]);
-          if (j + ahead < nb) {
-            if (ahead == 2 || w == 0) ok = full(sh.k_full, gk + ahead);
-            if (!ok) break;
-            qk(w, gk + ahead);
-            if (last) tc_commit(&sh.k_empty[(gk + ahead) & 1]);
-          }
+          n_p ^= 1u << w;
+          pv(w, gk + jp, jp < ahead);
+          if (closes) tc_commit(&sh.v_empty[(gk + jp) & 1]);
+        }
+        if (j < nb) {
+          if (opens) ok = full_k(gk + j);
+          if (!ok) break;
+          qk(w, gk + j);
+          if (closes) tc_commit(&sh.k_empty[(gk + j) % KS]);
         }
       }
+      gk += nb;
       tc_commit(&sh.q_free);
       mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
       ++n_seg;
@@ -901,11 +1023,7 @@ size_t paged_tiles_scratch(const IhbPagedAttn& a) {
 template <bool KV8>
 static cudaError_t pt_launch(const IhbPagedAttn& a, cudaStream_t stream) {
   const int grid = PT_MAX_GRID, rec_rows = pt_rec_rows(a);             // one CTA per SM
-  static const int regs = [] {                 // the register split draws on what the block is launched with
-    cudaFuncAttributes f;
-    return cudaFuncGetAttributes(&f, paged_tiles_kernel<KV8>) == cudaSuccess ? f.numRegs : 0;
-  }();
-  if (regs < PT_REGS) return cudaErrorInvalidConfiguration;
+  static_assert(sizeof(PtHdr) <= 1024, "header");
   constexpr int bytes = pt_smem<KV8>();
   cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
