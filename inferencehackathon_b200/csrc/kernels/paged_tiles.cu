@@ -38,7 +38,7 @@ constexpr int PT_SEGS = 4;
 // A piece of an item: rows [row0, row0 + rows) of a sequence's KV head, key blocks [blk0, blk1) of nblk.
 struct PtSeg {
   int b, kvh, row0, rows, blk0, blk1, nblk, first_in_range;
-  int seen_end;                                // keys that any of the rows sees lie below it
+  int seen_end, all_see;                       // keys that any of the rows sees lie below the one, keys below the other are seen by all of them
   PgSeq s;
   int last;                                    // no segment: the end
 };
@@ -49,10 +49,10 @@ constexpr int PT_SC = 8;                       // blocks whose page scales are k
 
 struct PtHdr {
   uint64_t k_full[4], k_empty[4], v_full[2], v_empty[2];
-  uint64_t q_full[2], q_free, s_full[2], p_ready[2], pv_done[2], hand[2];
+  uint64_t q_full[2], q_free, s_full[2], p_ready[4], pv_done[4], hand[2];
   uint32_t tmem;
   int abort_flag;
-  int odd;                                     // V rows of the call's own tokens that are not finite were seen (set by the loader)
+  int odd;                                     // V values that are not finite were met in keys that not every row sees (set by the loader)
   uint64_t seg_full[PT_SEGS], seg_free[PT_SEGS];
   PtSeg seg[PT_SEGS];
 };
@@ -128,6 +128,7 @@ struct PtIter {
       g.rows = min(RT, s.n * G - g.row0);
       const int i_last = (g.row0 + g.rows - 1) / G;
       g.seen_end = p.mask != nullptr ? s.len : min(s.len, s.base + i_last + 1);
+      g.all_see = max(0, p.mask != nullptr ? s.base : min(s.base + g.row0 / G + 1, s.len));
       g.nblk = max(1, (g.seen_end + PT_KB - 1) / PT_KB);
       g.blk0 = static_cast<int>(v0 * g.nblk / len);
       g.blk1 = static_cast<int>(v1 * g.nblk / len);
@@ -161,14 +162,14 @@ __device__ __forceinline__ void pt_ld32(uint32_t t, float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void pt_st32(uint32_t t, const float (&v)[32]) {
+__device__ __forceinline__ void pt_st32(uint32_t t, const unsigned (&v)[32]) {
   __syncwarp();
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
       "%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
-      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]),
-      "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]),
-      "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+      "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
+      "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
 }
 __device__ __forceinline__ void pt_st16(uint32_t t, const unsigned (&v)[16]) {
@@ -180,7 +181,7 @@ __device__ __forceinline__ void pt_st16(uint32_t t, const unsigned (&v)[16]) {
       : "memory");
 }
 __device__ __forceinline__ void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// Eight products, D[tmem] (+)= A B. PT_QK16: 16 channels each, both operands in shared memory (K-major, two swizzled halves); PT_QK8: e4m3, 32
+// Eight products (PT_PV: four), D[tmem] (+)= A B. PT_QK16: 16 channels each, both operands in shared memory (K-major, two swizzled halves); PT_QK8: e4m3, 32
 // channels each, first Q's heads, then its remainders (a half further on) with the same K; PT_PV: 16 keys each, A in tensor memory (8
 // columns per step), B in shared memory, MN-major. The issuing thread shares its scheduler with softmax warps, so the descriptors'
 // high words are constants and a step costs one or two additions.
@@ -194,11 +195,7 @@ __device__ __forceinline__ void pt_mma8(uint32_t d, uint32_t a, uint32_t b_lo, u
         "mov.b64 b, {%2, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t"
         "add.u32 x, %1, 8;\n\tadd.u32 y, %2, 128;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
         "add.u32 x, %1, 16;\n\tadd.u32 y, %2, 256;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
-        "add.u32 x, %1, 24;\n\tadd.u32 y, %2, 384;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
-        "add.u32 x, %1, 32;\n\tadd.u32 y, %2, 512;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
-        "add.u32 x, %1, 40;\n\tadd.u32 y, %2, 640;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
-        "add.u32 x, %1, 48;\n\tadd.u32 y, %2, 768;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t"
-        "add.u32 x, %1, 56;\n\tadd.u32 y, %2, 896;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t}"
+        "add.u32 x, %1, 24;\n\tadd.u32 y, %2, 384;\n\tmov.b64 b, {y, %5};\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %3, 1;\n\t}"
         ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(acc), "n"(0x40004040)
         : "memory");
   else if constexpr (KIND == PT_QK8)
@@ -383,7 +380,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       mbar_init(&sh.k_empty[2 * i], 1); mbar_init(&sh.k_empty[2 * i + 1], 1);
       mbar_init(&sh.v_full[i], 128); mbar_init(&sh.v_empty[i], 1);
       mbar_init(&sh.q_full[i], 128); mbar_init(&sh.s_full[i], 2);
-      mbar_init(&sh.p_ready[i], 128); mbar_init(&sh.pv_done[i], 1);
+      mbar_init(&sh.p_ready[2 * i], 128); mbar_init(&sh.p_ready[2 * i + 1], 128); mbar_init(&sh.pv_done[2 * i], 1); mbar_init(&sh.pv_done[2 * i + 1], 1);
     }
     mbar_init(&sh.q_free, 1);
     mbar_init(&sh.hand[0], 128);
@@ -514,87 +511,81 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             seen[q] = w;
           }
         }
-        // ---- maximum. Both passes read the scores from tensor memory, 32 at a time, in short loops: unrolled over the row's 128 scores the
-        // kernel's hot code is several times the first instruction cache, and every warp of the SM pays for it ----
-        float mx = -INFINITY;
+        // Half a block at a time, against the maximum so far: the probabilities are formed and held while this half's own maximum is
+        // found; only when it is more than 2^8 above (the first keys, and rarely later) the accumulators are rescaled and the half is done
+        // again. No pass for the maximum alone, and the first half's product with V runs under the second half's exponentials. The
+        // loops stay short: unrolled over the row's 128 scores the hot code is several times the first instruction cache, and every
+        // warp of the SM pays for it.
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          float v[32];
-          pt_ld32(t_s + q * 32, v);
-          if (edge) pt_mask32(v, q < 2 ? (q ? seen[1] : seen[0]) : (q == 2 ? seen[2] : seen[3]));
+        for (int hf = 0; hf < 2; ++hf) {
+          unsigned pk[32];
+          float sum;
+          for (int turn = 0;; ++turn) {        // (a third turn would only come from scores beyond fp32's whole numbers)
+            float mx = -INFINITY;
+            const float mo = OFF - (m == -INFINITY ? 0.f : m);
+            sum = 0.f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x = pt_max3(v[h * 16], v[h * 16 + 1], v[h * 16 + 2]);
+            for (int q = 0; q < 2; ++q) {
+              float v[32];
+              pt_ld32(t_s + hf * 64 + q * 32, v);
+              if (edge) pt_mask32(v, hf ? (q ? seen[3] : seen[2]) : (q ? seen[1] : seen[0]));
 #pragma unroll
-            for (int e = 3; e < 15; e += 2) x = pt_max3(x, v[h * 16 + e], v[h * 16 + e + 1]);
-            x = fmaxf(x, v[h * 16 + 15]);
-            if (KV8) {
-              const float2 ke = *reinterpret_cast<const float2*>(&sb[2 * q + h]);
-              mx = fmaxf(mx, fmaf(x, fabsf(ke.x) * rowf, ke.y));
-            } else {
-              mx = fmaxf(mx, x);
+              for (int h = 0; h < 2; ++h) {
+                float4 ke = make_float4(1.f, 0.f, 1.f, 0.f);
+                if (KV8) ke = sb[hf * 4 + 2 * q + h];
+                const float f = KV8 ? fabsf(ke.x) * rowf : rowf, add = KV8 ? ke.y + mo : mo;
+                const uint64_t f2 = pt_pair(f, f), add2 = pt_pair(add, add);
+                uint64_t s2 = 0;               // (0.f, 0.f)
+                float x = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                  float p0, p1;
+                  pt_unpair(pt_fma2(pt_pair(v[h * 16 + e], v[h * 16 + e + 1]), f2, add2), p0, p1);    // a masked score stays -inf: f > 0
+                  x = pt_max3(x, p0, p1);
+                  p0 = pd_ex2(p0);
+                  p1 = pd_ex2(p1);
+                  s2 = pt_add2(s2, pt_pair(p0, p1));
+                  pk[q * 16 + h * 8 + e / 2] = pd_pack<KV8>(p0, p1);
+                }
+                mx = fmaxf(mx, x);
+                float s0, s1;
+                pt_unpair(s2, s0, s1);
+                sum += KV8 ? (s0 + s1) * ke.z : s0 + s1;
+              }
+            }
+            mx -= mo;                          // this half's maximum of score + log2 of the V scale
+            const bool grow = m == -INFINITY ? mx > -INFINITY : mx > m + PD_LAZY;
+            if (!__any_sync(0xffffffffu, grow) || turn == 2) break;
+            const float mn = fmaxf(m, mx), r = m == -INFINITY ? 0.f : pd_ex2(m - mn);
+            m = mn;
+            l *= r;
+            if (have) {
+              // the last product with V: the other half's, of this block or of the one before (a barrier per half: a wait must not lag two phases)
+              if (ok) ok = tc_wait(&sh.pv_done[2 * wg + (hf ^ 1)], (n_blk - 1 + hf) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+              tc_fence_after();
+#pragma unroll 1
+              for (int q = 0; q < 8; ++q) {
+                float x[16];
+                __syncwarp();
+                tmem_ld16(t_o + q * 16, x);
+                unsigned y[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(x[e] * r);
+                pt_st16(t_o + q * 16, y);
+              }
             }
           }
+          l += sum;
+          have = true;
+          pt_st32(t_s + hf * 32, pk);          // in the place of scores that have been read
+          pt_wait_st();
+          tc_fence_before();
+          mbar_arrive(&sh.p_ready[2 * wg + hf]);         // (a barrier per half: both may be through before the issuer looks)
         }
-        if (!KV8) mx *= rowf;
-        // ---- rescale when the maximum has grown enough ----
-        if (__any_sync(0xffffffffu, mx > m + PD_LAZY)) {
-          const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : pd_ex2(m - mn);
-          m = mn;
-          l *= f;
-          if (have) {
-            if (ok) ok = tc_wait(&sh.pv_done[wg], (n_blk - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
-            tc_fence_after();
-#pragma unroll 1
-            for (int q = 0; q < 8; ++q) {
-              float x[16];
-              __syncwarp();
-              tmem_ld16(t_o + q * 16, x);
-              unsigned y[16];
-#pragma unroll
-              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(x[e] * f);
-              pt_st16(t_o + q * 16, y);
-            }
-          }
-        }
-        have = true;
-        // ---- probabilities, in the place of the scores ----
-        const float mo = OFF - (m == -INFINITY ? 0.f : m);
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          float v[32];
-          pt_ld32(t_s + q * 32, v);
-          if (edge) pt_mask32(v, q < 2 ? (q ? seen[1] : seen[0]) : (q == 2 ? seen[2] : seen[3]));
-          unsigned pk[16];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float4 ke = make_float4(1.f, 0.f, 1.f, 0.f);
-            if (KV8) ke = sb[2 * q + h];
-            const float f = KV8 ? fabsf(ke.x) * rowf : rowf, add = KV8 ? ke.y + mo : mo;
-            const uint64_t f2 = pt_pair(f, f), add2 = pt_pair(add, add);
-            uint64_t sum = 0;                  // (0.f, 0.f)
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              float p0, p1;
-              pt_unpair(pt_fma2(pt_pair(v[h * 16 + e], v[h * 16 + e + 1]), f2, add2), p0, p1);      // a masked score stays -inf: f > 0
-              p0 = pd_ex2(p0);
-              p1 = pd_ex2(p1);
-              sum = pt_add2(sum, pt_pair(p0, p1));
-              pk[h * 8 + e / 2] = pd_pack<KV8>(p0, p1);
-            }
-            float s0, s1;
-            pt_unpair(sum, s0, s1);
-            l += KV8 ? (s0 + s1) * ke.z : s0 + s1;
-          }
-          pt_st16(t_s + q * 16, pk);           // (the scores that these columns held have been read)
-        }
-        pt_wait_st();
-        tc_fence_before();
-        mbar_arrive(&sh.p_ready[wg]);
         ++n_blk;
       }
       // ---- the result ----
-      if (have && ok) ok = tc_wait(&sh.pv_done[wg], (n_blk - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+      if (have && ok) ok = tc_wait(&sh.pv_done[2 * wg + 1], (n_blk - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
       tc_fence_after();
       float f0 = 1.f, f1 = 0.f;
       const uint32_t xs = smem_u32(sq) + r_tile * 512;                   // the row's place
@@ -649,7 +640,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             for (int e = 0; e < 32; ++e) v[e] *= f0;
           }
           if (odd && live)                     // values that are not finite, left out of the products: added where they are seen
-            for (int key = max(max(s.base, 0), sg.blk0 * PT_KB); key < min(sg.seen_end, sg.blk1 * PT_KB); ++key) {
+            for (int key = max(sg.all_see, sg.blk0 * PT_KB); key < min(sg.seen_end, sg.blk1 * PT_KB); ++key) {
               const int pg = table[key >> psh];
               if (!pt_sees(a, s, mrow, vis, key) || static_cast<unsigned>(pg) >= static_cast<unsigned>(c.n_pages)) continue;
               const size_t row = (static_cast<size_t>(pg) * c.nkv + sg.kvh) * c.page + (key & (c.page - 1));
@@ -701,7 +692,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
     Rows rows(c, lt, psh);
     unsigned gk = 0;                           // blocks so far
     while (const PtSeg* gp = next_seg()) {
-      const int nb = gp->blk1 - gp->blk0, base = gp->s.base, first = gp->blk0 * PT_KB;
+      const int nb = gp->blk1 - gp->blk0, all_see = gp->all_see, first = gp->blk0 * PT_KB;
       rows.start(c, c.v, *gp);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
@@ -714,15 +705,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         const unsigned g = gk + n;
         const int r0 = rows.grp * 16 + rows.row, key = first + n * PT_KB + r0;
         const uint32_t dst = smem_u32(sv) + (g & 1) * PT_TILE + r0 * 128;
-        // rows of the call's own tokens, which not every row sees: what is not finite is taken out here and added where it is seen
-        const bool window = first + n * PT_KB + PT_KB > base;
+        // keys that not every row sees: what is not finite is taken out here and added where it is seen
+        const bool window = first + n * PT_KB + PT_KB > all_see;
         bool hit = false;
         if constexpr (KV8) {
           const uint32_t src = smem_u32(raw) + (n & 1) * PT_RAW + lt * 16;
           if (window)
 #pragma unroll 1
             for (int i = 0; i < Rows::RPT; ++i)
-              if (key + i >= base) {
+              if (key + i >= all_see) {
                 uint4 x = pt_lds(src + i * 2048);
                 if (pt_clean<true>(x)) { pt_sts(src + i * 2048, x); hit = true; }
               }
@@ -749,7 +740,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         } else if (window) {
 #pragma unroll 1
           for (int i = 0; i < Rows::RPT; ++i)
-            if (key + i >= base) {
+            if (key + i >= all_see) {
               const uint32_t p = ((dst + (rows.ch >> 3) * PT_HALF + ((rows.ch & 7) << 4)) ^ ((i & 7) << 4)) + i * 128;
               uint4 x = pt_lds(p);
               if (pt_clean<false>(x)) { pt_sts(p, x); hit = true; }
@@ -858,12 +849,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       tc_commit(&sh.s_full[w]);
       mbar_arrive(&sh.s_full[w]);              // hands on what the loader wrote beside the tile (the wait on k_full came before)
     };
-    auto pv = [&](int w, unsigned gk, bool first) {
+    auto pv = [&](int w, unsigned gk, int hf, bool first) {
       tc_fence_after();
-      pt_mma8<PT_PV>(tmem + 256 + w * 128, tmem + w * 128, v_lo + (gk & 1) * (PT_TILE >> 4), idesc_v, !first);
-      tc_commit(&sh.pv_done[w]);
+      pt_mma8<PT_PV>(tmem + 256 + w * 128, tmem + w * 128 + hf * 32, v_lo + (gk & 1) * (PT_TILE >> 4) + hf * 512, idesc_v, !first);
+      tc_commit(&sh.pv_done[2 * w + hf]);
     };
-    unsigned gk = 0, n_p = 0;                  // blocks so far; bit w: phase of p_ready[w]
+    unsigned gk = 0, n_p = 0;                  // blocks so far; bit w: phase of group w's p_ready
     auto full_k = [&](unsigned g) { return tc_wait(&sh.k_full[g % KS], (g / KS) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT); };
     auto full_v = [&](unsigned g) { return tc_wait(&sh.v_full[g & 1], (g >> 1) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT); };
     while (const PtSeg* gp = ok ? next_seg() : nullptr) {
@@ -880,10 +871,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         const bool opens = ahead == 2 || w == 0, closes = ahead == 2 || w == 1;     // the block's first / last use
         if (jp >= 0 && jp < nb) {
           if (opens) ok = full_v(gk + jp);
-          if (ok) ok = tc_wait(&sh.p_ready[w], (n_p >> w) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+#pragma unroll 1
+          for (int hf = 0; hf < 2 && ok; ++hf) {
+            ok = tc_wait(&sh.p_ready[2 * w + hf], (n_p >> w) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+            if (ok) pv(w, gk + jp, hf, jp < ahead && hf == 0);
+          }
           if (!ok) break;
           n_p ^= 1u << w;
-          pv(w, gk + jp, jp < ahead);
           if (closes) tc_commit(&sh.v_empty[(gk + jp) & 1]);
         }
         if (j < nb) {
