@@ -86,7 +86,7 @@ __device__ __forceinline__ void pd_cvt4(unsigned w, unsigned& lo, unsigned& hi) 
 }
 __device__ __forceinline__ float pd_ex2(float x) {
   float y;
-  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 // log2 of a page scale inside the range that append writes (a scale of 0 reads as the least one): the exponent from the bits, exact

@@ -8,7 +8,7 @@
 //   warps 8-11       bring V: page lookups, 16-byte asynchronous copies, e4m3 -> fp16 on the way into the swizzled tile
 //   warps 14, 15     bring K, and the page scales. e4m3 K needs no conversion: a bf16 query row, scaled by a power of two, is the sum of two
 //                    e4m3 rows (8 significant bits: 4 + 4), so S = Qhi K^T + Qlo K^T runs on e4m3 products, which are twice as fast
-//   warp 13          lays out the segments; warp 12 issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as an MN-major operand: the
+//   warps 12, 13     one issuer per tile (waits, fences and commits cost it more than the products' issue): S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as an MN-major operand: the
 //                    rows of the cache are used as they lie, no transpose)
 // While one group computes its softmax the tensor cores work for the other. A sequence with at most 128 rows gives both groups the
 // same rows: they take the even and the odd key blocks, and their results are added up at the end.
@@ -25,6 +25,10 @@ namespace ihb {
 constexpr int PT_M = 128, PT_KB = 128;
 constexpr int PT_THREADS = 512;
 constexpr int PT_MMA_WARP = 12;
+// Registers: 512 threads start with 128 each (all of the SM's); the others' groups give some to the softmax groups, where half a row's
+// scores, the probabilities and what the scheduler wants to overlap do not fit 128 (measured: 3 %).
+constexpr int PT_REGS = 128, PT_REGS_SOFTMAX = 168, PT_REGS_LOAD = 96, PT_REGS_MMA = 80;
+static_assert(256 * PT_REGS_SOFTMAX + 128 * PT_REGS_LOAD + 128 * PT_REGS_MMA <= PT_THREADS * PT_REGS, "more registers than the block has");
 constexpr int PT_HALF = 16384;                 // 128 rows x 128 bytes: one swizzled half (64 channels) of a tile
 constexpr int PT_TILE = 2 * PT_HALF;
 constexpr int PT_HDR = 3072;                   // barriers and segments; m and l of the second group at 1024 and 1536; page scales at 2048
@@ -48,8 +52,8 @@ constexpr int pt_k_stages() { return KV8 ? 4 : 2; }             // of 16 / 32 KB
 constexpr int PT_SC = 8;                       // blocks whose page scales are kept: more than are ever under way
 
 struct PtHdr {
-  uint64_t k_full[4], k_empty[4], v_full[2], v_empty[2];
-  uint64_t q_full[2], q_free, s_full[2], p_ready[4], pv_done[4], hand[2];
+  uint64_t k_full[4], k_empty[2][4], v_full[2], v_empty[2][2];         // empty: [group that used it][stage]
+  uint64_t q_full[2], q_free, s_full[2], p_ready[4], pv_done[4], hand[2], stagger[2];
   uint32_t tmem;
   int abort_flag;
   int odd;                                     // V values that are not finite were met in keys that not every row sees (set by the loader)
@@ -162,6 +166,27 @@ __device__ __forceinline__ void pt_ld32(uint32_t t, float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+// Loads that are waited for later: pt_ld32_issue, pt_wait_ld, pt_pin (ties the registers' first use to the wait).
+__device__ __forceinline__ void pt_ld32_issue(uint32_t t, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,"
+      "%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]),
+        "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]),
+        "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(t)
+      : "memory");
+}
+__device__ __forceinline__ void pt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pt_pin(float* v) {
+  asm volatile(""
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]),
+                 "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]),
+                 "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]),
+                 "+f"(v[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void pt_st32(uint32_t t, const unsigned (&v)[32]) {
   __syncwarp();
   asm volatile(
@@ -181,6 +206,10 @@ __device__ __forceinline__ void pt_st16(uint32_t t, const unsigned (&v)[16]) {
       : "memory");
 }
 __device__ __forceinline__ void pt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void pt_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void pt_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // Eight products (PT_PV: four), D[tmem] (+)= A B. PT_QK16: 16 channels each, both operands in shared memory (K-major, two swizzled halves); PT_QK8: e4m3, 32
 // channels each, first Q's heads, then its remainders (a half further on) with the same K; PT_PV: 16 keys each, A in tensor memory (8
 // columns per step), B in shared memory, MN-major. The issuing thread shares its scheduler with softmax warps, so the descriptors'
@@ -325,6 +354,24 @@ __device__ __noinline__ bool pt_clean(uint4& y) {
   y = make_uint4(x[0], x[1], x[2], x[3]);
   return bad;
 }
+// Bounded wait on a phase of an mbarrier; gives up when another role has. The clock is read only after a while of polling: the first
+// read would cost more than most waits.
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned* err, unsigned code) {
+  unsigned long long t0 = 0;
+  for (unsigned spins = 1; !mbar_try_wait(bar, parity); ++spins) {
+    if ((spins & 255u) == 0u) {
+      if (*abort_flag) return false;
+      const unsigned long long t = globaltimer_ns();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > IHB_LOCAL_WAIT_NS) {
+        *abort_flag = 1;
+        set_error(err, code);
+        return false;
+      }
+    }
+  }
+  return true;
+}
 // Shared memory by 32-bit address: the aligned base is a computed pointer, which the compiler would access as generic memory.
 __device__ __forceinline__ uint4 pt_lds(uint32_t a) {
   uint4 v;
@@ -336,6 +383,7 @@ __device__ __forceinline__ uint2 pt_lds8(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
+__device__ __forceinline__ void pt_sts8(uint32_t a, uint2 v) { asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(a), "r"(v.x), "r"(v.y) : "memory"); }
 __device__ __forceinline__ void pt_sts(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -377,15 +425,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.k_full[2 * i], 64); mbar_init(&sh.k_full[2 * i + 1], 64);
-      mbar_init(&sh.k_empty[2 * i], 1); mbar_init(&sh.k_empty[2 * i + 1], 1);
-      mbar_init(&sh.v_full[i], 128); mbar_init(&sh.v_empty[i], 1);
+      for (int j = 0; j < 4; ++j) mbar_init(&sh.k_empty[i][j], 1);
+      for (int j = 0; j < 2; ++j) mbar_init(&sh.v_empty[i][j], 1);
+      mbar_init(&sh.v_full[i], 128);
       mbar_init(&sh.q_full[i], 128); mbar_init(&sh.s_full[i], 2);
       mbar_init(&sh.p_ready[2 * i], 128); mbar_init(&sh.p_ready[2 * i + 1], 128); mbar_init(&sh.pv_done[2 * i], 1); mbar_init(&sh.pv_done[2 * i + 1], 1);
     }
-    mbar_init(&sh.q_free, 1);
+    mbar_init(&sh.q_free, 2);
+    mbar_init(&sh.stagger[0], 1);
+    mbar_init(&sh.stagger[1], 1);
     mbar_init(&sh.hand[0], 128);
     mbar_init(&sh.hand[1], 128);
-    for (int i = 0; i < PT_SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_free[i], 15); }
+    for (int i = 0; i < PT_SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_free[i], 16); }
     sh.abort_flag = 0;
     sh.odd = 0;
     fence_mbar_init();
@@ -412,13 +463,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
   // The next segment: every role reads the scheduler's records in order, and gives a record back (free_seg) when done with it.
   unsigned n_seg = 0;
   auto next_seg = [&]() -> const PtSeg* {
-    if (!tc_wait(&sh.seg_full[n_seg % PT_SEGS], (n_seg / PT_SEGS) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT)) return nullptr;
+    if (!pt_wait(&sh.seg_full[n_seg % PT_SEGS], (n_seg / PT_SEGS) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT)) return nullptr;
     const PtSeg* g = &sh.seg[n_seg % PT_SEGS];
     return g->last ? nullptr : g;
   };
   bool ok = true;
 
   if (warp < 8) {
+    pt_regs_inc<PT_REGS_SOFTMAX>();
     // =============================== softmax groups ===============================================================================
     const int wg = warp >> 2, quarter = warp & 3, r_tile = quarter * 32 + lane;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -436,50 +488,56 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       const int vis = !live ? max(sg.seen_end, 0) : (a.mask != nullptr ? max(s.base, 0) : min(max(s.base + tok + 1, 0), s.len));   // keys [0, vis) are seen
       const unsigned char* mrow = a.mask != nullptr && live ? a.mask + static_cast<size_t>(s.t0 + tok) * a.mask_stride : nullptr;
       const int* table = c.block_table + static_cast<size_t>(sg.b) * c.table_stride;
-      // ---- Q: one row per thread ----
+      // ---- Q: a warp brings its 32 rows, two at a time, 16 bytes per lane; each lane keeps the factor of its own row ----
       float rowf = a.scale * PG_LOG2E;
-      if (ok && n_seg > 0) ok = tc_wait(&sh.q_free, (n_seg - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
-      if (ok && n_hand > 0) ok = tc_wait(&sh.hand[1], (n_hand - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+      if (ok && n_seg > 0) ok = pt_wait(&sh.q_free, (n_seg - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+      if (ok && n_hand > 0) ok = pt_wait(&sh.hand[1], (n_hand - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+      __syncwarp();
       {
         const uint32_t dst = smem_u32(sq) + wg * PT_TILE;
-        const size_t off = static_cast<size_t>(s.t0 + tok) * a.q_stride_t + static_cast<size_t>(head) * a.q_stride_h;
-        uint4 v[16];
+        const int ch = lane & 15, first = sg.row0 + (pair ? wg * PT_M : 0) + quarter * 32 + (lane >> 4), end = sg.row0 + sg.rows;    // rows of the sequence
+        const __nv_bfloat16* qp = reinterpret_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(s.t0 + first / G) * a.q_stride_t +
+                                  static_cast<size_t>(sg.kvh * G) * a.q_stride_h + ch * 8;
+        int h = first % G;
+        uint4 qv[16];
 #pragma unroll
-        for (int ch = 0; ch < 16; ++ch) {
-          v[ch] = make_uint4(0, 0, 0, 0);
-          if (live) v[ch] = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) + off + ch * 8);
+        for (int i = 0; i < 16; ++i) {
+          qv[i] = make_uint4(0, 0, 0, 0);
+          if (first + 2 * i < end) qv[i] = *reinterpret_cast<const uint4*>(qp + h * a.q_stride_h);
+          for (h += 2; h >= G; h -= G) qp += a.q_stride_t;               // two rows on
         }
-        if constexpr (KV8) {                   // |q| of the row below 256 by a power of two, then an e4m3 head and an e4m3 remainder
-          float mx = 0.f;
 #pragma unroll
-          for (int ch = 0; ch < 16; ++ch) {
-            const unsigned x[4] = {v[ch].x, v[ch].y, v[ch].z, v[ch].w};
+        for (int i = 0; i < 16; ++i) {
+          const int rt = quarter * 32 + 2 * i + (lane >> 4);
+          const uint4 v = qv[i];
+          if constexpr (KV8) {                 // |q| of the row below 256 by a power of two, then an e4m3 head and an e4m3 remainder
+            const float y[8] = {__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u),
+                                __uint_as_float(v.z << 16), __uint_as_float(v.z & 0xffff0000u), __uint_as_float(v.w << 16), __uint_as_float(v.w & 0xffff0000u)};
+            float mx = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
-          }
-          const int e2 = min(max(static_cast<int>(__float_as_uint(mx) >> 23) - 127 - 7, -100), 100);
-          rowf *= mx <= 3.4028235e38f ? __uint_as_float(static_cast<unsigned>(127 + e2) << 23) : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
-          const float inv = __uint_as_float(static_cast<unsigned>(127 - e2) << 23);
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(y[e]));
 #pragma unroll
-          for (int ch = 0; ch < 8; ++ch) {
-            const unsigned x[8] = {v[2 * ch].x, v[2 * ch].y, v[2 * ch].z, v[2 * ch].w, v[2 * ch + 1].x, v[2 * ch + 1].y, v[2 * ch + 1].z, v[2 * ch + 1].w};
-            unsigned hi[4], lo[4];
+            for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const int e2 = min(max(static_cast<int>(__float_as_uint(mx) >> 23) - 127 - 7, -100), 100);
+            const float f = mx <= 3.4028235e38f ? __uint_as_float(static_cast<unsigned>(127 + e2) << 23) : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
+            const float f0 = __shfl_sync(0xffffffffu, f, 0), f1 = __shfl_sync(0xffffffffu, f, 16);
+            if ((lane >> 1) == i) rowf *= (lane & 1) ? f1 : f0;
+            const float inv = __uint_as_float(static_cast<unsigned>(127 - e2) << 23);
+            unsigned hi[2], lo[2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float y0 = __uint_as_float(x[2 * e] << 16) * inv, y1 = __uint_as_float(x[2 * e] & 0xffff0000u) * inv;
-              const float y2 = __uint_as_float(x[2 * e + 1] << 16) * inv, y3 = __uint_as_float(x[2 * e + 1] & 0xffff0000u) * inv;
+            for (int e = 0; e < 2; ++e) {
+              const float y0 = y[4 * e] * inv, y1 = y[4 * e + 1] * inv, y2 = y[4 * e + 2] * inv, y3 = y[4 * e + 3] * inv;
               hi[e] = static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y0, y1), __NV_SATFINITE, __NV_E4M3)) |
                       static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y2, y3), __NV_SATFINITE, __NV_E4M3)) << 16;
               const float4 h = e4m3x4_to_float4(hi[e]);
               lo[e] = static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y0 - h.x, y1 - h.y), __NV_SATFINITE, __NV_E4M3)) |
                       static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y2 - h.z, y3 - h.w), __NV_SATFINITE, __NV_E4M3)) << 16;
             }
-            pt_sts(dst + pt_at(r_tile, ch), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-            pt_sts(dst + PT_HALF + pt_at(r_tile, ch), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+            pt_sts8(dst + pt_at(rt, ch >> 1) + (ch & 1) * 8, make_uint2(hi[0], hi[1]));
+            pt_sts8(dst + PT_HALF + pt_at(rt, ch >> 1) + (ch & 1) * 8, make_uint2(lo[0], lo[1]));
+          } else {
+            pt_sts(dst + pt_at(rt, ch), v);
           }
-        } else {
-#pragma unroll
-          for (int ch = 0; ch < 16; ++ch) pt_sts(dst + pt_at(r_tile, ch), v[ch]);
         }
         fence_proxy_async_smem();
         mbar_arrive(&sh.q_full[wg]);
@@ -488,7 +546,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       float m = -INFINITY, l = 0.f;
       bool have = false;                       // O holds something
       for (int blk = blk_first + (pair ? 0 : wg); blk < blk_end; blk += step) {
-        if (ok) ok = tc_wait(&sh.s_full[wg], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+        if (ok) ok = pt_wait(&sh.s_full[wg], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
         tc_fence_after();
         const float4* sb = sc + ((g0 + blk - blk_first) % PT_SC) * 8;
         const int key0 = blk * PT_KB;
@@ -521,37 +579,47 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           unsigned pk[32];
           float sum;
           for (int turn = 0;; ++turn) {        // (a third turn would only come from scores beyond fp32's whole numbers)
+            float v[64];                       // (nothing but waits may stand between the loads and theirs: the registers fill behind the compiler's back)
+            __syncwarp();
+            pt_ld32_issue(t_s + hf * 64, v);
+            pt_ld32_issue(t_s + hf * 64 + 32, v + 32);
+            if (hf == 1 && turn == 0) {        // the first half's probabilities have had time to land
+              pt_wait_st();
+              tc_fence_before();
+              mbar_arrive(&sh.p_ready[2 * wg]);
+            }
+            pt_wait_ld();
+            pt_pin(v);
+            pt_pin(v + 32);
+            if (edge) {
+              pt_mask32(v, hf ? seen[2] : seen[0]);
+              pt_mask32(v + 32, hf ? seen[3] : seen[1]);
+            }
             float mx = -INFINITY;
             const float mo = OFF - (m == -INFINITY ? 0.f : m);
             sum = 0.f;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              float v[32];
-              pt_ld32(t_s + hf * 64 + q * 32, v);
-              if (edge) pt_mask32(v, hf ? (q ? seen[3] : seen[2]) : (q ? seen[1] : seen[0]));
+            for (int h = 0; h < 4; ++h) {
+              float4 ke = make_float4(1.f, 0.f, 1.f, 0.f);
+              if (KV8) ke = sb[hf * 4 + h];
+              const float f = KV8 ? fabsf(ke.x) * rowf : rowf, add = KV8 ? ke.y + mo : mo;
+              const uint64_t f2 = pt_pair(f, f), add2 = pt_pair(add, add);
+              uint64_t s2 = 0;                 // (0.f, 0.f)
+              float x = -INFINITY;
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float4 ke = make_float4(1.f, 0.f, 1.f, 0.f);
-                if (KV8) ke = sb[hf * 4 + 2 * q + h];
-                const float f = KV8 ? fabsf(ke.x) * rowf : rowf, add = KV8 ? ke.y + mo : mo;
-                const uint64_t f2 = pt_pair(f, f), add2 = pt_pair(add, add);
-                uint64_t s2 = 0;               // (0.f, 0.f)
-                float x = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                  float p0, p1;
-                  pt_unpair(pt_fma2(pt_pair(v[h * 16 + e], v[h * 16 + e + 1]), f2, add2), p0, p1);    // a masked score stays -inf: f > 0
-                  x = pt_max3(x, p0, p1);
-                  p0 = pd_ex2(p0);
-                  p1 = pd_ex2(p1);
-                  s2 = pt_add2(s2, pt_pair(p0, p1));
-                  pk[q * 16 + h * 8 + e / 2] = pd_pack<KV8>(p0, p1);
-                }
-                mx = fmaxf(mx, x);
-                float s0, s1;
-                pt_unpair(s2, s0, s1);
-                sum += KV8 ? (s0 + s1) * ke.z : s0 + s1;
+              for (int e = 0; e < 16; e += 2) {
+                float p0, p1;
+                pt_unpair(pt_fma2(pt_pair(v[h * 16 + e], v[h * 16 + e + 1]), f2, add2), p0, p1);      // a masked score stays -inf: f > 0
+                x = pt_max3(x, p0, p1);
+                p0 = pd_ex2(p0);
+                p1 = pd_ex2(p1);
+                s2 = pt_add2(s2, pt_pair(p0, p1));
+                pk[h * 8 + e / 2] = pd_pack<KV8>(p0, p1);
               }
+              mx = fmaxf(mx, x);
+              float s0, s1;
+              pt_unpair(s2, s0, s1);
+              sum += KV8 ? (s0 + s1) * ke.z : s0 + s1;
             }
             mx -= mo;                          // this half's maximum of score + log2 of the V scale
             const bool grow = m == -INFINITY ? mx > -INFINITY : mx > m + PD_LAZY;
@@ -561,7 +629,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             l *= r;
             if (have) {
               // the last product with V: the other half's, of this block or of the one before (a barrier per half: a wait must not lag two phases)
-              if (ok) ok = tc_wait(&sh.pv_done[2 * wg + (hf ^ 1)], (n_blk - 1 + hf) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+              if (ok) ok = pt_wait(&sh.pv_done[2 * wg + (hf ^ 1)], (n_blk - 1 + hf) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
               tc_fence_after();
 #pragma unroll 1
               for (int q = 0; q < 8; ++q) {
@@ -578,21 +646,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           l += sum;
           have = true;
           pt_st32(t_s + hf * 32, pk);          // in the place of scores that have been read
-          pt_wait_st();
-          tc_fence_before();
-          mbar_arrive(&sh.p_ready[2 * wg + hf]);         // (a barrier per half: both may be through before the issuer looks)
         }
+        pt_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sh.p_ready[2 * wg + 1]);  // (a barrier per half: both may be through before the issuer looks)
         ++n_blk;
       }
       // ---- the result ----
-      if (have && ok) ok = tc_wait(&sh.pv_done[2 * wg + 1], (n_blk - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+      if (have && ok) ok = pt_wait(&sh.pv_done[2 * wg + 1], (n_blk - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
       tc_fence_after();
       float f0 = 1.f, f1 = 0.f;
       const uint32_t xs = smem_u32(sq) + r_tile * 512;                   // the row's place
       if (!pair) {                             // the second group hands its result over through the place of Q, which no product reads now
         float* xm = reinterpret_cast<float*>(smem + 1024);
         float* xl = reinterpret_cast<float*>(smem + 1536);
-        if (ok) ok = tc_wait(&sh.q_free, n_seg & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+        if (ok) ok = pt_wait(&sh.q_free, n_seg & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
         if (wg == 1) {
           xm[r_tile] = m;
           xl[r_tile] = l;
@@ -608,7 +676,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           }
         }
         if (wg == 1) mbar_arrive(&sh.hand[0]);
-        else if (ok) ok = tc_wait(&sh.hand[0], n_hand & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+        else if (ok) ok = pt_wait(&sh.hand[0], n_hand & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
         if (wg == 0 && sg.blk1 - sg.blk0 > 1) {
           const float m1 = xm[r_tile], M = fmaxf(m, m1);
           f0 = M == -INFINITY ? 1.f : (m == -INFINITY ? 0.f : pd_ex2(m - M));       // M = -inf: nothing seen, or nothing but NaN
@@ -621,7 +689,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         const bool odd = *reinterpret_cast<volatile int*>(&sh.odd) != 0;
         const int slot = sg.first_in_range ? 0 : 1;
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-        float* rec = recs + ((static_cast<size_t>(blockIdx.x) * 2 + slot) * rec_rows + r) * PD_REC;
+        const uint32_t stage = smem_u32(sq) + (pair ? wg * PT_TILE + quarter * 8192 : quarter * 16384);      // the warp's rows, 256 bytes each
+        const int stage_row = pair ? 256 : 512;                          // (not a pair: at the head of the row's handed-over 512 bytes)
+        const bool wide_out = ((a.out_stride_t | a.out_stride_h) & 7) == 0;
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           float v[32];
@@ -650,27 +720,56 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 if (!(fabsf(x) <= 3.4028235e38f)) v[e] += x;
               }
             }
-          if (live && whole) {
-            const size_t o = static_cast<size_t>(s.t0 + tok) * a.out_stride_t + static_cast<size_t>(head) * a.out_stride_h + q * 32;
+          // into the row's 256 bytes of the stage (the place of Q), and out in whole rows when they are full
+          if (whole) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] *= inv;
-            if (a.out_bf16) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)      // (strides of out are multiples of four elements)
-                *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o + 4 * e) =
-                    make_uint2(pd_pack<false>(v[4 * e], v[4 * e + 1]), pd_pack<false>(v[4 * e + 2], v[4 * e + 3]));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o + 4 * e) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-            }
-          } else if (live && r < rec_rows) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) *reinterpret_cast<float4*>(rec + q * 32 + 4 * e) = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
           }
+          if (whole && a.out_bf16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              pt_sts(stage + lane * stage_row + (((q * 4 + e) ^ (lane & 7)) << 4),
+                     make_uint4(pd_pack<false>(v[8 * e], v[8 * e + 1]), pd_pack<false>(v[8 * e + 2], v[8 * e + 3]), pd_pack<false>(v[8 * e + 4], v[8 * e + 5]),
+                                pd_pack<false>(v[8 * e + 6], v[8 * e + 7])));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              pt_sts(stage + lane * stage_row + ((((q & 1) * 8 + e) ^ (lane & 7)) << 4),
+                     make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
+          }
+          if (whole && a.out_bf16 ? q != 3 : !(q & 1)) continue;
+          __syncwarp();
+          const int ch = lane & 15, first = r - r_tile + quarter * 32 + (lane >> 4);                       // row of the item
+          int h = (sg.row0 + first) % G;
+          size_t o0 = static_cast<size_t>(s.t0 + (sg.row0 + first) / G) * a.out_stride_t + static_cast<size_t>(sg.kvh * G) * a.out_stride_h;
+#pragma unroll 4
+          for (int i = 0; i < 16; ++i) {
+            const int rl = 2 * i + (lane >> 4), rr = first + 2 * i;
+            const uint4 x = pt_lds(stage + rl * stage_row + ((ch ^ (rl & 7)) << 4));
+            const size_t o = o0 + static_cast<size_t>(h) * a.out_stride_h;
+            for (h += 2; h >= G; h -= G) o0 += a.out_stride_t;           // two rows on
+            if (rr >= sg.rows) continue;
+            if (whole) {
+              if (a.out_bf16) {                // (out starts on 16 bytes, but its strides are multiples of four elements only)
+                uint2* d = reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o + ch * 8);
+                if (wide_out) {
+                  *reinterpret_cast<uint4*>(d) = x;
+                } else {
+                  d[0] = make_uint2(x.x, x.y);
+                  d[1] = make_uint2(x.z, x.w);
+                }
+              } else {
+                *reinterpret_cast<uint4*>(reinterpret_cast<float*>(a.out) + o + (q >> 1) * 64 + ch * 4) = x;
+              }
+            } else if (rr < rec_rows) {
+              *reinterpret_cast<uint4*>(recs + ((static_cast<size_t>(blockIdx.x) * 2 + slot) * rec_rows + rr) * PD_REC + (q >> 1) * 64 + ch * 4) = x;
+            }
+          }
+          __syncwarp();
         }
         if (live && whole && a.lse != nullptr) a.lse[static_cast<size_t>(s.t0 + tok) * a.nq + head] = pd_lse<KV8>(m, l);
-        if (live && !whole && r < rec_rows) *reinterpret_cast<float2*>(rec + PG_HD) = make_float2(m, l);
+        if (live && !whole && r < rec_rows)
+          *reinterpret_cast<float2*>(recs + ((static_cast<size_t>(blockIdx.x) * 2 + slot) * rec_rows + r) * PD_REC + PG_HD) = make_float2(m, l);
       }
       tc_fence_before();
       if (!pair) {
@@ -683,6 +782,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       ++n_seg;
     }
   } else if (warp < PT_MMA_WARP) {
+    pt_regs_dec<PT_REGS_LOAD>();
     // =============================== loader ===========================================================================================
     // V blocks, copied 16 bytes at a time by cp.async (rows that nobody sees: zeros). A thread works on the chunks that it copied itself, so a
     // block needs no barrier among the loader's threads. Two blocks are under way: e4m3 bytes land in `raw` and go from there, as fp16,
@@ -691,15 +791,89 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
     using Rows = PtRows<KV8, 128>;
     Rows rows(c, lt, psh);
     unsigned gk = 0;                           // blocks so far
+    unsigned used = 0, turn = 0;               // bit (group, stage): the stage's last block was the group's; parity of how many were
+    // The first warp also lays out the segments, one ahead of the one that it loads (the loader is ahead of the others).
+    PtIter it;
+    PtDesc desc = {0, 0, 0, 0, 0, 0, 0, 0};
+    unsigned n_out = 0;
+    bool more = true;
+    if (warp == 8) {
+      long long total = 0;
+      for (int b = lane; b < c.B; b += 32) total += pt_work(a, pg_seq(c, b), G, RT).head * c.nkv;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      const long long u = total * blockIdx.x / grid;
+      long long at = 0, before = 0;
+      int found = 0;
+      for (int b0 = 0; b0 < c.B; b0 += 32) {   // the sequence in which this CTA's range begins
+        long long t = 0;
+        if (b0 + lane < c.B) t = pt_work(a, pg_seq(c, b0 + lane), G, RT).head * c.nkv;
+        long long incl = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, at + incl > u);
+        if (hit) {
+          const int src = __ffs(hit) - 1;
+          before = at + __shfl_sync(0xffffffffu, incl - t, src);
+          found = b0 + src;
+          break;
+        }
+        at += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      it.start(a, G, RT, total, before, found, grid);
+    }
+    auto publish = [&]() {                     // the next segment with a key block, or the end
+      while (more) {
+        PtSeg g;
+        g.last = 0;
+        more = it.next(a, G, RT, g);
+        if (more) {
+          if (g.blk0 > 0) {
+            desc.cont = g.blk0 < g.blk1 ? 2 : 1;
+            desc.ends = g.blk1 == g.nblk;
+          }
+          if (g.blk0 == g.blk1) continue;
+          if (g.blk0 == 0 && g.blk1 < g.nblk) {
+            desc.tail = 1; desc.slot = g.first_in_range ? 0 : 1; desc.b = g.b; desc.kvh = g.kvh; desc.row0 = g.row0; desc.rows = g.rows;
+          }
+        } else {
+          g.last = 1;
+          descs[blockIdx.x] = desc;
+        }
+        const unsigned i = n_out % PT_SEGS;
+        if (n_out >= PT_SEGS && ok) ok = pt_wait(&sh.seg_free[i], ((n_out / PT_SEGS) & 1u) ^ 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
+        sh.seg[i] = g;
+        mbar_arrive(&sh.seg_full[i]);
+        ++n_out;
+        break;
+      }
+    };
+    if (tid == 256) publish();
+    __syncwarp();
     while (const PtSeg* gp = next_seg()) {
+      if (tid == 256) publish();
+      __syncwarp();
       const int nb = gp->blk1 - gp->blk0, all_see = gp->all_see, first = gp->blk0 * PT_KB;
       rows.start(c, c.v, *gp);
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
       ++n_seg;
+      const bool both = gp->rows > PT_M;       // groups that use a block: both, or n & 1
       auto wait_empty = [&](int n) {
-        const unsigned g = gk + n;
-        if (g >= 2 && ok) ok = tc_wait(&sh.v_empty[g & 1], ((g >> 1) & 1u) ^ 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
+        const int st = (gk + n) & 1;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {          // who has had the stage's last block is waited for, who gets this one is noted
+          const unsigned bit = 1u << (w * 2 + st);
+          if ((used & bit) && ok) ok = pt_wait(&sh.v_empty[w][st], (turn & bit) ? 0u : 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
+          used &= ~bit;
+          if (both || w == (n & 1)) {
+            used |= bit;
+            turn ^= bit;
+          }
+        }
       };
       auto finish = [&](int n) {               // block n has landed
         const unsigned g = gk + n;
@@ -775,14 +949,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       gk += nb;
     }
   } else {
+    pt_regs_dec<PT_REGS_MMA>();
     if (warp >= PT_MMA_WARP + 2) {
       // =============================== K and the page scales ==============================================================================
       constexpr int LAG = KS / 2;              // blocks under way
       const int lt = tid - (PT_MMA_WARP + 2) * 32;
       PtRows<KV8, 64> rows(c, lt, psh);
-      unsigned gk = 0;
+      unsigned gk = 0, used = 0, turn = 0;     // see the V loader
       while (const PtSeg* gp = next_seg()) {
         const int nb = gp->blk1 - gp->blk0, kvh = gp->kvh, first = gp->blk0 * PT_KB;
+        const bool both = gp->rows > PT_M;
         rows.start(c, c.k, *gp);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
@@ -821,7 +997,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         for (int n = 0; n < nb + LAG; ++n) {
           const unsigned g = gk + n;
           if (n < nb) {
-            if (g >= KS && ok) ok = tc_wait(&sh.k_empty[g % KS], ((g / KS) & 1u) ^ 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const unsigned bit = 1u << (w * 4 + g % KS);
+              if ((used & bit) && ok) ok = pt_wait(&sh.k_empty[w][g % KS], (turn & bit) ? 0u : 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
+              used &= ~bit;
+              if (both || w == (n & 1)) {
+                used |= bit;
+                turn ^= bit;
+              }
+            }
             rows.template issue<true>(smem_u32(sk) + (g % KS) * K_BYTES, c.n_pages);
           } else {
             asm volatile("cp.async.commit_group;" ::: "memory");       // (an empty group: the count below stays the same)
@@ -838,115 +1023,61 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         gk += nb;
       }
     } else
-    if (warp == PT_MMA_WARP && lane == 0) {
-    // =============================== MMA issuer =========================================================================================
+    if (lane == 0) {
+    // =============================== MMA issuers ========================================================================================
+    const int w = warp - PT_MMA_WARP;          // the group that this one works for
     constexpr uint32_t idesc = (1u << 4) | (KV8 ? 0u : ((1u << 7) | (1u << 10))) | (static_cast<uint32_t>(PT_KB >> 3) << 17) | (static_cast<uint32_t>(PT_M >> 4) << 24);
     constexpr uint32_t idesc_v = idesc | (1u << 16);                   // V: MN-major
     const uint32_t q_lo = pt_lo_k(smem_u32(sq)), k_lo = pt_lo_k(smem_u32(sk)), v_lo = pt_lo_mn(smem_u32(sv));
-    auto qk = [&](int w, unsigned gk) {
-      tc_fence_after();
-      pt_mma8<KV8 ? PT_QK8 : PT_QK16>(tmem + w * 128, q_lo + w * (PT_TILE >> 4), k_lo + (gk % KS) * (K_BYTES >> 4), idesc, 0);
-      tc_commit(&sh.s_full[w]);
-      mbar_arrive(&sh.s_full[w]);              // hands on what the loader wrote beside the tile (the wait on k_full came before)
-    };
-    auto pv = [&](int w, unsigned gk, int hf, bool first) {
-      tc_fence_after();
-      pt_mma8<PT_PV>(tmem + 256 + w * 128, tmem + w * 128 + hf * 32, v_lo + (gk & 1) * (PT_TILE >> 4) + hf * 512, idesc_v, !first);
-      tc_commit(&sh.pv_done[2 * w + hf]);
-    };
-    unsigned gk = 0, n_p = 0;                  // blocks so far; bit w: phase of group w's p_ready
-    auto full_k = [&](unsigned g) { return tc_wait(&sh.k_full[g % KS], (g / KS) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT); };
-    auto full_v = [&](unsigned g) { return tc_wait(&sh.v_full[g & 1], (g >> 1) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT); };
+    unsigned gk = 0, n_p = 0, n_st = 0;        // blocks so far; phase of the group's p_ready; blocks that both tiles took
     while (const PtSeg* gp = ok ? next_seg() : nullptr) {
-      const PtSeg& sg = *gp;
-      const int nb = sg.blk1 - sg.blk0, ahead = sg.rows > PT_M ? 1 : 2;   // pair: both groups take block j; else group j & 1 does
-      ok = tc_wait(&sh.q_full[0], n_seg & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT) &&
-           tc_wait(&sh.q_full[1], n_seg & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
-      // step i: O += P V of block j - ahead, then S of block j, for group w (one instance of either product: code that is rarely run is fetched
-      // from far, and the other warps' code is large)
-      const int steps = ahead == 1 ? 2 * (nb + 1) : nb + 2;
+      const int nb = gp->blk1 - gp->blk0, step = gp->rows > PT_M ? 1 : 2, first = step == 1 ? 0 : w;   // its blocks: all, or every other one
+      mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
+      ok = pt_wait(&sh.q_full[w], n_seg & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
+      tc_fence_after();
+      // S of the first block, then in turn: O += P V of a block, S of the next (one instance of either product: code that is rarely run is
+      // fetched from far)
 #pragma unroll 1
-      for (int i = 0; i < steps && ok; ++i) {
-        const int j = ahead == 1 ? i >> 1 : i, w = i & 1, jp = j - ahead;
-        const bool opens = ahead == 2 || w == 0, closes = ahead == 2 || w == 1;     // the block's first / last use
-        if (jp >= 0 && jp < nb) {
-          if (opens) ok = full_v(gk + jp);
+      for (int j = first; j < nb + step && ok; j += step) {
+        const int jp = j - step;
+        if (jp >= 0) {
+          const unsigned g = gk + jp;
+          ok = pt_wait(&sh.v_full[g & 1], (g >> 1) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
 #pragma unroll 1
-          for (int hf = 0; hf < 2 && ok; ++hf) {
-            ok = tc_wait(&sh.p_ready[2 * w + hf], (n_p >> w) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
-            if (ok) pv(w, gk + jp, hf, jp < ahead && hf == 0);
+          for (int hf = 0; hf < 2; ++hf) {
+            if (ok) ok = pt_wait(&sh.p_ready[2 * w + hf], n_p, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+            if (!ok) break;
+            if (step == 1 && w == 0 && hf == 0) mbar_arrive(&sh.stagger[0]);
+            tc_fence_after();
+            pt_mma8<PT_PV>(tmem + 256 + w * 128, tmem + w * 128 + hf * 32, v_lo + (g & 1) * (PT_TILE >> 4) + hf * 512, idesc_v, jp != first || hf);
+            tc_commit(&sh.pv_done[2 * w + hf]);
           }
           if (!ok) break;
-          n_p ^= 1u << w;
-          if (closes) tc_commit(&sh.v_empty[(gk + jp) & 1]);
+          n_p ^= 1u;
+          tc_commit(&sh.v_empty[w][g & 1]);
         }
         if (j < nb) {
-          if (opens) ok = full_k(gk + j);
+          const unsigned g = gk + j;
+          ok = pt_wait(&sh.k_full[g % KS], (g / KS) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
+          // Two tiles: the second gets its scores when the first group has half of its probabilities, the first its next ones after that. The
+          // groups then stay half a block apart; in step they would compete for the exponential unit and leave the tensor cores idle
+          // in turn.
+          if (ok && step == 1 && (w == 1 || n_st > 0)) ok = pt_wait(&sh.stagger[w ^ 1], (n_st - (w ^ 1)) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
           if (!ok) break;
-          qk(w, gk + j);
-          if (closes) tc_commit(&sh.k_empty[(gk + j) % KS]);
+          pt_mma8<KV8 ? PT_QK8 : PT_QK16>(tmem + w * 128, q_lo + w * (PT_TILE >> 4), k_lo + (g % KS) * (K_BYTES >> 4), idesc, 0);
+          tc_commit(&sh.s_full[w]);
+          mbar_arrive(&sh.s_full[w]);          // hands on what the loader wrote beside the tile (the wait on k_full came before)
+          tc_commit(&sh.k_empty[w][g % KS]);
+          if (step == 1) {
+            if (w == 1) mbar_arrive(&sh.stagger[1]);
+            ++n_st;
+          }
         }
       }
       gk += nb;
       tc_commit(&sh.q_free);
-      mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
       ++n_seg;
     }
-    } else if (warp == PT_MMA_WARP + 1) {
-      // =============================== scheduler ==========================================================================================
-      long long total = 0;
-      for (int b = lane; b < c.B; b += 32) total += pt_work(a, pg_seq(c, b), G, RT).head * c.nkv;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      const long long u = total * blockIdx.x / grid;
-      long long at = 0, before = 0;
-      int found = 0;
-      for (int b0 = 0; b0 < c.B; b0 += 32) {   // the sequence in which this CTA's range begins
-        long long t = 0;
-        if (b0 + lane < c.B) t = pt_work(a, pg_seq(c, b0 + lane), G, RT).head * c.nkv;
-        long long incl = t;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += v;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, at + incl > u);
-        if (hit) {
-          const int src = __ffs(hit) - 1;
-          before = at + __shfl_sync(0xffffffffu, incl - t, src);
-          found = b0 + src;
-          break;
-        }
-        at += __shfl_sync(0xffffffffu, incl, 31);
-      }
-      if (lane == 0) {
-        PtDesc desc = {0, 0, 0, 0, 0, 0, 0, 0};
-        PtIter it;
-        it.start(a, G, RT, total, before, found, grid);
-        for (bool more = true; more && ok;) {
-          PtSeg g;
-          g.last = 0;
-          more = it.next(a, G, RT, g);
-          if (more) {
-            if (g.blk0 > 0) {
-              desc.cont = g.blk0 < g.blk1 ? 2 : 1;
-              desc.ends = g.blk1 == g.nblk;
-            }
-            if (g.blk0 == g.blk1) continue;
-            if (g.blk0 == 0 && g.blk1 < g.nblk) {
-              desc.tail = 1; desc.slot = g.first_in_range ? 0 : 1; desc.b = g.b; desc.kvh = g.kvh; desc.row0 = g.row0; desc.rows = g.rows;
-            }
-          } else {
-            g.last = 1;
-            descs[blockIdx.x] = desc;
-          }
-          const unsigned i = n_seg % PT_SEGS;
-          if (n_seg >= PT_SEGS) ok = tc_wait(&sh.seg_free[i], ((n_seg / PT_SEGS) & 1u) ^ 1u, abort_flag, c.err, ERR_MBAR_EMPTY_TIMEOUT);
-          sh.seg[i] = g;
-          mbar_arrive(&sh.seg_full[i]);
-          ++n_seg;
-        }
-      }
     }
   }
   tc_fence_before();
@@ -1018,6 +1149,11 @@ template <bool KV8>
 static cudaError_t pt_launch(const IhbPagedAttn& a, cudaStream_t stream) {
   const int grid = PT_MAX_GRID, rec_rows = pt_rec_rows(a);             // one CTA per SM
   static_assert(sizeof(PtHdr) <= 1024, "header");
+  static const int regs = [] {                 // the register split draws on what the block is launched with
+    cudaFuncAttributes f;
+    return cudaFuncGetAttributes(&f, paged_tiles_kernel<KV8>) == cudaSuccess ? f.numRegs : 0;
+  }();
+  if (regs < PT_REGS) return cudaErrorInvalidConfiguration;
   constexpr int bytes = pt_smem<KV8>();
   cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;

@@ -259,6 +259,8 @@ CHUNKS = [
     ([2000], [17], 64, 4, 128),                                  # two tiles of a verify window
     ([5000, 128, 640], [8, 8, 8], 16, 1, 32),                    # one full tile: both groups share its key blocks
     ([384, 384], [128, 256], 2, 1, 128),
+    ([1500, 700, 2100, 129, 1900, 64, 1300, 900], [15, 1, 7, 9, 12, 3, 8, 14], 32, 2, 64),     # one and two tiles in turn
+    ([130, 140, 5, 129, 128, 300], [9, 8, 5, 1, 15, 2], 64, 4, 16),
 ]
 
 
