@@ -559,9 +559,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           for (int q = 0; q < 4; ++q) {
             const int kc = key0 + q * 32, n = min(max(vis - kc, 0), 32);
             unsigned w = n == 32 ? ~0u : (1u << n) - 1u;
-            if (mrow != nullptr && n < 32)
-              for (int e = n; e < 32; ++e)
-                if (pt_sees(a, s, mrow, vis, kc + e)) w |= 1u << e;
+            if (mrow != nullptr && n < 32 && kc < s.len) {               // (vis = base: the keys from there on are the call's tokens)
+              unsigned char b[32];
+              const int j0 = kc - s.base, j1 = min(static_cast<int>(min(a.mask_stride, static_cast<long long>(s.n))), s.len - s.base);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) b[e] = j0 + e >= 0 && j0 + e < j1 ? mrow[j0 + e] : 0;     // all in flight at once
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (b[e]) w |= 1u << e;
+            }
             if (bad) {
               if (sb[2 * q].x < 0.f) w &= 0xffff0000u;
               if (sb[2 * q + 1].x < 0.f) w &= 0x0000ffffu;
