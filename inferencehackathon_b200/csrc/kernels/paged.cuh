@@ -57,10 +57,6 @@ __device__ __forceinline__ int pg_seq_of_token(const IhbPaged& c, int t, int lan
   return before < c.B && t >= c.cu_q[before] ? before : -1;
 }
 
-__device__ __forceinline__ unsigned char pg_e4m3(float x) {
-  return static_cast<unsigned char>(__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3));
-}
-
 // ---- attention ------------------------------------------------------------------------------------------------------------------
 constexpr float PD_OFF = 6.f;                // e4m3 pages: log2 of what a probability is scaled by (fp16 keeps more small ones)
 constexpr float PD_LAZY = 8.f;               // the running maximum may be passed by 2^8 before the accumulators are rescaled

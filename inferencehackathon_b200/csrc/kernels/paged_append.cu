@@ -14,39 +14,56 @@ namespace ihb {
 
 constexpr int PA_WARPS = 8;
 
-template <bool BF16>
-__device__ __forceinline__ float2 pa_load2(const void* p, size_t i) {
-  if constexpr (BF16) {
-    const unsigned r = *reinterpret_cast<const unsigned*>(reinterpret_cast<const __nv_bfloat16*>(p) + i);
-    return make_float2(__uint_as_float(r << 16), __uint_as_float(r & 0xffff0000u));
-  } else {
-    return *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(p) + i);
-  }
-}
-__device__ __forceinline__ void pa_store2(void* p, bool bf16, size_t i, float x, float y) {
-  if (bf16) *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<__nv_bfloat16*>(p) + i) = __floats2bfloat162_rn(x, y);
-  else *reinterpret_cast<float2*>(reinterpret_cast<float*>(p) + i) = make_float2(x, y);
-}
-
-// One warp, one row of 128 channels: lane holds channels 2 lane, 2 lane + 1 (x) and the same + 64 (y): the pairs of the rotation.
+// Half a warp per row of 128 channels: lane c (0 .. 15) holds channels 4 c .. 4 c + 3 (x) and the same + 64 (y), the pairs of the
+// rotation, in two loads of 16 (fp32) or 8 (bf16) bytes. With a warp per row the same work took twice the instructions.
 struct PaRow {
-  float2 x, y;
+  float x[4], y[4];
 };
 template <bool BF16>
-__device__ __forceinline__ PaRow pa_load_row(const void* p, size_t i, int lane) {
-  return {pa_load2<BF16>(p, i + 2 * lane), pa_load2<BF16>(p, i + 64 + 2 * lane)};
-}
-__device__ __forceinline__ void pa_norm_rope(PaRow& r, const float* __restrict__ gamma, float eps, float2 c, float2 s, int lane) {
-  if (gamma != nullptr) {
-    const float ss = warp_sum(r.x.x * r.x.x + r.x.y * r.x.y + r.y.x * r.y.x + r.y.y * r.y.y);
-    const float rinv = rsqrtf(ss * (1.f / PG_HD) + eps);
-    const float2 g0 = *reinterpret_cast<const float2*>(gamma + 2 * lane), g1 = *reinterpret_cast<const float2*>(gamma + 64 + 2 * lane);
-    r.x.x *= rinv * g0.x; r.x.y *= rinv * g0.y;
-    r.y.x *= rinv * g1.x; r.y.y *= rinv * g1.y;
+__device__ __forceinline__ void pa_load4(const void* p, size_t i, float (&v)[4]) {
+  if constexpr (BF16) {
+    const uint2 r = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(p) + i);
+    v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xffff0000u);
+    v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xffff0000u);
+  } else {
+    const float4 r = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i);
+    v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
   }
-  const float2 a = r.x, b = r.y;
-  r.x = make_float2(a.x * c.x - b.x * s.x, a.y * c.y - b.y * s.y);
-  r.y = make_float2(b.x * c.x + a.x * s.x, b.y * c.y + a.y * s.y);
+}
+__device__ __forceinline__ void pa_store4(void* p, bool bf16, size_t i, const float (&v)[4]) {
+  if (bf16) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p) + i) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+  } else {
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+template <bool BF16>
+__device__ __forceinline__ void pa_load_row(PaRow& r, const void* p, size_t i, int c) {
+  pa_load4<BF16>(p, i + 4 * c, r.x);
+  pa_load4<BF16>(p, i + 64 + 4 * c, r.y);
+}
+// Norm (g: the lane's gammas, norm: whether there are any) and rotation of the two rows that a warp holds.
+__device__ __forceinline__ void pa_norm_rope(PaRow& r, bool norm, const PaRow& g, float eps, const float (&cs)[4], const float (&sn)[4]) {
+  if (norm) {
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ss += r.x[j] * r.x[j] + r.y[j] * r.y[j];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float rinv = rsqrtf(ss * (1.f / PG_HD) + eps);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      r.x[j] *= rinv * g.x[j];
+      r.y[j] *= rinv * g.y[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = r.x[j], b = r.y[j];
+    r.x[j] = a * cs[j] - b * sn[j];
+    r.y[j] = b * cs[j] + a * sn[j];
+  }
 }
 
 // Least e with amax <= 448 * 2^e (448 = 1.75 * 2^8), from the bits of amax >= 0, finite.
@@ -54,6 +71,10 @@ __device__ __forceinline__ int pa_exponent(float amax) {
   const unsigned u = __float_as_uint(amax);
   const int e = static_cast<int>(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
   return min(max(e, PG_EMIN), PG_EMAX);
+}
+__device__ __forceinline__ unsigned pa_e4m3x4(float x, float y, float z, float w, float f) {
+  return static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(x * f, y * f), __NV_SATFINITE, __NV_E4M3)) |
+         static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(z * f, w * f), __NV_SATFINITE, __NV_E4M3)) << 16;
 }
 __device__ __forceinline__ float pa_pow2(int e) { return __uint_as_float(static_cast<unsigned>(e + 127) << 23); }
 
@@ -99,18 +120,18 @@ __device__ __forceinline__ bool pa_segment(const IhbPaged& c, int seg, int lane,
   return rows > 0;
 }
 
-// Blocks [0, kv_blocks): one (segment, KV head, K or V) each; RPW rows per warp cover the page. The others: HQ query heads of one
-// token per warp.
+// Blocks [0, kv_blocks): one (segment, KV head, K or V) each; 2 * RPW rows per warp cover the page. The others: hq query heads of one
+// token per warp, two at a time.
 template <bool BF16, bool KV8, int RPW>
 __global__ void __launch_bounds__(PA_WARPS * 32) paged_append_kernel(const __grid_constant__ IhbPagedAppend a, int kv_blocks, int hq) {
   __shared__ float red[PA_WARPS];
   const IhbPaged& c = a.c;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = lane >> 4, ch = lane & 15;
   const int nq = a.nq, nkv = c.nkv;
   if (static_cast<int>(blockIdx.x) >= kv_blocks) {
     const int groups = (nq + hq - 1) / hq;
     const long long w = static_cast<long long>(blockIdx.x - kv_blocks) * PA_WARPS + warp;
-    const int t = static_cast<int>(w / groups), h0 = static_cast<int>(w % groups) * hq;
+    const int t = static_cast<int>(w / groups), h0 = static_cast<int>(w % groups) * hq, h1 = min(nq, h0 + hq);
     if (t >= c.T) return;
     const int b = pg_seq_of_token(c, t, lane);
     if (b < 0) return;
@@ -122,24 +143,33 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_append_kernel(const __gri
       if (lane == 0) set_error(c.err, ERR_BAD_ARGS);
       return;
     }
-    const float2 cs = *reinterpret_cast<const float2*>(a.cos_t + static_cast<size_t>(pos) * 64 + 2 * lane);
-    const float2 sn = *reinterpret_cast<const float2*>(a.sin_t + static_cast<size_t>(pos) * 64 + 2 * lane);
+    float cs[4], sn[4];
+    pa_load4<false>(a.cos_t, static_cast<size_t>(pos) * 64 + 4 * ch, cs);
+    pa_load4<false>(a.sin_t, static_cast<size_t>(pos) * 64 + 4 * ch, sn);
+    const bool norm = a.q_gamma != nullptr;
+    PaRow g = {};
+    if (norm) pa_load_row<false>(g, a.q_gamma, 0, ch);
     void* dst = a.q_out != nullptr ? a.q_out : a.qkv;
     const bool dbf = a.q_out != nullptr ? a.q_bf16 != 0 : BF16;
     const size_t src0 = static_cast<size_t>(t) * a.qkv_stride;
     const size_t dst0 = a.q_out != nullptr ? static_cast<size_t>(t) * a.q_stride : src0;
-    for (int h = h0; h < min(nq, h0 + hq); h += 4) {        // four rows in flight
+    for (int h = h0; h < h1; h += 8) {                      // eight rows in flight
       PaRow r[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (h + i < min(nq, h0 + hq)) r[i] = pa_load_row<BF16>(a.qkv, src0 + static_cast<size_t>(h + i) * PG_HD, lane);
+      for (int i = 0; i < 4; ++i) {
+        const int hh = h + 2 * i + half;
+        r[i] = {};
+        if (hh < h1) pa_load_row<BF16>(r[i], a.qkv, src0 + static_cast<size_t>(hh) * PG_HD, ch);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (h + i >= min(nq, h0 + hq)) break;
-        pa_norm_rope(r[i], a.q_gamma, a.eps, cs, sn, lane);
-        const size_t o = dst0 + static_cast<size_t>(h + i) * PG_HD + 2 * lane;
-        pa_store2(dst, dbf, o, r[i].x.x, r[i].x.y);
-        pa_store2(dst, dbf, o + 64, r[i].y.x, r[i].y.y);
+        const int hh = h + 2 * i + half;
+        if (h + 2 * i >= h1) break;
+        pa_norm_rope(r[i], norm, g, a.eps, cs, sn);
+        if (hh >= h1) continue;
+        const size_t o = dst0 + static_cast<size_t>(hh) * PG_HD + 4 * ch;
+        pa_store4(dst, dbf, o, r[i].x);
+        pa_store4(dst, dbf, o + 64, r[i].y);
       }
     }
     return;
@@ -158,51 +188,60 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_append_kernel(const __gri
   if (s.base < 0 && tid == 0) set_error(c.err, ERR_BAD_ARGS);
   const int r0 = first % c.page, tok0 = s.t0 + (first - s.base);
   const size_t head_row = (static_cast<size_t>(page) * nkv + h) * c.page;
-  PaRow x[RPW];
-  bool live[RPW];
+  const bool norm = a.k_gamma != nullptr && !is_v;
+  PaRow x[RPW], g = {};
+  if (norm) pa_load_row<false>(g, a.k_gamma, 0, ch);
+  unsigned live = 0;                                         // bit i: row 2 (warp + PA_WARPS i) + half is written
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < RPW; ++i) {
-    const int r = warp + PA_WARPS * i;
-    live[i] = r < rows;
-    if (live[i])
-      x[i] = pa_load_row<BF16>(a.qkv, static_cast<size_t>(tok0 + r) * a.qkv_stride + static_cast<size_t>(nq + (is_v ? nkv : 0) + h) * PG_HD, lane);
+    const int r = 2 * (warp + PA_WARPS * i) + half;
+    x[i] = {};
+    if (r < rows) {
+      live |= 1u << i;
+      pa_load_row<BF16>(x[i], a.qkv, static_cast<size_t>(tok0 + r) * a.qkv_stride + static_cast<size_t>(nq + (is_v ? nkv : 0) + h) * PG_HD, ch);
+    }
   }
 #pragma unroll
   for (int i = 0; i < RPW; ++i) {
-    const int r = warp + PA_WARPS * i;
-    if (!live[i]) continue;
-    const int pos = a.positions != nullptr ? a.positions[tok0 + r] : first + r;
-    if (pos < 0 || pos >= a.n_pos) {
-      if (lane == 0) set_error(c.err, ERR_BAD_ARGS);
-      live[i] = false;
-      continue;
+    const int r = 2 * (warp + PA_WARPS * i) + half;
+    if (2 * (warp + PA_WARPS * i) >= rows) break;            // (the same for the whole warp: the norm is a warp's work)
+    float cs[4] = {}, sn[4] = {};
+    if (r < rows) {
+      const int pos = a.positions != nullptr ? a.positions[tok0 + r] : first + r;
+      if (pos < 0 || pos >= a.n_pos) {
+        if (ch == 0) set_error(c.err, ERR_BAD_ARGS);
+        live &= ~(1u << i);
+      } else if (!is_v) {
+        pa_load4<false>(a.cos_t, static_cast<size_t>(pos) * 64 + 4 * ch, cs);
+        pa_load4<false>(a.sin_t, static_cast<size_t>(pos) * 64 + 4 * ch, sn);
+      }
     }
-    if (!is_v)
-      pa_norm_rope(x[i], a.k_gamma, a.eps, *reinterpret_cast<const float2*>(a.cos_t + static_cast<size_t>(pos) * 64 + 2 * lane),
-                   *reinterpret_cast<const float2*>(a.sin_t + static_cast<size_t>(pos) * 64 + 2 * lane), lane);
-    if constexpr (KV8) {
-      const float v[4] = {fabsf(x[i].x.x), fabsf(x[i].x.y), fabsf(x[i].y.x), fabsf(x[i].y.y)};
+    if (!is_v) pa_norm_rope(x[i], norm, g, a.eps, cs, sn);
+    if (KV8 && (live >> i & 1)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (v[j] <= 3.4028235e38f) amax = fmaxf(amax, v[j]);   // infinities saturate, NaN stays NaN: neither sets the scale
+      for (int j = 0; j < 4; ++j) {                          // infinities saturate, NaN stays NaN: neither sets the scale
+        const float u = fabsf(x[i].x[j]), v = fabsf(x[i].y[j]);
+        if (u <= 3.4028235e38f) amax = fmaxf(amax, u);
+        if (v <= 3.4028235e38f) amax = fmaxf(amax, v);
+      }
     }
   }
   if constexpr (!KV8) {
-    __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(is_v ? c.v : c.k);
+    void* dst = is_v ? c.v : c.k;
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
-      if (!live[i]) continue;
-      const size_t o = (head_row + r0 + warp + PA_WARPS * i) * PG_HD + 2 * lane;
-      pa_store2(dst, true, o, x[i].x.x, x[i].x.y);
-      pa_store2(dst, true, o + 64, x[i].y.x, x[i].y.y);
+      if (!(live >> i & 1)) continue;
+      const size_t o = (head_row + r0 + 2 * (warp + PA_WARPS * i) + half) * PG_HD + 4 * ch;
+      pa_store4(dst, true, o, x[i].x);
+      pa_store4(dst, true, o + 64, x[i].y);
     }
   } else {
     unsigned char* dst = reinterpret_cast<unsigned char*>(is_v ? c.v : c.k);
     float* sc = (is_v ? c.v_scale : c.k_scale) + static_cast<size_t>(page) * nkv + h;
+    const float old = r0 > 0 ? *sc : 0.f;
     amax = warp_max(amax);
     if (lane == 0) red[warp] = amax;
-    const float old = r0 > 0 ? *sc : 0.f;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < PA_WARPS; ++w) amax = fmaxf(amax, red[w]);
@@ -213,22 +252,16 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_append_kernel(const __gri
       uint2* rowp = reinterpret_cast<uint2*>(dst + head_row * PG_HD);
       for (int i = tid; i < r0 * (PG_HD / 8); i += PA_WARPS * 32) {
         const uint2 w = rowp[i];
-        unsigned o[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float4 q = e4m3x4_to_float4(u ? w.y : w.x);
-          o[u] = static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(q.x * f, q.y * f), __NV_SATFINITE, __NV_E4M3)) |
-                 static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(q.z * f, q.w * f), __NV_SATFINITE, __NV_E4M3)) << 16;
-        }
-        rowp[i] = make_uint2(o[0], o[1]);
+        const float4 p = e4m3x4_to_float4(w.x), q = e4m3x4_to_float4(w.y);
+        rowp[i] = make_uint2(pa_e4m3x4(p.x, p.y, p.z, p.w, f), pa_e4m3x4(q.x, q.y, q.z, q.w, f));
       }
     }
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
-      if (!live[i]) continue;
-      unsigned char* o = dst + (head_row + r0 + warp + PA_WARPS * i) * PG_HD + 2 * lane;
-      *reinterpret_cast<unsigned short*>(o) = __nv_cvt_float2_to_fp8x2(make_float2(x[i].x.x * inv, x[i].x.y * inv), __NV_SATFINITE, __NV_E4M3);
-      *reinterpret_cast<unsigned short*>(o + 64) = __nv_cvt_float2_to_fp8x2(make_float2(x[i].y.x * inv, x[i].y.y * inv), __NV_SATFINITE, __NV_E4M3);
+      if (!(live >> i & 1)) continue;
+      unsigned char* o = dst + (head_row + r0 + 2 * (warp + PA_WARPS * i) + half) * PG_HD + 4 * ch;
+      *reinterpret_cast<unsigned*>(o) = pa_e4m3x4(x[i].x[0], x[i].x[1], x[i].x[2], x[i].x[3], inv);
+      *reinterpret_cast<unsigned*>(o + 64) = pa_e4m3x4(x[i].y[0], x[i].y[1], x[i].y[2], x[i].y[3], inv);
     }
     if (tid == 0) *sc = now;
   }
@@ -243,10 +276,10 @@ static bool paged_ok(const IhbPaged& c) {
 template <bool BF16, bool KV8>
 static void paged_append_launch(const IhbPagedAppend& a, int grid, int kv_blocks, int hq, cudaStream_t stream) {
   switch (a.c.page) {
-    case 16: paged_append_kernel<BF16, KV8, 2><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
-    case 32: paged_append_kernel<BF16, KV8, 4><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
-    case 64: paged_append_kernel<BF16, KV8, 8><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
-    default: paged_append_kernel<BF16, KV8, 16><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
+    case 16: paged_append_kernel<BF16, KV8, 1><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
+    case 32: paged_append_kernel<BF16, KV8, 2><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
+    case 64: paged_append_kernel<BF16, KV8, 4><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
+    default: paged_append_kernel<BF16, KV8, 8><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
   }
 }
 
@@ -258,14 +291,15 @@ extern "C" int ihb_paged_append(const IhbPagedAppend* p, cudaStream_t stream) {
   const IhbPagedAppend& a = *p;
   const IhbPaged& c = a.c;
   if (!paged_ok(c) || a.qkv == nullptr || a.nq < 1 || a.n_pos < 1 || (a.q_gamma == nullptr) != (a.k_gamma == nullptr) ||
-      a.qkv_stride % 2 || a.q_stride % 2)
+      a.qkv_stride % 8 || a.q_stride % 8)
     return cudaErrorInvalidValue;
   // pages that n tokens of a sequence touch: at most (n - 1) / page + 2, and no more than tokens
   long long segs = c.cu_q == nullptr ? c.B : static_cast<long long>(c.T) / c.page + 2ll * c.B;
   if (segs > c.T) segs = c.T;
   const long long kv_blocks = segs * 2 * c.nkv;
-  // four heads per warp where that still leaves every SM a few blocks; one where tokens are few
-  const int hq = static_cast<long long>(c.T) * a.nq >= 148ll * 8 * 16 ? 8 : 1;
+  // heads per warp: eight (one round of loads) or sixteen where that still leaves every SM blocks to choose from; two where tokens are few
+  const long long pairs = static_cast<long long>(c.T) * a.nq;
+  const int hq = pairs >= 148ll * 64 * 16 * 4 ? 16 : pairs >= 148ll * 8 * 16 ? 8 : 2;
   const long long q_warps = static_cast<long long>(c.T) * ((a.nq + hq - 1) / hq);
   const long long grid = kv_blocks + (q_warps + PA_WARPS - 1) / PA_WARPS;
   if (grid > 0x7fffffffll) return cudaErrorInvalidValue;

@@ -25,55 +25,79 @@ from . import lib as K
 
 HEAD_DIM = 128
 PAGE_SIZES = (16, 32, 64, 128)
-_IO = (torch.float32, torch.bfloat16)
+_F32, _BF16, _I32, _E4M3 = torch.float32, torch.bfloat16, torch.int32, torch.float8_e4m3fn
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+# The checks below run on every call, beside kernels that take a few microseconds: plain conditions, messages formed only when they are
+# needed, every attribute of a tensor read once.
+def _bad(what: str) -> None:
+    raise ValueError(what)
 
 
-def _cache(T: int, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale, err, dev) -> K.IhbPaged:
-    """The cache part of an argument block, checked."""
-    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == HEAD_DIM,
-          f"pages must be [n_pages, kv heads, page, {HEAD_DIM}], k and v alike")
-    n_pages, nkv, page, _ = k_pages.shape
-    _need(page in PAGE_SIZES, f"page size must be one of {PAGE_SIZES}, got {page}")
-    _need(n_pages > 0 and nkv > 0, "there must be pages and KV heads")
-    _need(k_pages.is_contiguous() and v_pages.is_contiguous(), "pages must be contiguous")
-    _need(k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0, "pages must start on a 16-byte boundary")
-    if k_pages.dtype == torch.float8_e4m3fn and v_pages.dtype == torch.float8_e4m3fn:
-        _need(k_scale is not None and v_scale is not None, "e4m3 pages need k_scale and v_scale")
+def _cache(T: int, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale, err, dev: int) -> K.IhbPaged:
+    """The cache part of an argument block, checked. ``dev``: index of the device that all tensors must be on."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or shape[3] != HEAD_DIM:
+        _bad(f"pages must be [n_pages, kv heads, page, {HEAD_DIM}], k and v alike")
+    n_pages, nkv, page, _ = shape
+    if page not in PAGE_SIZES:
+        _bad(f"page size must be one of {PAGE_SIZES}, got {page}")
+    if n_pages < 1 or nkv < 1:
+        _bad("there must be pages and KV heads")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        _bad("pages must be contiguous")
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    if (kp | vp) & 15:
+        _bad("pages must start on a 16-byte boundary")
+    dtype = k_pages.dtype
+    if v_pages.dtype != dtype:
+        _bad("pages must be bfloat16 or float8_e4m3fn, k and v alike")
+    ksp = vsp = None
+    if dtype == _E4M3:
+        if k_scale is None or v_scale is None:
+            _bad("e4m3 pages need k_scale and v_scale")
         for s in (k_scale, v_scale):
-            _need(s.dtype == torch.float32 and s.shape == (n_pages, nkv) and s.is_contiguous() and s.device == dev,
-                  "page scales must be contiguous fp32 [n_pages, kv heads] on the pages' device")
+            if s.dtype != _F32 or s.shape != shape[:2] or not s.is_contiguous() or s.get_device() != dev:
+                _bad("page scales must be contiguous fp32 [n_pages, kv heads] on the pages' device")
+        ksp, vsp = k_scale.data_ptr(), v_scale.data_ptr()
+    elif dtype != _BF16:
+        _bad("pages must be bfloat16 or float8_e4m3fn")
+    elif k_scale is not None or v_scale is not None:
+        _bad("bf16 pages have no scales")
+    if kv_len.dtype != _I32 or kv_len.dim() != 1 or not kv_len.is_contiguous() or kv_len.shape[0] < 1:
+        _bad("kv_len must be contiguous int32 [B]")
+    B = kv_len.shape[0]
+    tshape = block_table.shape
+    if len(tshape) != 2 or tshape[0] != B or tshape[1] < 1 or block_table.dtype != _I32:
+        _bad("block_table must be int32 [B, blocks] with contiguous rows")
+    tstride = block_table.stride()
+    if tstride[1] != 1 and tshape[1] != 1:
+        _bad("block_table must be int32 [B, blocks] with contiguous rows")
+    cup = ep = None
+    if cu_q is None:
+        if T != B:
+            _bad(f"without cu_q there is one token per sequence: {T} tokens, {B} sequences")
     else:
-        _need(k_pages.dtype == torch.bfloat16 and v_pages.dtype == torch.bfloat16, "pages must be bfloat16 or float8_e4m3fn")
-        _need(k_scale is None and v_scale is None, "bf16 pages have no scales")
-    B = kv_len.shape[0] if kv_len.dim() == 1 else 0
-    _need(B > 0 and kv_len.dtype == torch.int32 and kv_len.is_contiguous(), "kv_len must be contiguous int32 [B]")
-    _need(block_table.dim() == 2 and block_table.shape[0] == B and block_table.shape[1] > 0 and block_table.dtype == torch.int32
-          and block_table.stride(1) == 1, "block_table must be int32 [B, blocks] with contiguous rows")
-    if cu_q is not None:
-        _need(cu_q.dtype == torch.int32 and cu_q.shape == (B + 1,) and cu_q.is_contiguous(), "cu_q must be contiguous int32 [B + 1]")
-    else:
-        _need(T == B, f"without cu_q there is one token per sequence: {T} tokens, {B} sequences")
+        if cu_q.dtype != _I32 or cu_q.shape != (B + 1,) or not cu_q.is_contiguous() or cu_q.get_device() != dev:
+            _bad("cu_q must be contiguous int32 [B + 1] on the pages' device")
+        cup = cu_q.data_ptr()
     if err is not None:
-        _need(err.dtype == torch.int32 and err.numel() >= 1, "err must be an int32 word")
-    for t in (k_pages, v_pages, block_table, kv_len, cu_q, err):
-        _need(t is None or t.device == dev, "all tensors must be on one device")
-    return K.IhbPaged(k_pages.data_ptr(), v_pages.data_ptr(), K.ptr(k_scale), K.ptr(v_scale), n_pages, nkv, page, B, T,
-                      block_table.shape[1], block_table.stride(0), block_table.data_ptr(), kv_len.data_ptr(), K.ptr(cu_q), K.ptr(err))
+        if err.dtype != _I32 or err.numel() < 1 or err.get_device() != dev:
+            _bad("err must be an int32 word on the pages' device")
+        ep = err.data_ptr()
+    if k_pages.get_device() != dev or v_pages.get_device() != dev or kv_len.get_device() != dev or block_table.get_device() != dev:
+        _bad("all tensors must be on one device")
+    return K.IhbPaged(kp, vp, ksp, vsp, n_pages, nkv, page, B, T, tshape[1], tstride[0], block_table.data_ptr(), kv_len.data_ptr(), cup, ep)
 
 
-def _launch(fn, args, dev: torch.device, what: str) -> None:
-    if dev.type != "cuda":
-        raise ValueError("the paged cache kernels need CUDA tensors")
-    if dev.index == torch.cuda.current_device():
-        K.check(fn(C.byref(args), K.stream_ptr()), what)
+def _launch(fn, args, dev: int, what: str) -> None:
+    if dev == torch.cuda.current_device():
+        code = fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream)
     else:                                   # the caller's current device is another one: launch on the tensors' own
         with torch.cuda.device(dev):
-            K.check(fn(C.byref(args), K.stream_ptr()), what)
+            code = fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+    if code:
+        K.check(code, what)
 
 
 def paged_append(qkv: torch.Tensor, nq: int, nkv: int, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -92,33 +116,60 @@ def paged_append(qkv: torch.Tensor, nq: int, nkv: int, k_pages: torch.Tensor, v_
     60; infinities saturate, NaN stays NaN, neither counts). Writing row 0 starts a page anew; otherwise the scale only grows, and
     rows already there are brought to it in place, so a page that is written to must belong to one sequence. Rows behind the last
     token and pages of other sequences are left as they are."""
-    _need(nq > 0 and nkv > 0, "nq and nkv must be positive")
-    _need(qkv.dim() == 2 and qkv.shape[1] == (nq + 2 * nkv) * HEAD_DIM and qkv.stride(1) == 1, "qkv must be [T, (nq + 2 nkv) * 128]")
-    T, dev = qkv.shape[0], qkv.device
-    _need(T > 0, "there must be a token")
-    _need(qkv.dtype in _IO, "qkv must be float32 or bfloat16")
-    vec = 8                                                     # bytes or two fp32: what one access takes
-    _need(qkv.stride(0) % 2 == 0 and qkv.data_ptr() % vec == 0, "qkv rows must start on 8-byte (fp32) or 4-byte (bf16) boundaries")
-    _need(q_out is not None or T == 1 or qkv.stride(0) >= qkv.shape[1], "qkv rows overlap: they cannot be rewritten in place")
+    if nq < 1 or nkv < 1:
+        _bad("nq and nkv must be positive")
+    shape = qkv.shape
+    if len(shape) != 2 or shape[1] != (nq + 2 * nkv) * HEAD_DIM:
+        _bad("qkv must be [T, (nq + 2 nkv) * 128]")
+    T, dev, dtype = shape[0], qkv.get_device(), qkv.dtype
+    if T < 1:
+        _bad("there must be a token")
+    stride = qkv.stride()
+    if stride[1] != 1:
+        _bad("qkv must be [T, (nq + 2 nkv) * 128] with contiguous rows")
+    if dtype != _F32 and dtype != _BF16:
+        _bad("qkv must be float32 or bfloat16")
+    qp = qkv.data_ptr()
+    if stride[0] & 7 or qp & 15:
+        _bad("qkv rows must start on 16-byte boundaries (strides multiples of 8)")
     c = _cache(T, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale, err, dev)
-    _need(c.nkv == nkv, f"pages have {c.nkv} KV heads, the call names {nkv}")
-    _need(cos_t.shape == sin_t.shape and cos_t.dim() == 2 and cos_t.shape[1] == HEAD_DIM // 2 and cos_t.shape[0] > 0
-          and cos_t.dtype == torch.float32 and sin_t.dtype == torch.float32 and cos_t.is_contiguous() and sin_t.is_contiguous(),
-          "cos_t and sin_t must be contiguous fp32 [n_pos, 64]")
-    _need((q_gamma is None) == (k_gamma is None), "q_gamma and k_gamma come together")
-    for t in (q_gamma, k_gamma):
-        _need(t is None or (t.dtype == torch.float32 and t.shape == (HEAD_DIM,) and t.is_contiguous() and t.data_ptr() % vec == 0),
-              "gammas must be contiguous fp32 [128]")
+    if c.nkv != nkv:
+        _bad(f"pages have {c.nkv} KV heads, the call names {nkv}")
+    cs = cos_t.shape
+    if (len(cs) != 2 or cs[1] != HEAD_DIM // 2 or cs[0] < 1 or sin_t.shape != cs or cos_t.dtype != _F32 or sin_t.dtype != _F32
+            or not cos_t.is_contiguous() or not sin_t.is_contiguous()):
+        _bad("cos_t and sin_t must be contiguous fp32 [n_pos, 64]")
+    cp, sp = cos_t.data_ptr(), sin_t.data_ptr()
+    gq = gk = pp = op = None
+    if q_gamma is not None or k_gamma is not None:
+        if q_gamma is None or k_gamma is None:
+            _bad("q_gamma and k_gamma come together")
+        for t in (q_gamma, k_gamma):
+            if t.dtype != _F32 or t.shape != (HEAD_DIM,) or not t.is_contiguous() or t.get_device() != dev:
+                _bad("gammas must be contiguous fp32 [128] on the pages' device")
+        gq, gk = q_gamma.data_ptr(), k_gamma.data_ptr()
+    if (cp | sp | (gq or 0) | (gk or 0)) & 15:
+        _bad("rope tables and gammas must start on 16-byte boundaries")
     if positions is not None:
-        _need(positions.dtype == torch.int32 and positions.shape == (T,) and positions.is_contiguous(), "positions must be contiguous int32 [T]")
-    if q_out is not None:
-        _need(q_out.shape == (T, nq, HEAD_DIM) and q_out.dtype in _IO and q_out.stride(2) == 1 and (nq == 1 or q_out.stride(1) == HEAD_DIM)
-              and q_out.stride(0) % 2 == 0 and (T == 1 or q_out.stride(0) >= nq * HEAD_DIM) and q_out.data_ptr() % vec == 0, "q_out must be fp32 or bf16 [T, nq, 128] with whole rows")
-    for t in (cos_t, sin_t, q_gamma, k_gamma, positions, q_out):
-        _need(t is None or t.device == dev, "all tensors must be on one device")
-    a = K.IhbPagedAppend(c, qkv.data_ptr(), qkv.dtype == torch.bfloat16, nq, qkv.stride(0), K.ptr(q_out),
-                         q_out is not None and q_out.dtype == torch.bfloat16, q_out.stride(0) if q_out is not None else 0,
-                         K.ptr(q_gamma), K.ptr(k_gamma), eps, cos_t.data_ptr(), sin_t.data_ptr(), cos_t.shape[0], K.ptr(positions))
+        if positions.dtype != _I32 or positions.shape != (T,) or not positions.is_contiguous() or positions.get_device() != dev:
+            _bad("positions must be contiguous int32 [T] on the pages' device")
+        pp = positions.data_ptr()
+    q_bf16, q_stride = 0, 0
+    if q_out is None:
+        if T > 1 and stride[0] < shape[1]:
+            _bad("qkv rows overlap: they cannot be rewritten in place")
+    else:
+        os = q_out.stride() if q_out.dim() == 3 else None
+        op, od = q_out.data_ptr(), q_out.dtype
+        if (os is None or q_out.shape != (T, nq, HEAD_DIM) or (od != _F32 and od != _BF16) or os[2] != 1 or (nq > 1 and os[1] != HEAD_DIM)
+                or os[0] & 7 or (T > 1 and os[0] < nq * HEAD_DIM) or op & 15 or q_out.get_device() != dev):
+            _bad("q_out must be fp32 or bf16 [T, nq, 128] with whole rows on 16-byte boundaries, on the pages' device")
+        q_bf16, q_stride = od == _BF16, os[0]
+    if cos_t.get_device() != dev or sin_t.get_device() != dev:
+        _bad("all tensors must be on one device")
+    if dev < 0:
+        _bad("the paged cache kernels need CUDA tensors")
+    a = K.IhbPagedAppend(c, qp, dtype == _BF16, nq, stride[0], op, q_bf16, q_stride, gq, gk, eps, cp, sp, cs[0], pp)
     _launch(K.load().ihb_paged_append, a, dev, "ihb_paged_append")
     return q_out if q_out is not None else qkv[:, :nq * HEAD_DIM].unflatten(1, (nq, HEAD_DIM))
 
@@ -136,36 +187,55 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     upper bound of the tokens per sequence. ``scale`` defaults to 128 ** -0.5. ``out [T, nq, 128]`` fp32 or bf16 (default: new, of
     ``q``'s type; tokens behind ``cu_q[B]`` are left as they are, so a new tensor holds nothing there). ``lse [T, nq]`` fp32
     receives the natural log of each softmax denominator, for merging with attention over other rows."""
-    _need(q.dim() == 3 and q.shape[2] == HEAD_DIM and q.stride(2) == 1 and q.shape[0] > 0, f"q must be [T, nq, {HEAD_DIM}]")
-    T, nq, _ = q.shape
-    dev = q.device
-    _need(q.dtype in _IO, "q must be float32 or bfloat16")
-    _need(q.stride(0) % 8 == 0 and q.stride(1) % 8 == 0 and q.data_ptr() % 16 == 0, "q strides must be multiples of 8, its start of 16 bytes")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != HEAD_DIM or shape[0] < 1:
+        _bad(f"q must be [T, nq, {HEAD_DIM}]")
+    T, nq, _ = shape
+    dev, dtype, qs, qp = q.get_device(), q.dtype, q.stride(), q.data_ptr()
+    if dtype != _F32 and dtype != _BF16:
+        _bad("q must be float32 or bfloat16")
+    if qs[2] != 1 or (qs[0] | qs[1]) & 7 or qp & 15:
+        _bad("q strides must be multiples of 8 (the last 1), its start of 16 bytes")
     c = _cache(T, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale, err, dev)
-    _need(nq % c.nkv == 0, f"{nq} query heads do not share {c.nkv} KV heads evenly")
-    _need(max_q > 0 and (cu_q is not None or max_q == 1), "max_q must be positive, and 1 without cu_q")
+    if nq % c.nkv or nq < 1:
+        _bad(f"{nq} query heads do not share {c.nkv} KV heads evenly")
+    if max_q < 1 or (cu_q is None and max_q != 1):
+        _bad("max_q must be positive, and 1 without cu_q")
     if scale is None:
         scale = HEAD_DIM ** -0.5
-    _need(0.0 < scale < 1e30, "scale must be positive and finite")
-    if out is None:
-        out = torch.empty(T, nq, HEAD_DIM, dtype=q.dtype, device=dev)
-    else:
-        _need(out.shape == q.shape and out.dtype in _IO and out.stride(2) == 1 and out.device == dev
-              and out.stride(0) % 4 == 0 and out.stride(1) % 4 == 0 and out.data_ptr() % 16 == 0,
-              "out must be fp32 or bf16 [T, nq, 128], strides multiples of 4, its start of 16 bytes")
-        _need((T == 1 or out.stride(0) >= HEAD_DIM) and (nq == 1 or out.stride(1) >= HEAD_DIM), "rows of out overlap")
+    elif not 0.0 < scale < 1e30:
+        _bad("scale must be positive and finite")
+    lp = mp = None
+    mask_stride = 0
     if lse is not None:
-        _need(lse.dtype == torch.float32 and lse.shape == (T, nq) and lse.is_contiguous() and lse.device == dev, "lse must be contiguous fp32 [T, nq]")
+        if lse.dtype != _F32 or lse.shape != (T, nq) or not lse.is_contiguous() or lse.get_device() != dev:
+            _bad("lse must be contiguous fp32 [T, nq] on the pages' device")
+        lp = lse.data_ptr()
     if mask is not None:
-        _need(mask.dtype in (torch.bool, torch.uint8) and mask.dim() == 2 and mask.shape[0] == T and mask.shape[1] >= max_q
-              and mask.stride(1) == 1 and mask.device == dev, "mask must be bool or uint8 [T, >= max_q] with contiguous rows")
-    a = K.IhbPagedAttn(c, q.data_ptr(), q.dtype == torch.bfloat16, nq, q.stride(0), q.stride(1), out.data_ptr(),
-                       out.dtype == torch.bfloat16, out.stride(0), out.stride(1), K.ptr(lse), K.ptr(mask),
-                       mask.stride(0) if mask is not None else 0, max_q, scale, None)
-    if dev.type != "cuda":
-        raise ValueError("the paged cache kernels need CUDA tensors")
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.dim() != 2 or mask.shape[0] != T or mask.shape[1] < max_q or mask.get_device() != dev:
+            _bad("mask must be bool or uint8 [T, >= max_q] on the pages' device")
+        mask_stride, last = mask.stride()
+        if last != 1 and mask.shape[1] > 1:
+            _bad("mask must have contiguous rows")
+        mp = mask.data_ptr()
+    if out is None:
+        if dev < 0:
+            _bad("the paged cache kernels need CUDA tensors")
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+        op, od, os = out.data_ptr(), dtype, (nq * HEAD_DIM, HEAD_DIM)
+    else:
+        op, od, os = out.data_ptr(), out.dtype, out.stride()
+        if (out.shape != shape or (od != _F32 and od != _BF16) or os[2] != 1 or (os[0] | os[1]) & 3 or op & 15 or out.get_device() != dev):
+            _bad("out must be fp32 or bf16 [T, nq, 128], strides multiples of 4, its start of 16 bytes, on the pages' device")
+        # tokens around heads, or heads around tokens, nothing in between
+        if not ((nq == 1 or os[1] >= HEAD_DIM) and (T == 1 or os[0] >= (nq - 1) * os[1] + HEAD_DIM)
+                or (T == 1 or os[0] >= HEAD_DIM) and (nq == 1 or os[1] >= (T - 1) * os[0] + HEAD_DIM)):
+            _bad("rows of out overlap")
+        if dev < 0:
+            _bad("the paged cache kernels need CUDA tensors")
+    a = K.IhbPagedAttn(c, qp, dtype == _BF16, nq, qs[0], qs[1], op, od == _BF16, os[0], os[1], lp, mp, mask_stride, max_q, scale, None)
     lib = K.load()
-    scratch = torch.empty(lib.ihb_paged_attention_scratch(C.byref(a)), dtype=torch.uint8, device=dev)
+    scratch = torch.empty(lib.ihb_paged_attention_scratch(C.byref(a)), dtype=torch.uint8, device=q.device)
     a.scratch = scratch.data_ptr()
     _launch(lib.ihb_paged_attention, a, dev, "ihb_paged_attention")
     return out
