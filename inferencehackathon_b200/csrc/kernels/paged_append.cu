@@ -123,12 +123,14 @@ __device__ __forceinline__ bool pa_segment(const IhbPaged& c, int seg, int lane,
 // Blocks [0, kv_blocks): one (segment, KV head, K or V) each; 2 * RPW rows per warp cover the page. The others: hq query heads of one
 // token per warp, two at a time.
 template <bool BF16, bool KV8, int RPW>
-__global__ void __launch_bounds__(PA_WARPS * 32) paged_append_kernel(const __grid_constant__ IhbPagedAppend a, int kv_blocks, int hq) {
+__global__ void __launch_bounds__(PA_WARPS * 32, RPW == 1 ? 4 : 1) paged_append_kernel(const __grid_constant__ IhbPagedAppend a, int kv_blocks, int hq) {
   __shared__ float red[PA_WARPS];
   const IhbPaged& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = lane >> 4, ch = lane & 15;
   const int nq = a.nq, nkv = c.nkv;
   if (static_cast<int>(blockIdx.x) >= kv_blocks) {
+    // (launched for itself, this part runs beside the pages' part: it waits for that one only before it ends)
+    struct AtEnd { __device__ ~AtEnd() { pdl_wait(); } } at_end;
     const int groups = (nq + hq - 1) / hq;
     const long long w = static_cast<long long>(blockIdx.x - kv_blocks) * PA_WARPS + warp;
     const int t = static_cast<int>(w / groups), h0 = static_cast<int>(w % groups) * hq, h1 = min(nq, h0 + hq);
@@ -174,6 +176,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32) paged_append_kernel(const __gri
     }
     return;
   }
+  pdl_launch_dependents();
   const int seg = blockIdx.x / (2 * nkv), which = blockIdx.x % (2 * nkv);
   const int h = which >> 1;
   const bool is_v = which & 1;
@@ -275,12 +278,28 @@ static bool paged_ok(const IhbPaged& c) {
 
 template <bool BF16, bool KV8>
 static void paged_append_launch(const IhbPagedAppend& a, int grid, int kv_blocks, int hq, cudaStream_t stream) {
+  // Large pages hold many rows per thread between the maximum and the rounding: 120 registers for 128-token pages, which leaves the query
+  // rows, most of the traffic, too few warps per SM. Where there are many they get a launch of their own at 64 registers, which need
+  // not wait for the pages' part (8 K tokens of 64 / 4 heads: 97 us in one launch, 72 in two one after the other).
+  const bool apart = hq == 16 && a.c.page >= 64;
+  const int blocks = apart ? kv_blocks : grid;
   switch (a.c.page) {
-    case 16: paged_append_kernel<BF16, KV8, 1><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
-    case 32: paged_append_kernel<BF16, KV8, 2><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
-    case 64: paged_append_kernel<BF16, KV8, 4><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
-    default: paged_append_kernel<BF16, KV8, 8><<<grid, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
+    case 16: paged_append_kernel<BF16, KV8, 1><<<blocks, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
+    case 32: paged_append_kernel<BF16, KV8, 2><<<blocks, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
+    case 64: paged_append_kernel<BF16, KV8, 4><<<blocks, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
+    default: paged_append_kernel<BF16, KV8, 8><<<blocks, PA_WARPS * 32, 0, stream>>>(a, kv_blocks, hq); break;
   }
+  if (!apart) return;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(grid - kv_blocks);
+  cfg.blockDim = dim3(PA_WARPS * 32);
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, paged_append_kernel<BF16, KV8, 1>, a, 0, hq);
 }
 
 }  // namespace ihb
@@ -299,7 +318,7 @@ extern "C" int ihb_paged_append(const IhbPagedAppend* p, cudaStream_t stream) {
   const long long kv_blocks = segs * 2 * c.nkv;
   // heads per warp: eight (one round of loads) or sixteen where that still leaves every SM blocks to choose from; two where tokens are few
   const long long pairs = static_cast<long long>(c.T) * a.nq;
-  const int hq = pairs >= 148ll * 64 * 16 * 4 ? 16 : pairs >= 148ll * 8 * 16 ? 8 : 2;
+  const int hq = pairs >= 148ll * 64 * 16 ? 16 : pairs >= 148ll * 8 * 16 ? 8 : 2;
   const long long q_warps = static_cast<long long>(c.T) * ((a.nq + hq - 1) / hq);
   const long long grid = kv_blocks + (q_warps + PA_WARPS - 1) / PA_WARPS;
   if (grid > 0x7fffffffll) return cudaErrorInvalidValue;
