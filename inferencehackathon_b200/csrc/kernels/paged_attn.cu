@@ -22,7 +22,7 @@
 namespace ihb {
 
 constexpr int PD_WARPS = 4;
-constexpr int PD_UNIT = 64;                  // keys per unit: 16 per warp
+constexpr int PD_UNIT = 128;                 // keys per unit of the work split
 constexpr float PD_NONE = 1e30f;             // OFF - running maximum before the first key
 
 template <bool F16>
@@ -109,14 +109,15 @@ __device__ __forceinline__ bool pd_sees(const IhbPagedAttn& a, const PgSeq& s, i
   return j < 0 || (j < a.mask_stride && a.mask[static_cast<size_t>(s.t0 + i) * a.mask_stride + j] != 0);
 }
 
-// Shared memory of a CTA: ST key steps per warp in flight (16 rows of K, 16 of V, the page's scales), the Q fragments of the row
+// Shared memory of a CTA: ST key steps per warp in flight (per group 16 rows of K, 16 of V, the page's scales), the Q fragments of the row
 // tile; the four warps' results take the place of the steps at the end of an item.
 template <int NT, bool KV8, int QT>
 struct PdSmem {
   static constexpr int ROWB = KV8 ? PG_HD : 2 * PG_HD;
-  static constexpr int STEP = 2 * 16 * ROWB + 16;
-  static constexpr int PER_SM = KV8 ? 4 : (NT == 2 && QT > 1 ? 2 : 3);          // CTAs per SM that ring and registers leave room for
-  static constexpr int ST = KV8 || PER_SM == 2 ? 3 : 2;
+  static constexpr int KG = KV8 ? 2 : 1;               // groups of 16 keys per step: two share the query fragments and the step's overhead
+  static constexpr int SUB = 2 * 16 * ROWB + 16, STEP = KG * SUB;
+  static constexpr int PER_SM = NT == 2 && QT > 1 && !KV8 ? 2 : 3;          // CTAs per SM that ring and registers leave room for
+  static constexpr int ST = !KV8 && PER_SM == 2 ? 3 : 2;
   static constexpr int QB = QT * NT * 8 * 32 * 8;
   static constexpr int STEPS = PD_WARPS * ST * STEP, OUT = PD_WARPS * 8 * NT * (PG_HD + 4) * 4;
   static constexpr int BYTES = QB + (STEPS > OUT ? STEPS : OUT);
@@ -204,11 +205,10 @@ __global__ void __launch_bounds__(PD_WARPS * 32, PdSmem<NT, KV8, QT>::PER_SM) pa
     const char* k0 = reinterpret_cast<const char*>(c.k) + in_page;
     const char* v0 = reinterpret_cast<const char*>(c.v) + in_page;
     const unsigned page_bytes = static_cast<unsigned>(c.nkv * c.page) * ROWB;
-    auto issue = [&](int key, int page, int slot) {       // the 16 keys from `key` on into one step of the ring
+    auto issue = [&](int key, int page, unsigned char* st) {             // the 16 keys from `key` on into one group of a step of the ring
       const bool ok = key < key_end && static_cast<unsigned>(page) < static_cast<unsigned>(c.n_pages);
       const unsigned pg = ok ? page : 0;
       const size_t off = static_cast<size_t>(pg) * page_bytes + (ok ? (key & (c.page - 1)) * ROWB : 0);
-      unsigned char* st = ring + slot * SM::STEP;
       const uint32_t kd = smem_u32(st), vd = kd + 16 * ROWB;
       const bool all = key + 16 <= s.len;     // rows behind the sequence may hold anything, and 0 * NaN is NaN: zeros instead
 #pragma unroll
@@ -221,13 +221,19 @@ __global__ void __launch_bounds__(PD_WARPS * 32, PdSmem<NT, KV8, QT>::PER_SM) pa
       if (lane == 2) *reinterpret_cast<int*>(st + 32 * ROWB + 8) = ok || key >= key_end;
     };
 
-    int key = unit0 * PD_UNIT + warp * 16;
-    int page_next = page_of(key);
+    constexpr int KG = SM::KG, STRIDE = PD_WARPS * 16 * KG;            // keys between a warp's steps
+    int key = unit0 * PD_UNIT + warp * 16 * KG;
+    int page_next[KG];
+#pragma unroll
+    for (int kg = 0; kg < KG; ++kg) page_next[kg] = page_of(key + 16 * kg);
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) {
-      const int page = page_next;
-      page_next = page_of(key + (i + 1) * PD_UNIT);
-      issue(key + i * PD_UNIT, page, i);
+#pragma unroll
+      for (int kg = 0; kg < KG; ++kg) {
+        const int page = page_next[kg];
+        page_next[kg] = page_of(key + (i + 1) * STRIDE + 16 * kg);
+        issue(key + i * STRIDE + 16 * kg, page, ring + i * SM::STEP + kg * SM::SUB);
+      }
       pd_commit();
     }
 
@@ -304,71 +310,93 @@ __global__ void __launch_bounds__(PD_WARPS * 32, PdSmem<NT, KV8, QT>::PER_SM) pa
     }
 
     int slot = 0;
-    for (; key < key_end; key += PD_UNIT) {
+    for (; key < key_end; key += STRIDE) {
       pd_wait<ST - 2>();                      // this step's copies have landed (those of the lane; the others' after the barrier)
       __syncwarp();
       {
-        const int page = page_next, nslot = slot == 0 ? ST - 1 : slot - 1;       // the step that was read last
-        page_next = page_of(key + ST * PD_UNIT);
-        issue(key + (ST - 1) * PD_UNIT, page, nslot);
+        const int nslot = slot == 0 ? ST - 1 : slot - 1;                 // the step that was read last
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg) {
+          const int page = page_next[kg];
+          page_next[kg] = page_of(key + ST * STRIDE + 16 * kg);
+          issue(key + (ST - 1) * STRIDE + 16 * kg, page, ring + nslot * SM::STEP + kg * SM::SUB);
+        }
         pd_commit();
       }
       const unsigned char* st = ring + slot * SM::STEP;
       slot = slot == ST - 1 ? 0 : slot + 1;
-      const float2 sc = *reinterpret_cast<const float2*>(st + 32 * ROWB);
-      const bool bad_page = *reinterpret_cast<const int*>(st + 32 * ROWB + 8) == 0;
-      if (bad_page && lane == 0) set_error(c.err, ERR_BAD_ARGS);
-      // ---- S^T: 16 keys x RT rows ----
-      float d[NT][4];
+      // ---- S^T: 16 keys x RT rows per group ----
+      float d[KG][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) d[nt][0] = d[nt][1] = d[nt][2] = d[nt][3] = 0.f;
+      for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) d[kg][nt][0] = d[kg][nt][1] = d[kg][nt][2] = d[kg][nt][3] = 0.f;
 #pragma unroll
       for (int k4 = 0; k4 < ROWB / 64; ++k4) {      // one 16-byte chunk of keys g and g + 8
-        const uint4 x0 = *reinterpret_cast<const uint4*>(st + g * ROWB + pd_kswz(g, k4 * 4 + t4) * 16);
-        const uint4 x1 = *reinterpret_cast<const uint4*>(st + (g + 8) * ROWB + pd_kswz(g + 8, k4 * 4 + t4) * 16);
+        uint4 x0[KG], x1[KG];
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg) {
+          x0[kg] = *reinterpret_cast<const uint4*>(st + kg * SM::SUB + g * ROWB + pd_kswz(g, k4 * 4 + t4) * 16);
+          x1[kg] = *reinterpret_cast<const uint4*>(st + kg * SM::SUB + (g + 8) * ROWB + pd_kswz(g + 8, k4 * 4 + t4) * 16);
+        }
 #pragma unroll
         for (int kk = 0; kk < (KV8 ? 4 : 2); ++kk) {
           const int k = k4 * (KV8 ? 4 : 2) + kk;
-          unsigned af[4];
-          if constexpr (KV8) {
-            pd_cvt4(pd_word(x0, kk), af[0], af[2]);
-            pd_cvt4(pd_word(x1, kk), af[1], af[3]);
-          } else {
-            af[0] = pd_word(x0, 2 * kk);     af[1] = pd_word(x1, 2 * kk);
-            af[2] = pd_word(x0, 2 * kk + 1); af[3] = pd_word(x1, 2 * kk + 1);
+          unsigned af[KG][4];
+#pragma unroll
+          for (int kg = 0; kg < KG; ++kg) {
+            if constexpr (KV8) {
+              pd_cvt4(pd_word(x0[kg], kk), af[kg][0], af[kg][2]);
+              pd_cvt4(pd_word(x1[kg], kk), af[kg][1], af[kg][3]);
+            } else {
+              af[kg][0] = pd_word(x0[kg], 2 * kk);     af[kg][1] = pd_word(x1[kg], 2 * kk);
+              af[kg][2] = pd_word(x0[kg], 2 * kk + 1); af[kg][3] = pd_word(x1[kg], 2 * kk + 1);
+            }
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
               const uint2 q2 = qf[((t * NT + nt) * 8 + k) * 32 + lane];
-              pd_mma<KV8>(d[nt], af, q2.x, q2.y);
+#pragma unroll
+              for (int kg = 0; kg < KG; ++kg) pd_mma<KV8>(d[kg][nt], af[kg], q2.x, q2.y);
             }
         }
       }
-      // ---- softmax: rows 2 t4, 2 t4 + 1, keys g, g + 8 ----
-      const float ev = KV8 ? pd_log2_scale(sc.y) : 0.f;
-      const bool edge = bad_page || key + 16 > key_all;
+      // ---- softmax: rows 2 t4, 2 t4 + 1, keys g, g + 8 of each group ----
       bool grow = false;
+      float lf[KG];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float f0 = KV8 ? rowf[nt][0] * sc.x : rowf[nt][0], f1 = KV8 ? rowf[nt][1] * sc.x : rowf[nt][1];
-        d[nt][0] = fmaf(d[nt][0], f0, ev);
-        d[nt][1] = fmaf(d[nt][1], f1, ev);
-        d[nt][2] = fmaf(d[nt][2], f0, ev);
-        d[nt][3] = fmaf(d[nt][3], f1, ev);
-        if (edge)
+      for (int kg = 0; kg < KG; ++kg) {
+        const float2 sc = *reinterpret_cast<const float2*>(st + kg * SM::SUB + 32 * ROWB);
+        const bool bad_page = *reinterpret_cast<const int*>(st + kg * SM::SUB + 32 * ROWB + 8) == 0;
+        if (bad_page && lane == 0) set_error(c.err, ERR_BAD_ARGS);
+        const float ev = KV8 ? pd_log2_scale(sc.y) : 0.f;
+        lf[kg] = KV8 ? pd_ex2(-ev) : 1.f;
+        const bool edge = bad_page || key + 16 * kg + 16 > key_all;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (bad_page || !pd_sees(a, s, (row0 + nt * 8 + 2 * t4 + (j & 1)) / G, key + g + 8 * (j >> 1))) d[nt][j] = -INFINITY;
-        grow |= fmaxf(d[nt][0], d[nt][2]) + mo[nt][0] > PD_LAZY + OFF || fmaxf(d[nt][1], d[nt][3]) + mo[nt][1] > PD_LAZY + OFF;
+        for (int nt = 0; nt < NT; ++nt) {
+          float (&x)[4] = d[kg][nt];
+          const float f0 = KV8 ? rowf[nt][0] * sc.x : rowf[nt][0], f1 = KV8 ? rowf[nt][1] * sc.x : rowf[nt][1];
+          x[0] = fmaf(x[0], f0, ev);
+          x[1] = fmaf(x[1], f1, ev);
+          x[2] = fmaf(x[2], f0, ev);
+          x[3] = fmaf(x[3], f1, ev);
+          if (edge)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (bad_page || !pd_sees(a, s, (row0 + nt * 8 + 2 * t4 + (j & 1)) / G, key + 16 * kg + g + 8 * (j >> 1))) x[j] = -INFINITY;
+          grow |= fmaxf(x[0], x[2]) + mo[nt][0] > PD_LAZY + OFF || fmaxf(x[1], x[3]) + mo[nt][1] > PD_LAZY + OFF;
+        }
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float mx = fmaxf(d[nt][r], d[nt][r + 2]);
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg) mx = fmaxf(mx, fmaxf(d[kg][nt][r], d[kg][nt][r + 2]));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -381,112 +409,115 @@ __global__ void __launch_bounds__(PD_WARPS * 32, PdSmem<NT, KV8, QT>::PER_SM) pa
             for (int j = 0; j < 8; ++j) { o[nt][j][r] *= f; o[nt][j][r + 2] *= f; }
           }
       }
-      const float lf = KV8 ? pd_ex2(-ev) : 1.f;
-      unsigned ph[NT][PT][2];
+      unsigned ph[KG][NT][PT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float p[4];
+      for (int kg = 0; kg < KG; ++kg)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          p[j] = pd_ex2(d[nt][j] + mo[nt][j & 1]);      // nothing seen yet: every score is -inf (or NaN), and so is the sum
-        }
-        l[nt][0] += (p[0] + p[2]) * lf;
-        l[nt][1] += (p[1] + p[3]) * lf;
+        for (int nt = 0; nt < NT; ++nt) {
+          float p[4];
 #pragma unroll
-        for (int t = 0; t < PT; ++t)
+          for (int j = 0; j < 4; ++j) p[j] = pd_ex2(d[kg][nt][j] + mo[nt][j & 1]);      // nothing seen yet: every score is -inf (or NaN), and so is the sum
+          l[nt][0] += (p[0] + p[2]) * lf[kg];
+          l[nt][1] += (p[1] + p[3]) * lf[kg];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const unsigned x = pd_pack<KV8>(p[2 * h], p[2 * h + 1]);
-            ph[nt][t][h] = pd_movt(x);
-            if (t + 1 < PT) {
-              const float2 v = pd_unpack<KV8>(x);
-              p[2 * h] -= v.x;
-              p[2 * h + 1] -= v.y;
+          for (int t = 0; t < PT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const unsigned x = pd_pack<KV8>(p[2 * h], p[2 * h + 1]);
+              ph[kg][nt][t][h] = pd_movt(x);
+              if (t + 1 < PT) {
+                const float2 v = pd_unpack<KV8>(x);
+                p[2 * h] -= v.x;
+                p[2 * h + 1] -= v.y;
+              }
             }
-          }
-      }
+        }
       // ---- V rows 2 t4, 2 t4 + 1, + 8, + 9: 16 channels ----
-      const unsigned char* vst = st + 16 * ROWB;
 #pragma unroll
-      for (int jv = 0; jv < (KV8 ? 1 : 2); ++jv) {
-        uint4 vr[4];
+      for (int kg = 0; kg < KG; ++kg) {
+        const unsigned char* vst = st + kg * SM::SUB + 16 * ROWB;
+        const int key0 = key + 16 * kg;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 2 * t4 + (i & 1) + 8 * (i >> 1);
-          vr[i] = *reinterpret_cast<const uint4*>(vst + r * ROWB + pd_vswz(r, jv * 8 + g) * 16);
-        }
-        // a value that is not finite in a row that not every query sees: those who see it get it, the others nothing
-        if (key + 16 > key_all) {
-          bool odd = false;
+        for (int jv = 0; jv < (KV8 ? 1 : 2); ++jv) {
+          uint4 vr[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i) {
+            const int r = 2 * t4 + (i & 1) + 8 * (i >> 1);
+            vr[i] = *reinterpret_cast<const uint4*>(vst + r * ROWB + pd_vswz(r, jv * 8 + g) * 16);
+          }
+          // a value that is not finite in a row that not every query sees: those who see it get it, the others nothing
+          if (key0 + 16 > key_all) {
+            bool odd = false;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const unsigned x = pd_word(vr[i], q);
-              if constexpr (KV8) odd |= ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u);
-              else odd |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
-            }
-          if (__any_sync(0xffffffffu, odd)) {
-            for (int kk = 0; kk < 16; ++kk) {
-              const unsigned* xr = reinterpret_cast<const unsigned*>(vst + kk * ROWB + pd_vswz(kk, jv * 8 + g) * 16);
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                const unsigned x = xr[q];
-                float v[4];
-                if constexpr (KV8) {
-                  const float4 f = e4m3x4_to_float4(x);
-                  v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-                } else {
-                  v[0] = __uint_as_float(x << 16); v[1] = __uint_as_float(x & 0xffff0000u);
-                  v[2] = v[3] = 0.f;
-                }
+                const unsigned x = pd_word(vr[i], q);
+                if constexpr (KV8) odd |= ((((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0u);
+                else odd |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+              }
+            if (__any_sync(0xffffffffu, odd)) {
+              for (int kk = 0; kk < 16; ++kk) {
+                const unsigned* xr = reinterpret_cast<const unsigned*>(vst + kk * ROWB + pd_vswz(kk, jv * 8 + g) * 16);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int r = 0; r < 2; ++r) {
-                    if (!pd_sees(a, s, (row0 + nt * 8 + 2 * t4 + r) / G, key + kk)) continue;
-#pragma unroll
-                    for (int e = 0; e < (KV8 ? 4 : 2); ++e)
-                      if (!(fabsf(v[e]) <= 3.4028235e38f)) o[nt][KV8 ? 2 * q + (e >> 1) : jv * 4 + q][r + 2 * (e & 1)] += v[e];
+                for (int q = 0; q < 4; ++q) {
+                  const unsigned x = xr[q];
+                  float v[4];
+                  if constexpr (KV8) {
+                    const float4 f = e4m3x4_to_float4(x);
+                    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+                  } else {
+                    v[0] = __uint_as_float(x << 16); v[1] = __uint_as_float(x & 0xffff0000u);
+                    v[2] = v[3] = 0.f;
                   }
-              }
-            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {     // and out of the product
-              unsigned x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+                  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                if constexpr (KV8) {
+                    for (int r = 0; r < 2; ++r) {
+                      if (!pd_sees(a, s, (row0 + nt * 8 + 2 * t4 + r) / G, key0 + kk)) continue;
 #pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    if (((x[q] >> (8 * e)) & 0x7fu) == 0x7fu) x[q] &= ~(0xffu << (8 * e));
-                } else {
-                  if ((x[q] & 0x7f80u) == 0x7f80u) x[q] &= 0xffff0000u;
-                  if ((x[q] & 0x7f800000u) == 0x7f800000u) x[q] &= 0x0000ffffu;
+                      for (int e = 0; e < (KV8 ? 4 : 2); ++e)
+                        if (!(fabsf(v[e]) <= 3.4028235e38f)) o[nt][KV8 ? 2 * q + (e >> 1) : jv * 4 + q][r + 2 * (e & 1)] += v[e];
+                    }
                 }
               }
-              vr[i] = make_uint4(x[0], x[1], x[2], x[3]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {     // and out of the product
+                unsigned x[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  if constexpr (KV8) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                      if (((x[q] >> (8 * e)) & 0x7fu) == 0x7fu) x[q] &= ~(0xffu << (8 * e));
+                  } else {
+                    if ((x[q] & 0x7f80u) == 0x7f80u) x[q] &= 0xffff0000u;
+                    if ((x[q] & 0x7f800000u) == 0x7f800000u) x[q] &= 0x0000ffffu;
+                  }
+                }
+                vr[i] = make_uint4(x[0], x[1], x[2], x[3]);
+              }
             }
           }
-        }
-        // ---- O^T += V^T P^T: tiles of 16 channels ----
+          // ---- O^T += V^T P^T: tiles of 16 channels ----
 #pragma unroll
-        for (int jj = 0; jj < (KV8 ? 8 : 4); ++jj) {
-          const int j = KV8 ? jj : jv * 4 + jj;
-          unsigned af[4];
-          if constexpr (KV8) {
-            const unsigned sel = (jj & 1) ? 0x7362u : 0x5140u;
-            pd_cvt4(__byte_perm(pd_word(vr[0], jj >> 1), pd_word(vr[1], jj >> 1), sel), af[0], af[1]);
-            pd_cvt4(__byte_perm(pd_word(vr[2], jj >> 1), pd_word(vr[3], jj >> 1), sel), af[2], af[3]);
-          } else {
-            const unsigned w0 = pd_word(vr[0], jj), w1 = pd_word(vr[1], jj), w2 = pd_word(vr[2], jj), w3 = pd_word(vr[3], jj);
-            af[0] = __byte_perm(w0, w1, 0x5410); af[1] = __byte_perm(w0, w1, 0x7632);
-            af[2] = __byte_perm(w2, w3, 0x5410); af[3] = __byte_perm(w2, w3, 0x7632);
+          for (int jj = 0; jj < (KV8 ? 8 : 4); ++jj) {
+            const int j = KV8 ? jj : jv * 4 + jj;
+            unsigned af[4];
+            if constexpr (KV8) {
+              const unsigned sel = (jj & 1) ? 0x7362u : 0x5140u;
+              pd_cvt4(__byte_perm(pd_word(vr[0], jj >> 1), pd_word(vr[1], jj >> 1), sel), af[0], af[1]);
+              pd_cvt4(__byte_perm(pd_word(vr[2], jj >> 1), pd_word(vr[3], jj >> 1), sel), af[2], af[3]);
+            } else {
+              const unsigned w0 = pd_word(vr[0], jj), w1 = pd_word(vr[1], jj), w2 = pd_word(vr[2], jj), w3 = pd_word(vr[3], jj);
+              af[0] = __byte_perm(w0, w1, 0x5410); af[1] = __byte_perm(w0, w1, 0x7632);
+              af[2] = __byte_perm(w2, w3, 0x5410); af[3] = __byte_perm(w2, w3, 0x7632);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int t = 0; t < PT; ++t) pd_mma<KV8>(o[nt][j], af, ph[kg][nt][t][0], ph[kg][nt][t][1]);
           }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int t = 0; t < PT; ++t) pd_mma<KV8>(o[nt][j], af, ph[nt][t][0], ph[nt][t][1]);
         }
       }
     }
@@ -638,7 +669,7 @@ static PdPlan pd_plan(const IhbPagedAttn& a) {
   const int G = a.nq / a.c.nkv;
   p.nt = static_cast<long long>(a.max_q) * G <= 8 ? 1 : 2;
   const bool kv8 = a.c.k_scale != nullptr;
-  p.per_sm = kv8 ? 4 : (p.nt == 2 && !a.q_bf16 ? 2 : 3);       // what is resident at once (PdSmem::PER_SM)
+  p.per_sm = !kv8 && p.nt == 2 && !a.q_bf16 ? 2 : 3;       // what is resident at once (PdSmem::PER_SM)
   p.grid = 148 * p.per_sm;
   return p;
 }
