@@ -128,3 +128,78 @@ def test_a_page_filled_token_by_token_equals_one_filled_at_once():
 def test_oracle_rounding_is_torch_rounding():
     x = torch.cat([torch.linspace(-448, 448, 40001), torch.linspace(-0.05, 0.05, 40001)])
     assert torch.equal(O.e4m3_round(x.double()).float(), x.to(torch.float8_e4m3fn).float())
+
+
+# ---- the cache's bookkeeping ------------------------------------------------------------------------------------------------
+def _cache(n_pages=10, page=16, kv="fp8"):
+    from inferencehackathon_b200.runtime.paged_kv import PagedKVCache
+    return PagedKVCache(2, n_pages, 2, page, kv, device="cpu")
+
+
+def test_pages_are_taken_and_given_back():
+    c = _cache()
+    c.add("a")
+    c.add("b")
+    b = c.extend({"a": 17, "b": 16})
+    assert c.free_pages == 7 and b.max_q == 17 and b.n_tokens == 33 and b.cu_q.tolist() == [0, 17, 33]
+    assert b.kv_len.tolist() == [17, 16] and b.block_table.shape == (2, 2) and b.block_table[1, 1] == -1
+    b = c.extend({"b": 1, "a": 1})
+    assert b.cu_q is None and b.kv_len.tolist() == [17, 18] and c.free_pages == 6
+    c.truncate("a", 16)
+    assert c.free_pages == 7 and c.length("a") == 16
+    c.free("a")
+    c.truncate("b", 0)
+    assert c.free_pages == 10
+    with pytest.raises(ValueError, match="cannot keep"):
+        c.truncate("b", 1)
+    with pytest.raises(ValueError, match="exists"):
+        c.add("b")
+    with pytest.raises(ValueError, match="no sequences"):
+        c.extend({})
+    with pytest.raises(ValueError, match="must be a token"):
+        c.extend({"b": 0})
+
+
+def test_a_full_pool_refuses_before_anything_changes():
+    c = _cache(n_pages=3)
+    c.add(1)
+    c.add(2)
+    c.extend({1: 20})
+    with pytest.raises(RuntimeError, match="2 pages needed, 1 free"):
+        c.extend({1: 13, 2: 1})
+    assert c.free_pages == 1 and c.length(1) == 20 and c.length(2) == 0
+    c.extend({1: 12, 2: 1})
+    assert c.free_pages == 0
+
+
+def test_a_forked_page_is_copied_when_it_is_written():
+    c = _cache(n_pages=6)
+    c.add("a")
+    c.extend({"a": 20})
+    c.k.view(torch.uint8).random_(0, 100)
+    c.k_scale.uniform_(0.5, 2.0)
+    c.fork("a", "b")
+    c.fork("a", "d")
+    shared = c.pages("a")
+    assert c.pages("b") == shared and c.free_pages == 4
+    c.extend({"b": 1})                                        # b writes into the partly filled page: its own copy
+    assert c.pages("b")[0] == shared[0] and c.pages("b")[1] != shared[1] and c.free_pages == 3
+    new = c.pages("b")[1]
+    assert torch.equal(c.k[:, new].view(torch.uint8), c.k[:, shared[1]].view(torch.uint8)) and torch.equal(c.k_scale[:, new], c.k_scale[:, shared[1]])
+    c.extend({"a": 1, "d": 1})                                # of the two that are left the first copies, the last keeps the page
+    assert c.free_pages == 2 and c.pages("d")[1] == shared[1] and c.pages("a")[1] not in (shared[1], new)
+    for q in "abd":
+        c.free(q)
+    assert c.free_pages == 6
+    c.add("e")
+    c.extend({"e": 32})
+    c.fork("e", "f")
+    c.truncate("f", 20)                                       # now inside a shared page
+    c.extend({"f": 1})
+    assert c.pages("f")[1] != c.pages("e")[1]
+
+
+@pytest.mark.parametrize("kw", [dict(page=48), dict(kv="int8")])
+def test_cache_refuses(kw):
+    with pytest.raises(ValueError):
+        _cache(**kw)

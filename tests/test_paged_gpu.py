@@ -425,3 +425,66 @@ def test_scales_of_very_different_size():
         seen = float((pages.v * vs[:, :, None, None].double())[ids].abs().max())
         assert float((got - want).abs().max()) <= seen * 2.0 ** -17
         assert float((l.double().cpu() - want_lse).abs().max()) <= 2.0 ** -17
+
+
+@pytest.mark.parametrize("kv,io", [("fp8", "bf16"), ("fp8", "fp32"), ("bf16", "bf16")])
+def test_serving_several_sequences_from_prompt_to_tokens(kv, io):
+    """The two operators as a server uses them, two layers: ragged prompt chunks, decode steps of a batch, a fork of a common prefix, a token
+    tree whose tail is dropped, a freed sequence. Every attention output against 64-bit attention over what the pages hold, and what
+    they hold against the rows that went in."""
+    from inferencehackathon_b200.runtime.paged_kv import PagedKVCache
+    gen = torch.Generator().manual_seed(12)
+    nq, nkv, P, layers = 8, 2, 16, 2
+    cache = PagedKVCache(layers, 64, nkv, P, kv, DEV)
+    cos, sin = _dev(*O.rope_tables(400))
+    rows = {}                                                 # (sequence, layer) -> list of V rows [nkv, 128] that went in
+
+    def step(new, tree=False):
+        batch = cache.extend(new)
+        T = batch.n_tokens
+        mask = O.tree_mask(list(new.values()), batch.max_q, T) if tree else None
+        for layer in range(layers):
+            qkv = torch.randn(T, (nq + 2 * nkv) * 128, generator=gen).to(_io(io))
+            q = cache.append(layer, qkv.to(DEV), batch, cos, sin, nq=nq)
+            t = 0
+            for s, n in new.items():
+                have = rows.setdefault((s, layer), [])
+                del have[cache.length(s) - n:]
+                have += [x for x in qkv[t:t + n, (nq + nkv) * 128:].double().view(n, nkv, 128)]
+                t += n
+            out = cache.attend(layer, q, batch, mask=None if mask is None else mask.to(DEV))
+            cache.check_error()
+            ks, vs = (None, None) if cache.k_scale is None else (cache.k_scale[layer].cpu(), cache.v_scale[layer].cpu())
+            pages = O.Pages(cache.k[layer].float().cpu(), cache.v[layer].float().cpu(), ks, vs)
+            for t in (pages.k, pages.v):
+                t.nan_to_num_(0.0)                            # pages that nothing was written to hold anything
+            cu = O.cu_of(list(new.values()))
+            ref, _ = O.attention(pages, q.cpu(), batch.block_table, batch.kv_len, cu, nkv, mask)
+            tol = _tol(ref, q.cpu(), _live(pages, cache, rows), 128 ** -0.5, kv, io, io, tiles=batch.max_q * (nq // nkv) > 32)
+            assert bool(((out.double().cpu() - ref).abs() <= tol).all())
+            for s in new:
+                got = pages.rows("v", torch.tensor(cache.pages(s)), 0, cache.length(s))
+                want = torch.stack([r[0] for r in rows[(s, layer)]])
+                big = max(float(want.abs().max()), 1.0)
+                assert float((got - want).abs().max()) <= big * (2.0 ** -4 if kv == "fp8" else 2.0 ** -8)
+
+    def _live(pages, cache, rows):
+        ids = sorted({p for s in {k[0] for k in rows} for p in cache.pages(s)})
+        return O.Pages(pages.k[ids], pages.v[ids], None if pages.ks is None else pages.ks[ids], None if pages.vs is None else pages.vs[ids])
+
+    for s in "abc":
+        cache.add(s)
+    step({"a": 37, "b": 1, "c": 64})
+    step({"a": 1, "b": 1, "c": 1})
+    step({"b": 90, "a": 3})
+    cache.fork("a", "d")
+    for layer in range(layers):
+        rows[("d", layer)] = list(rows[("a", layer)])
+    step({"d": 1, "a": 1, "b": 1, "c": 1})
+    step({"c": 9, "d": 4}, tree=True)
+    cache.truncate("c", cache.length("c") - 6)
+    step({"c": 2, "d": 1})
+    cache.free("b")
+    for layer in range(layers):
+        del rows[("b", layer)]
+    step({"a": 1, "c": 1, "d": 1})
