@@ -57,6 +57,14 @@ __device__ __forceinline__ int pg_seq_of_token(const IhbPaged& c, int t, int lan
   return before < c.B && t >= c.cu_q[before] ? before : -1;
 }
 
+// What both entry points ask of a cache block before anything is launched. Rows of a sequence are counted in 32 bits.
+static inline bool paged_ok(const IhbPaged& c) {
+  const bool page = c.page == 16 || c.page == 32 || c.page == 64 || c.page == 128;
+  return page && c.k != nullptr && c.v != nullptr && (c.k_scale == nullptr) == (c.v_scale == nullptr) && c.n_pages > 0 && c.nkv > 0 &&
+         c.nkv <= 4096 && c.B > 0 && c.T > 0 && c.max_blocks > 0 && c.max_blocks <= (1 << 30) / c.page && c.block_table != nullptr &&
+         c.kv_len != nullptr && (c.cu_q != nullptr || c.B == c.T);
+}
+
 // ---- attention ------------------------------------------------------------------------------------------------------------------
 constexpr float PD_OFF = 6.f;                // e4m3 pages: log2 of what a probability is scaled by (fp16 keeps more small ones)
 constexpr float PD_LAZY = 8.f;               // the running maximum may be passed by 2^8 before the accumulators are rescaled

@@ -270,12 +270,6 @@ __global__ void __launch_bounds__(PA_WARPS * 32, RPW == 1 ? 4 : 1) paged_append_
   }
 }
 
-static bool paged_ok(const IhbPaged& c) {
-  const bool page = c.page == 16 || c.page == 32 || c.page == 64 || c.page == 128;
-  return page && c.k != nullptr && c.v != nullptr && (c.k_scale == nullptr) == (c.v_scale == nullptr) && c.n_pages > 0 && c.nkv > 0 &&
-         c.B > 0 && c.T > 0 && c.max_blocks > 0 && c.block_table != nullptr && c.kv_len != nullptr && (c.cu_q != nullptr || c.B == c.T);
-}
-
 template <bool BF16, bool KV8>
 static void paged_append_launch(const IhbPagedAppend& a, int grid, int kv_blocks, int hq, cudaStream_t stream) {
   // Large pages hold many rows per thread between the maximum and the rounding: 120 registers for 128-token pages, which leaves the query

@@ -704,11 +704,8 @@ static cudaError_t pd_launch(const IhbPagedAttn& a, const PdPlan& p, cudaStream_
 using namespace ihb;
 
 static bool paged_attn_ok(const IhbPagedAttn& a) {
-  const IhbPaged& c = a.c;
-  const bool page = c.page == 16 || c.page == 32 || c.page == 64 || c.page == 128;
-  return page && c.k != nullptr && c.v != nullptr && (c.k_scale == nullptr) == (c.v_scale == nullptr) && c.n_pages > 0 && c.nkv > 0 &&
-         c.B > 0 && c.T > 0 && c.max_blocks > 0 && c.block_table != nullptr && c.kv_len != nullptr && (c.cu_q != nullptr || c.B == c.T) &&
-         a.q != nullptr && a.out != nullptr && a.nq > 0 && a.nq % c.nkv == 0 && a.max_q > 0 && (a.mask == nullptr || a.mask_stride >= 1) &&
+  return paged_ok(a.c) && a.nq > 0 && a.nq % a.c.nkv == 0 &&
+         a.q != nullptr && a.out != nullptr && a.max_q > 0 && (a.mask == nullptr || a.mask_stride >= 1) &&
          a.q_stride_t % 8 == 0 && a.q_stride_h % 8 == 0;
 }
 

@@ -56,20 +56,24 @@ def _cache(T: int, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale
     if dtype == _E4M3:
         if k_scale is None or v_scale is None:
             _bad("e4m3 pages need k_scale and v_scale")
+        per_page = shape[:2]
         for s in (k_scale, v_scale):
-            if s.dtype != _F32 or s.shape != shape[:2] or not s.is_contiguous() or s.get_device() != dev:
+            if s.dtype != _F32 or s.shape != per_page or not s.is_contiguous() or s.get_device() != dev:
                 _bad("page scales must be contiguous fp32 [n_pages, kv heads] on the pages' device")
         ksp, vsp = k_scale.data_ptr(), v_scale.data_ptr()
     elif dtype != _BF16:
         _bad("pages must be bfloat16 or float8_e4m3fn")
     elif k_scale is not None or v_scale is not None:
         _bad("bf16 pages have no scales")
-    if kv_len.dtype != _I32 or kv_len.dim() != 1 or not kv_len.is_contiguous() or kv_len.shape[0] < 1:
+    lens = kv_len.shape
+    if kv_len.dtype != _I32 or len(lens) != 1 or lens[0] < 1 or not kv_len.is_contiguous():
         _bad("kv_len must be contiguous int32 [B]")
-    B = kv_len.shape[0]
+    B = lens[0]
     tshape = block_table.shape
     if len(tshape) != 2 or tshape[0] != B or tshape[1] < 1 or block_table.dtype != _I32:
         _bad("block_table must be int32 [B, blocks] with contiguous rows")
+    if tshape[1] * page > 1 << 30 or nkv > 4096:
+        _bad("a sequence can have at most 2^30 rows, a cache 4096 KV heads")
     tstride = block_table.stride()
     if tstride[1] != 1 and tshape[1] != 1:
         _bad("block_table must be int32 [B, blocks] with contiguous rows")
@@ -90,12 +94,16 @@ def _cache(T: int, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale
     return K.IhbPaged(kp, vp, ksp, vsp, n_pages, nkv, page, B, T, tshape[1], tstride[0], block_table.data_ptr(), kv_len.data_ptr(), cup, ep)
 
 
+# the stream pointer without a Stream object around it where this build of torch has that (2 us less per call)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _launch(fn, args, dev: int, what: str) -> None:
     if dev == torch.cuda.current_device():
-        code = fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+        code = fn(C.byref(args), _stream(dev))
     else:                                   # the caller's current device is another one: launch on the tensors' own
         with torch.cuda.device(dev):
-            code = fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream)
+            code = fn(C.byref(args), _stream(dev))
     if code:
         K.check(code, what)
 
