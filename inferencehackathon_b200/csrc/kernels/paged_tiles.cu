@@ -61,6 +61,14 @@ struct PtHdr {
   PtSeg seg[PT_SEGS];
 };
 
+// a / b for 0 <= a < 2^62, b > 0, by way of a double (a 64-bit division is some hundred instructions, and laying out a segment takes eight)
+__device__ __forceinline__ long long pt_div(long long a, long long b) {
+  long long q = static_cast<long long>(static_cast<double>(a) / static_cast<double>(b));
+  while (q * b > a) --q;
+  while ((q + 1) * b <= a) ++q;
+  return q;
+}
+
 // ---- work items ----------------------------------------------------------------------------------------------------------------
 // Tile pair j of a sequence has the virtual length a + d * (j + 1): an arithmetic progression, so that positions are found in closed
 // form; it is mapped onto the pair's key blocks proportionally.
@@ -91,8 +99,8 @@ struct PtIter {
   PgSeq s;
   PtWork w;
   __device__ __forceinline__ void start(const IhbPagedAttn& p, int G, int RT, long long total, long long before_, int b_, int grid) {
-    u0 = u = total * blockIdx.x / grid;
-    u_end = total * (blockIdx.x + 1) / grid;
+    u0 = u = pt_div(total * blockIdx.x, grid);
+    u_end = pt_div(total * (blockIdx.x + 1), grid);
     before = before_;
     b = b_;
     if (u < u_end) {
@@ -111,11 +119,11 @@ struct PtIter {
         w = pt_work(p, s, G, RT);
         all = w.head * p.c.nkv;
       }
-      const long long q = (u - before) % w.head;
-      g.kvh = static_cast<int>((u - before) / w.head);
+      g.kvh = static_cast<int>(pt_div(u - before, w.head));
+      const long long q = u - before - g.kvh * w.head;
       long long j;
       if (w.d == 0) {
-        j = q / w.a;
+        j = pt_div(q, w.a);
       } else {
         const double h = static_cast<double>(w.a) + 0.5 * static_cast<double>(w.d);
         j = static_cast<long long>((sqrt(h * h + 2.0 * static_cast<double>(w.d) * static_cast<double>(q)) - h) / static_cast<double>(w.d));
@@ -134,8 +142,8 @@ struct PtIter {
       g.seen_end = p.mask != nullptr ? s.len : min(s.len, s.base + i_last + 1);
       g.all_see = max(0, p.mask != nullptr ? s.base : min(s.base + g.row0 / G + 1, s.len));
       g.nblk = max(1, (g.seen_end + PT_KB - 1) / PT_KB);
-      g.blk0 = static_cast<int>(v0 * g.nblk / len);
-      g.blk1 = static_cast<int>(v1 * g.nblk / len);
+      g.blk0 = v0 == 0 ? 0 : static_cast<int>(pt_div(v0 * g.nblk, len));
+      g.blk1 = v1 == len ? g.nblk : static_cast<int>(pt_div(v1 * g.nblk, len));
       g.first_in_range = u == u0;
       u += v1 - v0;
       if (g.blk0 < g.blk1 || g.blk0 > 0) return true;
@@ -511,27 +519,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           const int rt = quarter * 32 + 2 * i + (lane >> 4);
           const uint4 v = qv[i];
           if constexpr (KV8) {                 // |q| of the row below 256 by a power of two, then an e4m3 head and an e4m3 remainder
-            const float y[8] = {__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u),
-                                __uint_as_float(v.z << 16), __uint_as_float(v.z & 0xffff0000u), __uint_as_float(v.w << 16), __uint_as_float(v.w & 0xffff0000u)};
-            float mx = 0.f;
+            unsigned mx2 = 0;                  // largest magnitudes of both halves: bf16 bits without the sign order like integers
+            const unsigned x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(y[e]));
+            for (int e = 0; e < 4; ++e) mx2 = __vmaxu2(mx2, x[e] & 0x7fff7fffu);
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const int e2 = min(max(static_cast<int>(__float_as_uint(mx) >> 23) - 127 - 7, -100), 100);
-            const float f = mx <= 3.4028235e38f ? __uint_as_float(static_cast<unsigned>(127 + e2) << 23) : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
+            for (int o = 8; o > 0; o >>= 1) mx2 = __vmaxu2(mx2, __shfl_xor_sync(0xffffffffu, mx2, o));
+            const unsigned mx = max(mx2 & 0xffffu, mx2 >> 16);           // (NaN is larger than anything: its row then gets the factor NaN)
+            const int e2 = min(max(static_cast<int>(mx >> 7) - 127 - 7, -100), 100);
+            const float f = mx < 0x7f80u ? __uint_as_float(static_cast<unsigned>(127 + e2) << 23) : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
             const float f0 = __shfl_sync(0xffffffffu, f, 0), f1 = __shfl_sync(0xffffffffu, f, 16);
             if ((lane >> 1) == i) rowf *= (lane & 1) ? f1 : f0;
             const float inv = __uint_as_float(static_cast<unsigned>(127 - e2) << 23);
             unsigned hi[2], lo[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float y0 = y[4 * e] * inv, y1 = y[4 * e + 1] * inv, y2 = y[4 * e + 2] * inv, y3 = y[4 * e + 3] * inv;
-              hi[e] = static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y0, y1), __NV_SATFINITE, __NV_E4M3)) |
-                      static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y2, y3), __NV_SATFINITE, __NV_E4M3)) << 16;
-              const float4 h = e4m3x4_to_float4(hi[e]);
-              lo[e] = static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y0 - h.x, y1 - h.y), __NV_SATFINITE, __NV_E4M3)) |
-                      static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(y2 - h.z, y3 - h.w), __NV_SATFINITE, __NV_E4M3)) << 16;
+              unsigned h8[2], l8[2];
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {    // through fp16, which holds the scaled bf16 values and the differences exactly
+                const __half2 y = __floats2half2_rn(__uint_as_float(x[2 * e + k] << 16) * inv, __uint_as_float(x[2 * e + k] & 0xffff0000u) * inv);
+                h8[k] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(y), __NV_SATFINITE, __NV_E4M3);
+                const __half2 z = __hsub2(y, cvt_e4m3x2(static_cast<unsigned short>(h8[k])));
+                l8[k] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(z), __NV_SATFINITE, __NV_E4M3);
+              }
+              hi[e] = h8[0] | h8[1] << 16;
+              lo[e] = l8[0] | l8[1] << 16;
             }
             pt_sts8(dst + pt_at(rt, ch >> 1) + (ch & 1) * 8, make_uint2(hi[0], hi[1]));
             pt_sts8(dst + PT_HALF + pt_at(rt, ch >> 1) + (ch & 1) * 8, make_uint2(lo[0], lo[1]));
@@ -745,6 +757,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           }
           if (whole && a.out_bf16 ? q != 3 : !(q & 1)) continue;
           __syncwarp();
+          if (!whole) {                        // a piece: rows of the record
+            const int ch = lane & 15, row = r - r_tile + quarter * 32 + (lane >> 4), n = min(sg.rows, rec_rows) - row;
+            float* d = recs + ((static_cast<size_t>(blockIdx.x) * 2 + slot) * rec_rows + row) * PD_REC + (q >> 1) * 64 + ch * 4;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int rl = 2 * i + (lane >> 4);
+              if (2 * i < n) *reinterpret_cast<uint4*>(d + 2 * i * PD_REC) = pt_lds(stage + rl * stage_row + ((ch ^ (rl & 7)) << 4));
+            }
+            __syncwarp();
+            continue;
+          }
           const int ch = lane & 15, first = r - r_tile + quarter * 32 + (lane >> 4);                       // row of the item
           int h = (sg.row0 + first) % G;
           size_t o0 = static_cast<size_t>(s.t0 + (sg.row0 + first) / G) * a.out_stride_t + static_cast<size_t>(sg.kvh * G) * a.out_stride_h;
@@ -755,20 +778,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             const size_t o = o0 + static_cast<size_t>(h) * a.out_stride_h;
             for (h += 2; h >= G; h -= G) o0 += a.out_stride_t;           // two rows on
             if (rr >= sg.rows) continue;
-            if (whole) {
-              if (a.out_bf16) {                // (out starts on 16 bytes, but its strides are multiples of four elements only)
-                uint2* d = reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o + ch * 8);
-                if (wide_out) {
-                  *reinterpret_cast<uint4*>(d) = x;
-                } else {
-                  d[0] = make_uint2(x.x, x.y);
-                  d[1] = make_uint2(x.z, x.w);
-                }
+            if (a.out_bf16) {                  // (out starts on 16 bytes, but its strides are multiples of four elements only)
+              uint2* d = reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o + ch * 8);
+              if (wide_out) {
+                *reinterpret_cast<uint4*>(d) = x;
               } else {
-                *reinterpret_cast<uint4*>(reinterpret_cast<float*>(a.out) + o + (q >> 1) * 64 + ch * 4) = x;
+                d[0] = make_uint2(x.x, x.y);
+                d[1] = make_uint2(x.z, x.w);
               }
-            } else if (rr < rec_rows) {
-              *reinterpret_cast<uint4*>(recs + ((static_cast<size_t>(blockIdx.x) * 2 + slot) * rec_rows + rr) * PD_REC + (q >> 1) * 64 + ch * 4) = x;
+            } else {
+              *reinterpret_cast<uint4*>(reinterpret_cast<float*>(a.out) + o + (q >> 1) * 64 + ch * 4) = x;
             }
           }
           __syncwarp();
@@ -808,7 +827,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       for (int b = lane; b < c.B; b += 32) total += pt_work(a, pg_seq(c, b), G, RT).head * c.nkv;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      const long long u = total * blockIdx.x / grid;
+      const long long u = pt_div(total * blockIdx.x, grid);
       long long at = 0, before = 0;
       int found = 0;
       for (int b0 = 0; b0 < c.B; b0 += 32) {   // the sequence in which this CTA's range begins
@@ -860,8 +879,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
     if (tid == 256) publish();
     __syncwarp();
     while (const PtSeg* gp = next_seg()) {
-      if (tid == 256) publish();
-      __syncwarp();
       const int nb = gp->blk1 - gp->blk0, all_see = gp->all_see, first = gp->blk0 * PT_KB;
       rows.start(c, c.v, *gp);
       __syncwarp();
@@ -945,6 +962,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         if (n + AHEAD < nb) {
           if constexpr (KV8) rows.template issue<false>(smem_u32(raw) + ((n + AHEAD) & 1) * PT_RAW + lt * 16, c.n_pages);
           else rows.template issue<true>(smem_u32(sv) + ((gk + n) & 1) * PT_TILE, c.n_pages);
+        }
+        if (n == 0) {                          // the next segment, while this one's first blocks are on their way
+          if (tid == 256) publish();
+          __syncwarp();
         }
         if (!KV8 && f >= 0) {
           if (n < nb) asm volatile("cp.async.wait_group 1;" ::: "memory");
