@@ -36,7 +36,7 @@ constexpr int PT_RAW = 128 * PG_HD;             // e4m3 bytes of a key block's K
 template <bool KV8>
 constexpr int pt_smem() { return PT_HDR + 6 * PT_TILE + (KV8 ? 2 * PT_RAW : 0); }
 constexpr int PT_MAX_GRID = 148;              // one CTA per SM
-constexpr int PT_START = 256;                  // start-up cost of an item, in keys
+constexpr int PT_START = 512;                  // start-up cost of an item, in keys
 
 constexpr int PT_SEGS = 4;
 // A piece of an item: rows [row0, row0 + rows) of a sequence's KV head, key blocks [blk0, blk1) of nblk.
