@@ -704,13 +704,27 @@ static cudaError_t pd_launch(const IhbPagedAttn& a, const PdPlan& p, cudaStream_
 using namespace ihb;
 
 static bool paged_attn_ok(const IhbPagedAttn& a) {
-  return paged_ok(a.c) && a.nq > 0 && a.nq % a.c.nkv == 0 &&
+  return paged_ok(a.c) && a.nq > 0 && a.nq % a.c.nkv == 0 && a.nq / a.c.nkv <= 256 &&
          a.q != nullptr && a.out != nullptr && a.max_q > 0 && (a.mask == nullptr || a.mask_stride >= 1) &&
          a.q_stride_t % 8 == 0 && a.q_stride_h % 8 == 0;
 }
 
-// Which kernel: tiles of 128 rows on tcgen05 where a sequence may have more rows ((token, head) pairs) than two small tiles hold
-static bool use_tiles(const IhbPagedAttn& a) { return a.q_bf16 && static_cast<long long>(a.max_q) * (a.nq / a.c.nkv) > 32; }
+// Which kernel. The tiles of paged_tiles.cu cost the same from 1 to 128 rows ((token, head) pairs of a sequence) and some 13 us more to
+// start; here each 16 rows read the keys again. Measured, 32 / 4 heads, us here / there:
+//   32 sequences of 2048 keys  32 rows 40 / 63 (bf16 pages 52 / 57)   64: 69 / 66 (91 / 58)   128: 122 / 73 (166 / 64)
+//    8 sequences of 4096       32: 28 / 49 (34 / 42)                  64: 38 / 49 (50 / 43)   128:  61 / 51 ( 83 / 47)
+//    1 sequence of 8192        32: 19 / 48 (23 / 44)                  64: 21 / 48 (25 / 44)   128:  27 / 49 ( 33 / 46)
+//    4 sequences of 32768      32: 58 / 91 (81 / 81)                  64: 100 / 92 (143 / 81) 128: 182 / 94 (300 / 85)
+// so up to 32 rows they stay here, above 128 they go there, and between it is where the lines cross: with t sixteens of rows and W keys
+// of all heads, 50 t W us a million here (bf16 pages 80), 180 W + 10 there. The lengths are on the device: W comes from the table's width,
+// and a table much wider than its sequences gets the tiles earlier than it need. fp32 queries always stay: their precision has no tile form.
+static bool use_tiles(const IhbPagedAttn& a) {
+  const long long rows = static_cast<long long>(a.max_q) * (a.nq / a.c.nkv);
+  if (!a.q_bf16 || rows <= 32) return false;
+  if (rows > 128) return true;
+  const double t = static_cast<double>((rows + 15) / 16), w = 1e-6 * a.c.B * a.c.nkv * a.c.max_blocks * a.c.page;
+  return ((a.c.k_scale != nullptr ? 50. : 80.) * t - 180.) * w > 10.;
+}
 
 extern "C" size_t ihb_paged_attention_scratch(const IhbPagedAttn* a) {
   if (a->c.nkv < 1 || a->nq % a->c.nkv) return 0;

@@ -31,7 +31,7 @@ constexpr int PT_REGS = 128, PT_REGS_SOFTMAX = 168, PT_REGS_LOAD = 96, PT_REGS_M
 static_assert(256 * PT_REGS_SOFTMAX + 128 * PT_REGS_LOAD + 128 * PT_REGS_MMA <= PT_THREADS * PT_REGS, "more registers than the block has");
 constexpr int PT_HALF = 16384;                 // 128 rows x 128 bytes: one swizzled half (64 channels) of a tile
 constexpr int PT_TILE = 2 * PT_HALF;
-constexpr int PT_HDR = 3072;                   // barriers and segments; m and l of the second group at 1024 and 1536; page scales at 2048
+constexpr int PT_HDR = 3 * 1024;                  // barriers and segments; m and l of the second group at 1024 and 1536; page scales at 2048
 constexpr int PT_RAW = 128 * PG_HD;             // e4m3 bytes of a key block's K or V
 template <bool KV8>
 constexpr int pt_smem() { return PT_HDR + 6 * PT_TILE + (KV8 ? 2 * PT_RAW : 0); }
@@ -61,12 +61,20 @@ struct PtHdr {
   PtSeg seg[PT_SEGS];
 };
 
-// a / b for 0 <= a < 2^62, b > 0, by way of a double (a 64-bit division is some hundred instructions, and laying out a segment takes eight)
+// a / b for 0 <= a < 2^62, b > 0, a quotient below 2^40: two steps in fp32, each leaves 2^-21 of the quotient, and whole corrections. (A 64-bit
+// division, and one in fp64, are subroutines of some hundred dependent instructions, and laying out a segment took eight.)
 __device__ __forceinline__ long long pt_div(long long a, long long b) {
-  long long q = static_cast<long long>(static_cast<double>(a) / static_cast<double>(b));
+  const float fb = static_cast<float>(b);
+  long long q = static_cast<long long>(__fdividef(static_cast<float>(a), fb));
+  q += static_cast<long long>(__fdividef(static_cast<float>(a - q * b), fb));
   while (q * b > a) --q;
   while ((q + 1) * b <= a) ++q;
   return q;
+}
+// First position of CTA i's range: `total` in PT_MAX_GRID parts that differ by one at most (a division by a constant).
+__device__ __forceinline__ long long pt_cut(long long total, int i) {
+  const long long per = total / PT_MAX_GRID;
+  return per * i + min(static_cast<long long>(i), total - per * PT_MAX_GRID);
 }
 
 // ---- work items ----------------------------------------------------------------------------------------------------------------
@@ -98,9 +106,9 @@ struct PtIter {
   int b;
   PgSeq s;
   PtWork w;
-  __device__ __forceinline__ void start(const IhbPagedAttn& p, int G, int RT, long long total, long long before_, int b_, int grid) {
-    u0 = u = pt_div(total * blockIdx.x, grid);
-    u_end = pt_div(total * (blockIdx.x + 1), grid);
+  __device__ __forceinline__ void start(const IhbPagedAttn& p, int G, int RT, long long total, long long before_, int b_) {
+    u0 = u = pt_cut(total, blockIdx.x);
+    u_end = pt_cut(total, blockIdx.x + 1);
     before = before_;
     b = b_;
     if (u < u_end) {
@@ -125,8 +133,8 @@ struct PtIter {
       if (w.d == 0) {
         j = pt_div(q, w.a);
       } else {
-        const double h = static_cast<double>(w.a) + 0.5 * static_cast<double>(w.d);
-        j = static_cast<long long>((sqrt(h * h + 2.0 * static_cast<double>(w.d) * static_cast<double>(q)) - h) / static_cast<double>(w.d));
+        const float h = static_cast<float>(w.a) + 0.5f * static_cast<float>(w.d), fq = static_cast<float>(q);    // the root that cancels nothing
+        j = static_cast<long long>(__fdividef(2.f * fq, h + sqrtf(h * h + 2.f * static_cast<float>(w.d) * fq)));
         j = min(max(j, 0ll), static_cast<long long>(w.tiles - 1));
         while (j > 0 && pt_prefix(w, j) > q) --j;
         while (j + 1 < w.tiles && pt_prefix(w, j + 1) <= q) ++j;
@@ -391,7 +399,6 @@ __device__ __forceinline__ uint2 pt_lds8(uint32_t a) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
-__device__ __forceinline__ void pt_sts8(uint32_t a, uint2 v) { asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(a), "r"(v.x), "r"(v.y) : "memory"); }
 __device__ __forceinline__ void pt_sts(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -496,7 +503,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       const int vis = !live ? max(sg.seen_end, 0) : (a.mask != nullptr ? max(s.base, 0) : min(max(s.base + tok + 1, 0), s.len));   // keys [0, vis) are seen
       const unsigned char* mrow = a.mask != nullptr && live ? a.mask + static_cast<size_t>(s.t0 + tok) * a.mask_stride : nullptr;
       const int* table = c.block_table + static_cast<size_t>(sg.b) * c.table_stride;
-      // ---- Q: a warp brings its 32 rows, two at a time, 16 bytes per lane; each lane keeps the factor of its own row ----
+      // ---- Q: a warp brings its 32 rows, two at a time, 16 bytes per lane ----
       float rowf = a.scale * PG_LOG2E;
       if (ok && n_seg > 0) ok = pt_wait(&sh.q_free, (n_seg - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
       if (ok && n_hand > 0) ok = pt_wait(&sh.hand[1], (n_hand - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
@@ -507,33 +514,39 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         const __nv_bfloat16* qp = reinterpret_cast<const __nv_bfloat16*>(a.q) + static_cast<size_t>(s.t0 + first / G) * a.q_stride_t +
                                   static_cast<size_t>(sg.kvh * G) * a.q_stride_h + ch * 8;
         int h = first % G;
-        uint4 qv[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          qv[i] = make_uint4(0, 0, 0, 0);
-          if (first + 2 * i < end) qv[i] = *reinterpret_cast<const uint4*>(qp + h * a.q_stride_h);
-          for (h += 2; h >= G; h -= G) qp += a.q_stride_t;               // two rows on
-        }
-#pragma unroll
+        // e4m3: the row's even 16 bytes in the tile's first half, the odd ones beside them in the second: what becomes of a pair of them,
+        // 16 bytes of head and 16 of remainder, then has the same two places
+        const uint32_t half = (KV8 ? ch & 1 : ch >> 3) * PT_HALF;
+        const int pos = KV8 ? ch >> 1 : ch & 7;
+#pragma unroll 4
         for (int i = 0; i < 16; ++i) {
           const int rt = quarter * 32 + 2 * i + (lane >> 4);
-          const uint4 v = qv[i];
-          if constexpr (KV8) {                 // |q| of the row below 256 by a power of two, then an e4m3 head and an e4m3 remainder
-            unsigned mx2 = 0;                  // largest magnitudes of both halves: bf16 bits without the sign order like integers
-            const unsigned x[4] = {v.x, v.y, v.z, v.w};
+          const bool in = first + 2 * i < end;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + half + pt_at(rt, pos)), "l"(in ? qp + h * a.q_stride_h : a.q), "r"(in ? 16 : 0) : "memory");
+          for (h += 2; h >= G; h -= G) qp += a.q_stride_t;               // two rows on
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        if constexpr (KV8) {                   // |q| of the lane's row below 256 by a power of two, then an e4m3 head and an e4m3 remainder
+          const uint32_t row = dst + r_tile * 128;
+          unsigned mx2 = 0;                    // largest magnitudes of both halves: bf16 bits without the sign order like integers
+#pragma unroll 4
+          for (int p = 0; p < 16; ++p) {
+            const uint4 v = pt_lds(row + (p & 1) * PT_HALF + (((p >> 1) ^ (lane & 7)) << 4));
+            mx2 = __vmaxu2(mx2, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+          }
+          const unsigned mx = max(mx2 & 0xffffu, mx2 >> 16);             // (NaN is larger than anything: its row then gets the factor NaN)
+          const int e2 = min(max(static_cast<int>(mx >> 7) - 127 - 7, -100), 100);
+          rowf *= mx < 0x7f80u ? __uint_as_float(static_cast<unsigned>(127 + e2) << 23) : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
+          const float inv = __uint_as_float(static_cast<unsigned>(127 - e2) << 23);
+#pragma unroll 2
+          for (int p = 0; p < 8; ++p) {
+            const uint32_t at = row + ((p ^ (lane & 7)) << 4);
+            const uint4 v0 = pt_lds(at), v1 = pt_lds(at + PT_HALF);
+            const unsigned x[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+            unsigned hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx2 = __vmaxu2(mx2, x[e] & 0x7fff7fffu);
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) mx2 = __vmaxu2(mx2, __shfl_xor_sync(0xffffffffu, mx2, o));
-            const unsigned mx = max(mx2 & 0xffffu, mx2 >> 16);           // (NaN is larger than anything: its row then gets the factor NaN)
-            const int e2 = min(max(static_cast<int>(mx >> 7) - 127 - 7, -100), 100);
-            const float f = mx < 0x7f80u ? __uint_as_float(static_cast<unsigned>(127 + e2) << 23) : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
-            const float f0 = __shfl_sync(0xffffffffu, f, 0), f1 = __shfl_sync(0xffffffffu, f, 16);
-            if ((lane >> 1) == i) rowf *= (lane & 1) ? f1 : f0;
-            const float inv = __uint_as_float(static_cast<unsigned>(127 - e2) << 23);
-            unsigned hi[2], lo[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < 4; ++e) {
               unsigned h8[2], l8[2];
 #pragma unroll
               for (int k = 0; k < 2; ++k) {    // through fp16, which holds the scaled bf16 values and the differences exactly
@@ -545,10 +558,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
               hi[e] = h8[0] | h8[1] << 16;
               lo[e] = l8[0] | l8[1] << 16;
             }
-            pt_sts8(dst + pt_at(rt, ch >> 1) + (ch & 1) * 8, make_uint2(hi[0], hi[1]));
-            pt_sts8(dst + PT_HALF + pt_at(rt, ch >> 1) + (ch & 1) * 8, make_uint2(lo[0], lo[1]));
-          } else {
-            pt_sts(dst + pt_at(rt, ch), v);
+            pt_sts(at, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            pt_sts(at + PT_HALF, make_uint4(lo[0], lo[1], lo[2], lo[3]));
           }
         }
         fence_proxy_async_smem();
@@ -732,10 +743,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
               const int pg = table[key >> psh];
               if (!pt_sees(a, s, mrow, vis, key) || static_cast<unsigned>(pg) >= static_cast<unsigned>(c.n_pages)) continue;
               const size_t row = (static_cast<size_t>(pg) * c.nkv + sg.kvh) * c.page + (key & (c.page - 1));
-#pragma unroll
+#pragma unroll 1
               for (int e = 0; e < 32; ++e) {
                 const float x = pt_v_at<KV8>(c, row, q * 32 + e);
-                if (!(fabsf(x) <= 3.4028235e38f)) v[e] += x;
+                if (!(fabsf(x) <= 3.4028235e38f)) {
+#pragma unroll
+                  for (int k = 0; k < 32; ++k)                           // (registers have no index; unrolled the other way it is 5 KB in the epilogue's path)
+                    if (k == e) v[k] += x;
+                }
               }
             }
           // into the row's 256 bytes of the stage (the place of Q), and out in whole rows when they are full
@@ -760,7 +775,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           if (!whole) {                        // a piece: rows of the record
             const int ch = lane & 15, row = r - r_tile + quarter * 32 + (lane >> 4), n = min(sg.rows, rec_rows) - row;
             float* d = recs + ((static_cast<size_t>(blockIdx.x) * 2 + slot) * rec_rows + row) * PD_REC + (q >> 1) * 64 + ch * 4;
-#pragma unroll
+#pragma unroll 4
             for (int i = 0; i < 16; ++i) {
               const int rl = 2 * i + (lane >> 4);
               if (2 * i < n) *reinterpret_cast<uint4*>(d + 2 * i * PD_REC) = pt_lds(stage + rl * stage_row + ((ch ^ (rl & 7)) << 4));
@@ -827,7 +842,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       for (int b = lane; b < c.B; b += 32) total += pt_work(a, pg_seq(c, b), G, RT).head * c.nkv;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      const long long u = pt_div(total * blockIdx.x, grid);
+      const long long u = pt_cut(total, blockIdx.x);
       long long at = 0, before = 0;
       int found = 0;
       for (int b0 = 0; b0 < c.B; b0 += 32) {   // the sequence in which this CTA's range begins
@@ -848,7 +863,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         }
         at += __shfl_sync(0xffffffffu, incl, 31);
       }
-      it.start(a, G, RT, total, before, found, grid);
+      it.start(a, G, RT, total, before, found);
     }
     auto publish = [&]() {                     // the next segment with a key block, or the end
       while (more) {

@@ -207,6 +207,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     c = _cache(T, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale, err, dev)
     if nq % c.nkv or nq < 1:
         _bad(f"{nq} query heads do not share {c.nkv} KV heads evenly")
+    if nq > 256 * c.nkv:
+        _bad("a KV head can have at most 256 query heads")
     if max_q < 1 or (cu_q is None and max_q != 1):
         _bad("max_q must be positive, and 1 without cu_q")
     if scale is None:

@@ -285,6 +285,40 @@ def test_attention_chunks(lens, news, nq, nkv, page, cache, io):
     assert torch.equal(out, again)
 
 
+WINDOWS = [
+    # 33 to 128 rows: the table's width chooses the kernel
+    ([5000, 128, 640], [8, 8, 8], 16, 1, 32),
+    ([9, 100], [9, 17], 5, 1, 16),
+    ([200, 31, 64], [3, 1, 5], 32, 2, 32),
+    ([700, 0, 1300], [16, 4, 0], 8, 1, 128),
+    ([130], [5], 28, 4, 64),
+]
+
+
+@pytest.mark.parametrize("lens,news,nq,nkv,page", WINDOWS)
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_windows_with_narrow_and_wide_tables(lens, news, nq, nkv, page, cache, masked):
+    """A table much wider than its sequences changes the kernel, not the result."""
+    k, v, ks, vs, table, q, cu, mask = _attn_case(lens, news, nq, nkv, page, cache, "bf16", 17, masked)
+    T = sum(news)
+    ref_pages = O.Pages(k, v, ks, vs)
+    ref, ref_lse = O.attention(ref_pages, q[:T], table, lens, cu, nkv, mask[:T] if masked else None)
+    wide = torch.full((len(lens), 300000 // page), 1 << 30, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    smax = float(q.double().norm(dim=-1).max()) * 128 ** -0.5 * float(torch.nan_to_num(
+        (ref_pages.k * (1.0 if ref_pages.ks is None else ref_pages.ks[:, :, None, None]))).norm(dim=-1).max())
+    for t, tiles in ((table, False), (wide, True)):
+        out, lse = _run_attn(k, v, ks, vs, t, q, cu, mask, lens, news)
+        assert bool((out[T:] == 7.0).all())
+        far = (out[:T].double().cpu() - ref).abs()
+        assert bool((far <= _tol(ref, q[:T], ref_pages, 128 ** -0.5, cache, "bf16", "bf16", tiles=tiles)).all()), (tiles, float(far.max()))
+        seen = torch.isfinite(ref_lse)
+        got = lse[:T].double().cpu()
+        assert torch.equal(seen, torch.isfinite(got))
+        assert float((got - ref_lse)[seen].abs().max()) <= _score_error(cache, "bf16", tiles) * smax + 2.0 ** -17
+
+
 @pytest.mark.parametrize("cache", ["fp8", "bf16"])
 def test_attention_long_contexts_are_cut_over_the_gpu(cache):
     """Contexts long enough that every range cuts items; one sequence far longer than the others."""
