@@ -53,7 +53,7 @@ constexpr int PT_SC = 8;                       // blocks whose page scales are k
 
 struct PtHdr {
   uint64_t k_full[4], k_empty[2][4], v_full[2], v_empty[2][2];         // empty: [group that used it][stage]
-  uint64_t q_full[2], q_free, s_full[2], p_ready[4], pv_done[4], hand[2], stagger[2];
+  uint64_t q_full[2], q_free, s_full[4], p_ready[4], pv_done[4], hand[2];     // s_full .. pv_done: [group][half of the block]
   uint32_t tmem;
   int abort_flag;
   int odd;                                     // V values that are not finite were met in keys that not every row sees (set by the loader)
@@ -443,12 +443,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       for (int j = 0; j < 4; ++j) mbar_init(&sh.k_empty[i][j], 1);
       for (int j = 0; j < 2; ++j) mbar_init(&sh.v_empty[i][j], 1);
       mbar_init(&sh.v_full[i], 128);
-      mbar_init(&sh.q_full[i], 128); mbar_init(&sh.s_full[i], 2);
+      mbar_init(&sh.q_full[i], 128); mbar_init(&sh.s_full[2 * i], 2); mbar_init(&sh.s_full[2 * i + 1], 2);
       mbar_init(&sh.p_ready[2 * i], 128); mbar_init(&sh.p_ready[2 * i + 1], 128); mbar_init(&sh.pv_done[2 * i], 1); mbar_init(&sh.pv_done[2 * i + 1], 1);
     }
     mbar_init(&sh.q_free, 2);
-    mbar_init(&sh.stagger[0], 1);
-    mbar_init(&sh.stagger[1], 1);
     mbar_init(&sh.hand[0], 128);
     mbar_init(&sh.hand[1], 128);
     for (int i = 0; i < PT_SEGS; ++i) { mbar_init(&sh.seg_full[i], 1); mbar_init(&sh.seg_free[i], 16); }
@@ -569,7 +567,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       float m = -INFINITY, l = 0.f;
       bool have = false;                       // O holds something
       for (int blk = blk_first + (pair ? 0 : wg); blk < blk_end; blk += step) {
-        if (ok) ok = pt_wait(&sh.s_full[wg], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+        if (ok) ok = pt_wait(&sh.s_full[2 * wg], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
         tc_fence_after();
         const float4* sb = sc + ((g0 + blk - blk_first) % PT_SC) * 8;
         const int key0 = blk * PT_KB;
@@ -607,6 +605,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         for (int hf = 0; hf < 2; ++hf) {
           unsigned pk[32];
           float sum;
+          if (hf == 1) {
+            if (ok) ok = pt_wait(&sh.s_full[2 * wg + 1], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+            tc_fence_after();
+          }
           for (int turn = 0;; ++turn) {        // (a third turn would only come from scores beyond fp32's whole numbers)
             float v[64];                       // (nothing but waits may stand between the loads and theirs: the registers fill behind the compiler's back)
             __syncwarp();
@@ -674,7 +676,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           }
           l += sum;
           have = true;
-          pt_st32(t_s + hf * 32, pk);          // in the place of scores that have been read
+          pt_st32(t_s + hf * 64, pk);          // in the place of the scores
         }
         pt_wait_st();
         tc_fence_before();
@@ -1068,52 +1070,42 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
     if (lane == 0) {
     // =============================== MMA issuers ========================================================================================
     const int w = warp - PT_MMA_WARP;          // the group that this one works for
-    constexpr uint32_t idesc = (1u << 4) | (KV8 ? 0u : ((1u << 7) | (1u << 10))) | (static_cast<uint32_t>(PT_KB >> 3) << 17) | (static_cast<uint32_t>(PT_M >> 4) << 24);
-    constexpr uint32_t idesc_v = idesc | (1u << 16);                   // V: MN-major
+    constexpr uint32_t idesc = (1u << 4) | (KV8 ? 0u : ((1u << 7) | (1u << 10))) | (static_cast<uint32_t>(PT_M >> 4) << 24) | (static_cast<uint32_t>(PT_KB / 2 >> 3) << 17);
+    constexpr uint32_t idesc_v = (idesc & ~(63u << 17)) | (static_cast<uint32_t>(PG_HD >> 3) << 17) | (1u << 16);      // V: MN-major
     const uint32_t q_lo = pt_lo_k(smem_u32(sq)), k_lo = pt_lo_k(smem_u32(sk)), v_lo = pt_lo_mn(smem_u32(sv));
-    unsigned gk = 0, n_p = 0, n_st = 0;        // blocks so far; phase of the group's p_ready; blocks that both tiles took
+    unsigned gk = 0, n_p = 0;                  // blocks so far; phase of the group's p_ready
     while (const PtSeg* gp = ok ? next_seg() : nullptr) {
       const int nb = gp->blk1 - gp->blk0, step = gp->rows > PT_M ? 1 : 2, first = step == 1 ? 0 : w;   // its blocks: all, or every other one
       mbar_arrive(&sh.seg_free[n_seg % PT_SEGS]);
       ok = pt_wait(&sh.q_full[w], n_seg & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
       tc_fence_after();
-      // S of the first block, then in turn: O += P V of a block, S of the next (one instance of either product: code that is rarely run is
-      // fetched from far)
+      // By halves of a block, two ahead: O += P V of a half as soon as its probabilities are there, then S of the next block's same half
+      // into their place (products of one issuer run in order). The group meanwhile works on the other half.
+      const int halves = 2 * ((nb - first + step - 1) / step);
 #pragma unroll 1
-      for (int j = first; j < nb + step && ok; j += step) {
-        const int jp = j - step;
-        if (jp >= 0) {
-          const unsigned g = gk + jp;
-          ok = pt_wait(&sh.v_full[g & 1], (g >> 1) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
-#pragma unroll 1
-          for (int hf = 0; hf < 2; ++hf) {
-            if (ok) ok = pt_wait(&sh.p_ready[2 * w + hf], n_p, abort_flag, c.err, ERR_TMEM_TIMEOUT);
-            if (!ok) break;
-            if (step == 1 && w == 0 && hf == 0) mbar_arrive(&sh.stagger[0]);
-            tc_fence_after();
-            pt_mma8<PT_PV>(tmem + 256 + w * 128, tmem + w * 128 + hf * 32, v_lo + (g & 1) * (PT_TILE >> 4) + hf * 512, idesc_v, jp != first || hf);
-            tc_commit(&sh.pv_done[2 * w + hf]);
-          }
+      for (int t = 0; t < halves + 2 && ok; ++t) {
+        const int hf = t & 1, j = first + (t >> 1) * step;
+        if (t >= 2) {
+          const unsigned g = gk + j - step;
+          if (hf == 0) ok = pt_wait(&sh.v_full[g & 1], (g >> 1) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
+          if (ok) ok = pt_wait(&sh.p_ready[2 * w + hf], n_p, abort_flag, c.err, ERR_TMEM_TIMEOUT);
           if (!ok) break;
-          n_p ^= 1u;
-          tc_commit(&sh.v_empty[w][g & 1]);
+          tc_fence_after();
+          pt_mma8<PT_PV>(tmem + 256 + w * 128, tmem + w * 128 + hf * 64, v_lo + (g & 1) * (PT_TILE >> 4) + hf * 512, idesc_v, t > 2);
+          tc_commit(&sh.pv_done[2 * w + hf]);
+          if (hf == 1) {
+            n_p ^= 1u;
+            tc_commit(&sh.v_empty[w][g & 1]);
+          }
         }
-        if (j < nb) {
+        if (t < halves) {
           const unsigned g = gk + j;
-          ok = pt_wait(&sh.k_full[g % KS], (g / KS) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
-          // Two tiles: the second gets its scores when the first group has half of its probabilities, the first its next ones after that. The
-          // groups then stay half a block apart; in step they would compete for the exponential unit and leave the tensor cores idle
-          // in turn.
-          if (ok && step == 1 && (w == 1 || n_st > 0)) ok = pt_wait(&sh.stagger[w ^ 1], (n_st - (w ^ 1)) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
+          if (hf == 0) ok = pt_wait(&sh.k_full[g % KS], (g / KS) & 1u, abort_flag, c.err, ERR_MBAR_FULL_TIMEOUT);
           if (!ok) break;
-          pt_mma8<KV8 ? PT_QK8 : PT_QK16>(tmem + w * 128, q_lo + w * (PT_TILE >> 4), k_lo + (g % KS) * (K_BYTES >> 4), idesc, 0);
-          tc_commit(&sh.s_full[w]);
-          mbar_arrive(&sh.s_full[w]);          // hands on what the loader wrote beside the tile (the wait on k_full came before)
-          tc_commit(&sh.k_empty[w][g % KS]);
-          if (step == 1) {
-            if (w == 1) mbar_arrive(&sh.stagger[1]);
-            ++n_st;
-          }
+          pt_mma8<KV8 ? PT_QK8 : PT_QK16>(tmem + w * 128 + hf * 64, q_lo + w * (PT_TILE >> 4), k_lo + (g % KS) * (K_BYTES >> 4) + hf * 512, idesc, 0);
+          tc_commit(&sh.s_full[2 * w + hf]);
+          mbar_arrive(&sh.s_full[2 * w + hf]); // hands on what the loader wrote beside the tile (the wait on k_full came before)
+          if (hf == 1) tc_commit(&sh.k_empty[w][g % KS]);
         }
       }
       gk += nb;
