@@ -574,28 +574,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         const bool bad = sb[0].w != 0.f;
         if (bad && lane == 0) set_error(c.err, ERR_BAD_ARGS);
         const bool edge = __any_sync(0xffffffffu, key0 + PT_KB > vis) || bad;
-        unsigned seen[4] = {~0u, ~0u, ~0u, ~0u};      // bit e of word q: the row sees key q * 32 + e of the block
-        if (edge) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int kc = key0 + q * 32, n = min(max(vis - kc, 0), 32);
-            unsigned w = n == 32 ? ~0u : (1u << n) - 1u;
-            if (mrow != nullptr && n < 32 && kc < s.len) {               // (vis = base: the keys from there on are the call's tokens)
-              unsigned char b[32];
-              const int j0 = kc - s.base, j1 = min(static_cast<int>(min(a.mask_stride, static_cast<long long>(s.n))), s.len - s.base);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) b[e] = j0 + e >= 0 && j0 + e < j1 ? mrow[j0 + e] : 0;     // all in flight at once
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (b[e]) w |= 1u << e;
-            }
-            if (bad) {
-              if (sb[2 * q].x < 0.f) w &= 0xffff0000u;
-              if (sb[2 * q + 1].x < 0.f) w &= 0x0000ffffu;
-            }
-            seen[q] = w;
-          }
-        }
         // Half a block at a time, against the maximum so far: the probabilities are formed and held while this half's own maximum is
         // found; only when it is more than 2^8 above (the first keys, and rarely later) the accumulators are rescaled and the half is done
         // again. No pass for the maximum alone, and the first half's product with V runs under the second half's exponentials. The
@@ -609,23 +587,45 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             if (ok) ok = pt_wait(&sh.s_full[2 * wg + 1], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
             tc_fence_after();
           }
+          // Keys that the row does not see: -infinity, written over their scores here. A branch with the masks between the loads and the arithmetic
+          // below costs every half block 200 cycles of 1600, taken or not.
+          if (edge) {
+#pragma unroll 1
+            for (int q = 2 * hf; q < 2 * hf + 2; ++q) {
+              const int kc = key0 + q * 32, n = min(max(vis - kc, 0), 32);
+              unsigned w = n == 32 ? ~0u : (1u << n) - 1u;               // bit e: the row sees key kc + e
+              if (mrow != nullptr && n < 32 && kc < s.len) {             // (vis = base: the keys from there on are the call's tokens)
+                unsigned char b[32];
+                const int j0 = kc - s.base, j1 = min(static_cast<int>(min(a.mask_stride, static_cast<long long>(s.n))), s.len - s.base);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) b[e] = j0 + e >= 0 && j0 + e < j1 ? mrow[j0 + e] : 0;       // all in flight at once
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (b[e]) w |= 1u << e;
+              }
+              if (bad) {
+                if (sb[2 * q].x < 0.f) w &= 0xffff0000u;
+                if (sb[2 * q + 1].x < 0.f) w &= 0x0000ffffu;
+              }
+              float x[32];
+              pt_ld32(t_s + q * 32, x);
+              pt_mask32(x, w);
+              unsigned y[32];
+#pragma unroll
+              for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(x[e]);
+              __syncwarp();
+              pt_st32(t_s + q * 32, y);
+            }
+            pt_wait_st();
+          }
           for (int turn = 0;; ++turn) {        // (a third turn would only come from scores beyond fp32's whole numbers)
             float v[64];                       // (nothing but waits may stand between the loads and theirs: the registers fill behind the compiler's back)
             __syncwarp();
             pt_ld32_issue(t_s + hf * 64, v);
             pt_ld32_issue(t_s + hf * 64 + 32, v + 32);
-            if (hf == 1 && turn == 0) {        // the first half's probabilities have had time to land
-              pt_wait_st();
-              tc_fence_before();
-              mbar_arrive(&sh.p_ready[2 * wg]);
-            }
             pt_wait_ld();
             pt_pin(v);
             pt_pin(v + 32);
-            if (edge) {
-              pt_mask32(v, hf ? seen[2] : seen[0]);
-              pt_mask32(v + 32, hf ? seen[3] : seen[1]);
-            }
             float mx = -INFINITY;
             const float mo = OFF - (m == -INFINITY ? 0.f : m);
             sum = 0.f;
@@ -677,10 +677,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           l += sum;
           have = true;
           pt_st32(t_s + hf * 64, pk);          // in the place of the scores
+          pt_wait_st();
+          tc_fence_before();
+          mbar_arrive(&sh.p_ready[2 * wg + hf]);                         // (a barrier per half: both may be through before the issuer looks)
         }
-        pt_wait_st();
-        tc_fence_before();
-        mbar_arrive(&sh.p_ready[2 * wg + 1]);  // (a barrier per half: both may be through before the issuer looks)
         ++n_blk;
       }
       // ---- the result ----
