@@ -221,11 +221,11 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.ihb_allreduce_counted.restype = C.c_int
     lib.ihb_dequant_bf16.argtypes = [_vp, _vp, C.c_longlong, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _vp, _vp]
     lib.ihb_dequant_bf16.restype = C.c_int
-    lib.ihb_paged_append.argtypes = [C.POINTER(IhbPagedAppend), _vp]
+    lib.ihb_paged_append.argtypes = [_vp, _vp]                # IhbPagedAppend / IhbPagedAttn, packed bytes or byref
     lib.ihb_paged_append.restype = C.c_int
-    lib.ihb_paged_attention.argtypes = [C.POINTER(IhbPagedAttn), _vp]
+    lib.ihb_paged_attention.argtypes = [_vp, _vp]
     lib.ihb_paged_attention.restype = C.c_int
-    lib.ihb_paged_attention_scratch.argtypes = [C.POINTER(IhbPagedAttn)]
+    lib.ihb_paged_attention_scratch.argtypes = [_vp]
     lib.ihb_paged_attention_scratch.restype = C.c_size_t
     lib.ihb_mega_decode.argtypes = [C.POINTER(IhbMegaArgs), C.c_int, _vp]
     lib.ihb_mega_decode.restype = C.c_int

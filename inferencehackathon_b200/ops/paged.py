@@ -16,7 +16,7 @@ The contiguous, one-sequence siblings are :func:`..lib.qk_norm_rope_kv`, :func:`
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional
 
 import torch
@@ -26,6 +26,12 @@ from . import lib as K
 HEAD_DIM = 128
 PAGE_SIZES = (16, 32, 64, 128)
 _F32, _BF16, _I32, _E4M3 = torch.float32, torch.bfloat16, torch.int32, torch.float8_e4m3fn
+# The argument blocks as bytes (:class:`..lib.IhbPaged`, :class:`..lib.IhbPagedAppend`, :class:`..lib.IhbPagedAttn`; native layout, 0 is
+# NULL): packed in 1 us where filling the structures takes 4.
+_CACHE = "PPPPiiiiiiqPPPP"
+_APPEND = struct.Struct("@" + _CACHE + "PiiqPiqPPfPPiP")
+_ATTN = struct.Struct("@" + _CACHE + "PiiqqPiqqPPqifP")
+_PTR = struct.Struct("@P")
 
 
 # The checks below run on every call, beside kernels that take a few microseconds: plain conditions, messages formed only when they are
@@ -34,7 +40,7 @@ def _bad(what: str) -> None:
     raise ValueError(what)
 
 
-def _cache(T: int, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale, err, dev: int) -> K.IhbPaged:
+def _cache(T: int, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale, err, dev: int) -> tuple:
     """The cache part of an argument block, checked. ``dev``: index of the device that all tensors must be on."""
     shape = k_pages.shape
     if len(shape) != 4 or v_pages.shape != shape or shape[3] != HEAD_DIM:
@@ -52,11 +58,11 @@ def _cache(T: int, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale
     dtype = k_pages.dtype
     if v_pages.dtype != dtype:
         _bad("pages must be bfloat16 or float8_e4m3fn, k and v alike")
-    ksp = vsp = None
+    ksp = vsp = 0
     if dtype == _E4M3:
         if k_scale is None or v_scale is None:
             _bad("e4m3 pages need k_scale and v_scale")
-        per_page = shape[:2]
+        per_page = (n_pages, nkv)
         for s in (k_scale, v_scale):
             if s.dtype != _F32 or s.shape != per_page or not s.is_contiguous() or s.get_device() != dev:
                 _bad("page scales must be contiguous fp32 [n_pages, kv heads] on the pages' device")
@@ -77,7 +83,7 @@ def _cache(T: int, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale
     tstride = block_table.stride()
     if tstride[1] != 1 and tshape[1] != 1:
         _bad("block_table must be int32 [B, blocks] with contiguous rows")
-    cup = ep = None
+    cup = ep = 0
     if cu_q is None:
         if T != B:
             _bad(f"without cu_q there is one token per sequence: {T} tokens, {B} sequences")
@@ -91,19 +97,19 @@ def _cache(T: int, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale
         ep = err.data_ptr()
     if k_pages.get_device() != dev or v_pages.get_device() != dev or kv_len.get_device() != dev or block_table.get_device() != dev:
         _bad("all tensors must be on one device")
-    return K.IhbPaged(kp, vp, ksp, vsp, n_pages, nkv, page, B, T, tshape[1], tstride[0], block_table.data_ptr(), kv_len.data_ptr(), cup, ep)
+    return kp, vp, ksp, vsp, n_pages, nkv, page, B, T, tshape[1], tstride[0], block_table.data_ptr(), kv_len.data_ptr(), cup, ep
 
 
 # the stream pointer without a Stream object around it where this build of torch has that (2 us less per call)
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _launch(fn, args, dev: int, what: str) -> None:
+def _launch(fn, args: bytes, dev: int, what: str) -> None:
     if dev == torch.cuda.current_device():
-        code = fn(C.byref(args), _stream(dev))
+        code = fn(args, _stream(dev))
     else:                                   # the caller's current device is another one: launch on the tensors' own
         with torch.cuda.device(dev):
-            code = fn(C.byref(args), _stream(dev))
+            code = fn(args, _stream(dev))
     if code:
         K.check(code, what)
 
@@ -141,14 +147,14 @@ def paged_append(qkv: torch.Tensor, nq: int, nkv: int, k_pages: torch.Tensor, v_
     if stride[0] & 7 or qp & 15:
         _bad("qkv rows must start on 16-byte boundaries (strides multiples of 8)")
     c = _cache(T, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale, err, dev)
-    if c.nkv != nkv:
-        _bad(f"pages have {c.nkv} KV heads, the call names {nkv}")
+    if c[5] != nkv:
+        _bad(f"pages have {c[5]} KV heads, the call names {nkv}")
     cs = cos_t.shape
     if (len(cs) != 2 or cs[1] != HEAD_DIM // 2 or cs[0] < 1 or sin_t.shape != cs or cos_t.dtype != _F32 or sin_t.dtype != _F32
             or not cos_t.is_contiguous() or not sin_t.is_contiguous()):
         _bad("cos_t and sin_t must be contiguous fp32 [n_pos, 64]")
     cp, sp = cos_t.data_ptr(), sin_t.data_ptr()
-    gq = gk = pp = op = None
+    gq = gk = pp = op = 0
     if q_gamma is not None or k_gamma is not None:
         if q_gamma is None or k_gamma is None:
             _bad("q_gamma and k_gamma come together")
@@ -156,7 +162,7 @@ def paged_append(qkv: torch.Tensor, nq: int, nkv: int, k_pages: torch.Tensor, v_
             if t.dtype != _F32 or t.shape != (HEAD_DIM,) or not t.is_contiguous() or t.get_device() != dev:
                 _bad("gammas must be contiguous fp32 [128] on the pages' device")
         gq, gk = q_gamma.data_ptr(), k_gamma.data_ptr()
-    if (cp | sp | (gq or 0) | (gk or 0)) & 15:
+    if (cp | sp | gq | gk) & 15:
         _bad("rope tables and gammas must start on 16-byte boundaries")
     if positions is not None:
         if positions.dtype != _I32 or positions.shape != (T,) or not positions.is_contiguous() or positions.get_device() != dev:
@@ -177,7 +183,7 @@ def paged_append(qkv: torch.Tensor, nq: int, nkv: int, k_pages: torch.Tensor, v_
         _bad("all tensors must be on one device")
     if dev < 0:
         _bad("the paged cache kernels need CUDA tensors")
-    a = K.IhbPagedAppend(c, qp, dtype == _BF16, nq, stride[0], op, q_bf16, q_stride, gq, gk, eps, cp, sp, cs[0], pp)
+    a = _APPEND.pack(*c, qp, dtype == _BF16, nq, stride[0], op, q_bf16, q_stride, gq, gk, eps, cp, sp, cs[0], pp)
     _launch(K.load().ihb_paged_append, a, dev, "ihb_paged_append")
     return q_out if q_out is not None else qkv[:, :nq * HEAD_DIM].unflatten(1, (nq, HEAD_DIM))
 
@@ -205,9 +211,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if qs[2] != 1 or (qs[0] | qs[1]) & 7 or qp & 15:
         _bad("q strides must be multiples of 8 (the last 1), its start of 16 bytes")
     c = _cache(T, k_pages, v_pages, block_table, kv_len, cu_q, k_scale, v_scale, err, dev)
-    if nq % c.nkv or nq < 1:
-        _bad(f"{nq} query heads do not share {c.nkv} KV heads evenly")
-    if nq > 256 * c.nkv:
+    nkv = c[5]
+    if nq % nkv or nq < 1:
+        _bad(f"{nq} query heads do not share {nkv} KV heads evenly")
+    if nq > 256 * nkv:
         _bad("a KV head can have at most 256 query heads")
     if max_q < 1 or (cu_q is None and max_q != 1):
         _bad("max_q must be positive, and 1 without cu_q")
@@ -215,7 +222,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         scale = HEAD_DIM ** -0.5
     elif not 0.0 < scale < 1e30:
         _bad("scale must be positive and finite")
-    lp = mp = None
+    lp = mp = 0
     mask_stride = 0
     if lse is not None:
         if lse.dtype != _F32 or lse.shape != (T, nq) or not lse.is_contiguous() or lse.get_device() != dev:
@@ -243,9 +250,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             _bad("rows of out overlap")
         if dev < 0:
             _bad("the paged cache kernels need CUDA tensors")
-    a = K.IhbPagedAttn(c, qp, dtype == _BF16, nq, qs[0], qs[1], op, od == _BF16, os[0], os[1], lp, mp, mask_stride, max_q, scale, None)
+    a = _ATTN.pack(*c, qp, dtype == _BF16, nq, qs[0], qs[1], op, od == _BF16, os[0], os[1], lp, mp, mask_stride, max_q, scale, 0)
     lib = K.load()
-    scratch = torch.empty(lib.ihb_paged_attention_scratch(C.byref(a)), dtype=torch.uint8, device=q.device)
-    a.scratch = scratch.data_ptr()
-    _launch(lib.ihb_paged_attention, a, dev, "ihb_paged_attention")
+    scratch = torch.empty(lib.ihb_paged_attention_scratch(a), dtype=torch.uint8, device=q.device)
+    _launch(lib.ihb_paged_attention, a[:-_PTR.size] + _PTR.pack(scratch.data_ptr()), dev, "ihb_paged_attention")
     return out

@@ -203,3 +203,18 @@ def test_a_forked_page_is_copied_when_it_is_written():
 def test_cache_refuses(kw):
     with pytest.raises(ValueError):
         _cache(**kw)
+
+
+def test_packed_argument_blocks_are_the_structures():
+    """Every field of the byte blocks that the entry points pack lies where the C structures have it."""
+    def flat(st):
+        for name, kind in st._fields_:
+            v = getattr(st, name)
+            yield from (flat(v) if isinstance(v, C.Structure) else [v])
+
+    for block, kind in ((paged._APPEND, K.IhbPagedAppend), (paged._ATTN, K.IhbPagedAttn)):
+        n = len([c for c in block.format if c.isalpha()])
+        assert block.size == C.sizeof(kind)
+        values = [i + 1 for i in range(n)]
+        assert [int(v) for v in flat(kind.from_buffer_copy(block.pack(*values)))] == values
+    assert list(flat(K.IhbPagedAttn.from_buffer_copy(paged._ATTN.pack(*values))))[-1] == n and paged._PTR.size == C.sizeof(C.c_void_p)
