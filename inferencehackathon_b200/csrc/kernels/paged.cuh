@@ -65,6 +65,16 @@ static inline bool paged_ok(const IhbPaged& c) {
          c.kv_len != nullptr && (c.cu_q != nullptr || c.B == c.T);
 }
 
+// a / b for 0 <= a < 2^62, b > 0, a quotient below 2^40: two steps in fp32, each leaves 2^-21 of the quotient, and whole corrections. (A 64-bit
+// division, and one in fp64, are subroutines of some hundred dependent instructions, and laying out a segment took eight.)
+__device__ __forceinline__ long long pg_div(long long a, long long b) {
+  const float fb = static_cast<float>(b);
+  long long q = static_cast<long long>(__fdividef(static_cast<float>(a), fb));
+  q += static_cast<long long>(__fdividef(static_cast<float>(a - q * b), fb));
+  while (q * b > a) --q;
+  while ((q + 1) * b <= a) ++q;
+  return q;
+}
 // ---- attention ------------------------------------------------------------------------------------------------------------------
 constexpr float PD_OFF = 6.f;                // e4m3 pages: log2 of what a probability is scaled by (fp16 keeps more small ones)
 constexpr float PD_LAZY = 8.f;               // the running maximum may be passed by 2^8 before the accumulators are rescaled

@@ -92,9 +92,17 @@ __device__ __forceinline__ int pd_find(const IhbPaged& c, int G, int RT, int lan
   before = at;
   return c.B;
 }
-// Ranges: CTA i of `parts` takes positions [i * total / parts, (i + 1) * total / parts).
+// Ranges: the positions in `parts` pieces that differ by one at most, the longer ones first; CTA i takes [at(i), at(i + 1)).
 __device__ __forceinline__ int pd_parts(long long total, int grid) { return static_cast<int>(total < grid ? total : grid); }
-__device__ __forceinline__ long long pd_cut(long long total, int parts, int i) { return total * i / parts; }
+struct PdCuts {
+  long long per, rem;
+  __device__ __forceinline__ PdCuts(long long total, int parts) : per(pg_div(total, max(parts, 1))), rem(total - per * parts) {}
+  __device__ __forceinline__ long long at(int i) const { return per * i + min(static_cast<long long>(i), rem); }
+  __device__ __forceinline__ int of(long long p) const {               // the range that holds position p
+    const long long edge = rem * (per + 1);
+    return static_cast<int>(p < edge ? pg_div(p, per + 1) : rem + pg_div(p - edge, per));
+  }
+};
 
 __device__ __forceinline__ void pd_store(const IhbPagedAttn& a, int t, int h, int ch, float v) {
   const size_t o = static_cast<size_t>(t) * a.out_stride_t + static_cast<size_t>(h) * a.out_stride_h + ch;
@@ -166,8 +174,9 @@ __global__ void __launch_bounds__(PD_WARPS * 32, PdSmem<NT, KV8, QT>::PER_SM) pa
   const long long total = pd_total(c, G, RT, lane);
   const int parts = pd_parts(total, grid);
   if (static_cast<int>(blockIdx.x) >= parts) return;
-  long long u = pd_cut(total, parts, blockIdx.x);
-  const long long u_end = pd_cut(total, parts, blockIdx.x + 1), u_first = u;
+  const PdCuts cuts(total, parts);
+  long long u = cuts.at(blockIdx.x);
+  const long long u_end = cuts.at(blockIdx.x + 1), u_first = u;
   long long before;
   int b = pd_find(c, G, RT, lane, u, before);
   PgSeq s = pg_seq(c, b);
@@ -181,7 +190,8 @@ __global__ void __launch_bounds__(PD_WARPS * 32, PdSmem<NT, KV8, QT>::PER_SM) pa
       s = pg_seq(c, b);
       w = pd_work(c, s, G, RT);
     }
-    const int span = w.units + PD_START, item = static_cast<int>((u - before) / span), at = static_cast<int>((u - before) % span);
+    const int span = w.units + PD_START, item = static_cast<int>(pg_div(u - before, span));
+    const int at = static_cast<int>(u - before - static_cast<long long>(item) * span);
     const int taken = static_cast<int>(min(static_cast<long long>(span - at), u_end - u));
     const int unit0 = max(at - PD_START, 0), n_units = at + taken - PD_START - unit0;
     if (n_units <= 0) {                       // only start-up cost of the item lies in this range
@@ -610,16 +620,12 @@ __global__ void __launch_bounds__(WPR == 1 ? 128 : WPR * 32) paged_fold_kernel(c
     const PdWork w = pd_work(c, s, G, RT);
     lo += static_cast<long long>(left) * (w.units + PD_START);
     const long long hi = lo + w.units + PD_START, key0 = lo + PD_START;
-    const int parts = pd_parts(total, grid);
-    first = static_cast<int>(key0 * parts / total);            // the range that holds the item's first unit
-    while (first + 1 < parts && pd_cut(total, parts, first + 1) <= key0) ++first;
-    while (first > 0 && pd_cut(total, parts, first) > key0) --first;
-    last = static_cast<int>((hi - 1) * parts / total);         // the range that holds its last unit
-    while (last + 1 < parts && pd_cut(total, parts, last + 1) < hi) ++last;
-    while (last > first && pd_cut(total, parts, last) >= hi) --last;
+    const PdCuts cuts(total, pd_parts(total, grid));
+    first = cuts.of(key0);                                     // the range that holds the item's first unit
+    last = cuts.of(hi - 1);                                    // the range that holds its last unit
     kvh = left / w.tiles;
     row0 = (left % w.tiles) * RT;
-    slot0 = pd_cut(total, parts, first) >= lo ? 0 : 1;         // the first piece is its range's last segment: slot 1, or 0 if the only one
+    slot0 = cuts.at(first) >= lo ? 0 : 1;         // the first piece is its range's last segment: slot 1, or 0 if the only one
   }
   pdl_wait();
   if (b < 0 || first == last) return;                          // one range had all of it and has written the result

@@ -61,16 +61,6 @@ struct PtHdr {
   PtSeg seg[PT_SEGS];
 };
 
-// a / b for 0 <= a < 2^62, b > 0, a quotient below 2^40: two steps in fp32, each leaves 2^-21 of the quotient, and whole corrections. (A 64-bit
-// division, and one in fp64, are subroutines of some hundred dependent instructions, and laying out a segment took eight.)
-__device__ __forceinline__ long long pt_div(long long a, long long b) {
-  const float fb = static_cast<float>(b);
-  long long q = static_cast<long long>(__fdividef(static_cast<float>(a), fb));
-  q += static_cast<long long>(__fdividef(static_cast<float>(a - q * b), fb));
-  while (q * b > a) --q;
-  while ((q + 1) * b <= a) ++q;
-  return q;
-}
 // First position of CTA i's range: `total` in PT_MAX_GRID parts that differ by one at most (a division by a constant).
 __device__ __forceinline__ long long pt_cut(long long total, int i) {
   const long long per = total / PT_MAX_GRID;
@@ -127,11 +117,11 @@ struct PtIter {
         w = pt_work(p, s, G, RT);
         all = w.head * p.c.nkv;
       }
-      g.kvh = static_cast<int>(pt_div(u - before, w.head));
+      g.kvh = static_cast<int>(pg_div(u - before, w.head));
       const long long q = u - before - g.kvh * w.head;
       long long j;
       if (w.d == 0) {
-        j = pt_div(q, w.a);
+        j = pg_div(q, w.a);
       } else {
         const float h = static_cast<float>(w.a) + 0.5f * static_cast<float>(w.d), fq = static_cast<float>(q);    // the root that cancels nothing
         j = static_cast<long long>(__fdividef(2.f * fq, h + sqrtf(h * h + 2.f * static_cast<float>(w.d) * fq)));
@@ -150,8 +140,8 @@ struct PtIter {
       g.seen_end = p.mask != nullptr ? s.len : min(s.len, s.base + i_last + 1);
       g.all_see = max(0, p.mask != nullptr ? s.base : min(s.base + g.row0 / G + 1, s.len));
       g.nblk = max(1, (g.seen_end + PT_KB - 1) / PT_KB);
-      g.blk0 = v0 == 0 ? 0 : static_cast<int>(pt_div(v0 * g.nblk, len));
-      g.blk1 = v1 == len ? g.nblk : static_cast<int>(pt_div(v1 * g.nblk, len));
+      g.blk0 = v0 == 0 ? 0 : static_cast<int>(pg_div(v0 * g.nblk, len));
+      g.blk1 = v1 == len ? g.nblk : static_cast<int>(pg_div(v1 * g.nblk, len));
       g.first_in_range = u == u0;
       u += v1 - v0;
       if (g.blk0 < g.blk1 || g.blk0 > 0) return true;
