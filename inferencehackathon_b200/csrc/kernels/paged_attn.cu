@@ -5,17 +5,25 @@
 // The rows of a (sequence, KV head) are its (token, query head) pairs, RT = 8 or 16 of them per tile. Scores are computed
 // transposed, S^T = K Q^T with m16n8k16 (16 keys x 8 rows), and so is the output, O^T = V^T P^T: the large operand is the A operand
 // of both products and a thread's fragments of it are contiguous bytes of the cache (the channel order inside a product is free,
-// so a thread takes 16 neighbouring bytes), so K and V go from global memory to registers in 16-byte loads and never touch
-// shared memory. With queries as the A operand (the usual way round) 8 query heads would waste half of every product.
+// so a thread takes 16 neighbouring bytes). With queries as the A operand (the usual way round) 8 query heads would waste half of
+// every product. Each warp walks its own keys, 16 per step (bf16 pages) or 32 (e4m3: two groups share the query fragments and the
+// step's overhead: 75 -> 67 us at 64 sequences of 129 to 8191 keys), through a ring of asynchronous 16-byte copies in shared memory that
+// only it reads: no barrier until the four warps' results are added at the end of an item.
 //
 // e4m3 pages: bytes become fp16 exactly; q is scaled per row by a power of two into fp16 (head and remainder for fp32
 // queries: 22 bits); the K scale is a factor of the score, the V scale s_v goes into the exponent of the probability: with
 // m the running maximum of score + log2 s_v, O = sum 2^(s + log2 s_v - m) v_bytes and l = sum 2^(s - m). The probability that
 // meets the bytes is then at most 2^14 whatever the scales are, which is what fp16 holds.
 //
-// Work split: the 64-key units of all (sequence, head, tile) items are laid end to end and cut into equal ranges, one per CTA, so
+// Work split: the 128-key units of all (sequence, head, tile) items are laid end to end and cut into equal ranges, one per CTA, so
 // ragged batches and single long sequences load every SM the same. Lengths are read on the device. An item cut by a range end
-// leaves one record (O, m, l) per piece, folded by a second kernel in a fixed order: results do not depend on timing.
+// leaves one record (O, m, l) per piece, folded by a second kernel in a fixed order: results do not depend on timing. The folding
+// kernel is launched with the first one and works out its pieces while that runs.
+//
+// Measured (64 query heads, 4 KV heads): 64 sequences of 129 to 8191 keys, e4m3 pages, 64 us, 66 % of the measured copy bandwidth; one
+// sequence of 131071 keys 42 us, 50 %; bf16 pages of 16 tokens, 32 / 4 heads, fp32 queries, 24 sequences of up to 4096 keys, 29 us, 52 %.
+// Bound by instructions and their latency: 47 % of the issue slots at 12
+// warps per SM (shared memory for the rings), each 16-byte chunk of e4m3 being eight conversions and two matrix instructions.
 #include "paged.cuh"
 #include "paged_tiles.h"
 
@@ -42,9 +50,10 @@ __device__ __forceinline__ unsigned pd_movt(unsigned x) {       // transpose of 
 __device__ __forceinline__ unsigned pd_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // ---- work items ------------------------------------------------------------------------------------------------------------
-// An item costs its units and PD_START more (loading Q, filling the ring, adding the warps up): ranges are cut on that cost, so a CTA
+// An item costs its units and PD_START more (loading Q, filling the ring, adding the warps up; 64 sequences of e4m3 pages: 2 73 us, 3 68, 4 64,
+// 6 66): ranges are cut on that cost, so a CTA
 // with many short items gets fewer keys. Positions inside an item: [0, PD_START) start-up, then the units.
-constexpr int PD_START = 3;
+constexpr int PD_START = 4;
 
 struct PdWork {
   int tiles, units, items;       // of one sequence: row tiles, units per item, items = nkv * tiles

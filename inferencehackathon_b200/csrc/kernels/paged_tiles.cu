@@ -8,14 +8,21 @@
 //   warps 8-11       bring V: page lookups, 16-byte asynchronous copies, e4m3 -> fp16 on the way into the swizzled tile
 //   warps 14, 15     bring K, and the page scales. e4m3 K needs no conversion: a bf16 query row, scaled by a power of two, is the sum of two
 //                    e4m3 rows (8 significant bits: 4 + 4), so S = Qhi K^T + Qlo K^T runs on e4m3 products, which are twice as fast
-//   warps 12, 13     one issuer per tile (waits, fences and commits cost it more than the products' issue): S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory, V as an MN-major operand: the
-//                    rows of the cache are used as they lie, no transpose)
-// While one group computes its softmax the tensor cores work for the other. A sequence with at most 128 rows gives both groups the
-// same rows: they take the even and the odd key blocks, and their results are added up at the end.
+//   warps 12, 13     one issuer per tile (waits, fences and commits cost it more than the products' issue): S = Q K^T (both operands
+//                    in shared memory) and O += P V (P in tensor memory, V as an MN-major operand: the rows of the cache are used as
+//                    they lie, no transpose)
+// Scores live in two halves of 64 keys: while a group computes the probabilities of one half the tensor cores multiply the other's
+// with V and form the next block's scores in their place, so that the group does not wait for them (prompt of 8000 tokens: 1160 us
+// with whole blocks in turn, 1040 with halves, 990 with the masks out of the hot loop). A sequence with at most 128 rows gives both
+// groups the same rows: they take the even and the odd key blocks, and their results are added up at the end.
 // The accumulators are rescaled only when a row's maximum has grown by more than 2^8 since the last time.
 //
 // Work split as in paged_attn.cu: items (sequence, KV head, pair of tiles) are laid end to end, with lengths that follow their causal
 // key ranges, and cut into one equal range per SM; pieces of a cut item are folded by a second kernel.
+//
+// Bound by the groups' latency: a half block is 512 cycles of the exponential unit per warp, two warps share the unit, and a half takes 2050
+// cycles with loads from tensor memory, conversion, vote, store and hand-over. The tensor pipe is busy half of the time. Per segment
+// 5 us of set-up and result, most of what a batch of short windows costs.
 #include "paged.cuh"
 #include "paged_tiles.h"
 #include "tc_common.cuh"
@@ -36,7 +43,12 @@ constexpr int PT_RAW = 128 * PG_HD;             // e4m3 bytes of a key block's K
 template <bool KV8>
 constexpr int pt_smem() { return PT_HDR + 6 * PT_TILE + (KV8 ? 2 * PT_RAW : 0); }
 constexpr int PT_MAX_GRID = 148;              // one CTA per SM
-constexpr int PT_START = 512;                  // start-up cost of an item, in keys
+// Start-up cost of an item, in keys (a prompt of 4096 tokens, chunks of 4 sequences: 256 258 / 359 us, 384 221 / 360, 512 201 / 357,
+// 768 200 / 354).
+constexpr int PT_START = 512;
+// A cut nearer than this to an end of its item, in keys, moves there: a short piece costs more (set-up, a record, its part in the fold) than the
+// longer range. At most half a range, which bounds what one CTA can be given on top (token trees of 8 sequences 50 -> 44 us; a quarter 50).
+constexpr int PT_SNAP = 1024;
 
 constexpr int PT_SEGS = 4;
 // A piece of an item: rows [row0, row0 + rows) of a sequence's KV head, key blocks [blk0, blk1) of nblk.
@@ -92,13 +104,14 @@ __device__ __forceinline__ long long pt_prefix(const PtWork& w, long long j) { r
 
 // The segments of a CTA's range, in order.
 struct PtIter {
-  long long u, u_end, u0, before;
+  long long u, u_end, u0, before, snap;
   int b;
   PgSeq s;
   PtWork w;
   __device__ __forceinline__ void start(const IhbPagedAttn& p, int G, int RT, long long total, long long before_, int b_) {
     u0 = u = pt_cut(total, blockIdx.x);
     u_end = pt_cut(total, blockIdx.x + 1);
+    snap = min(static_cast<long long>(PT_SNAP) * G, total / (2 * PT_MAX_GRID));
     before = before_;
     b = b_;
     if (u < u_end) {
@@ -130,7 +143,10 @@ struct PtIter {
         while (j + 1 < w.tiles && pt_prefix(w, j + 1) <= q) ++j;
       }
       const long long lo = pt_prefix(w, j), len = w.a + w.d * (j + 1);
-      const long long v0 = q - lo, v1 = min(len, v0 + (u_end - u));
+      const long long p0 = q - lo, p1 = min(len, p0 + (u_end - u));
+      // (a position is moved the same way by the CTA that ends there and by the one that begins)
+      auto snapped = [&](long long v) { return v == len ? v : v < snap ? 0 : len - v < snap ? len : v; };
+      const long long v0 = snapped(p0), v1 = snapped(p1);
       g.b = b;
       g.s = s;
       g.last = 0;
@@ -143,8 +159,8 @@ struct PtIter {
       g.blk0 = v0 == 0 ? 0 : static_cast<int>(pg_div(v0 * g.nblk, len));
       g.blk1 = v1 == len ? g.nblk : static_cast<int>(pg_div(v1 * g.nblk, len));
       g.first_in_range = u == u0;
-      u += v1 - v0;
-      if (g.blk0 < g.blk1 || g.blk0 > 0) return true;
+      u += p1 - p0;
+      if (g.blk0 < g.blk1 || (g.blk0 > 0 && v0 < len)) return true;
     }
     return false;
   }
