@@ -218,3 +218,13 @@ def test_packed_argument_blocks_are_the_structures():
         values = [i + 1 for i in range(n)]
         assert [int(v) for v in flat(kind.from_buffer_copy(block.pack(*values)))] == values
     assert list(flat(K.IhbPagedAttn.from_buffer_copy(paged._ATTN.pack(*values))))[-1] == n and paged._PTR.size == C.sizeof(C.c_void_p)
+
+
+def test_more_query_heads_per_kv_head_than_the_work_split_counts_are_refused():
+    a = _attn_args(q=torch.zeros(3, 2 * 257, 128))
+    with pytest.raises(ValueError, match="256 query heads"):
+        paged.paged_attention(a.pop("q"), **a)
+    lib = K.load()
+    c = K.IhbPaged(k=16, v=16, n_pages=4, nkv=1, page=16, B=1, T=1, max_blocks=1, block_table=16, kv_len=16)
+    b = K.IhbPagedAttn(c=c, q=16, nq=257, out=16, max_q=1, scratch=16, q_stride_t=8, q_stride_h=8)
+    assert lib.ihb_paged_attention(C.byref(b), None) != 0
