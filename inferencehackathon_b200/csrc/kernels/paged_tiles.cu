@@ -726,8 +726,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         const bool odd = *reinterpret_cast<volatile int*>(&sh.odd) != 0;
         const int slot = sg.first_in_range ? 0 : 1;
         const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-        const uint32_t stage = smem_u32(sq) + (pair ? wg * PT_TILE + quarter * 8192 : quarter * 16384);      // the warp's rows, 256 bytes each
-        const int stage_row = pair ? 256 : 512;                          // (not a pair: at the head of the row's handed-over 512 bytes)
+        // The stage, 256 bytes per row. A pair's: rows 0 to 15 and 16 to 31 in the two pieces of 4 KB that the warp's own queries have, nowhere else: the
+        // group's other warps may be loading their next queries by now. Not a pair's: at the head of the row's handed-over 512 bytes (hand[1] orders it).
+        const uint32_t stage = smem_u32(sq) + (pair ? wg * PT_TILE + quarter * 4096 : quarter * 16384);
+        const int stage_row = pair ? 256 : 512, stage_gap = pair ? PT_HALF - 4096 : 0;
+        const uint32_t mine = stage + lane * stage_row + (lane >> 4) * stage_gap;
         const bool wide_out = ((a.out_stride_t | a.out_stride_h) & 7) == 0;
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
@@ -761,7 +764,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 }
               }
             }
-          // into the row's 256 bytes of the stage (the place of Q), and out in whole rows when they are full
+          // into the row's 256 bytes of the stage, and out in whole rows when they are full
           if (whole) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] *= inv;
@@ -769,13 +772,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           if (whole && a.out_bf16) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              pt_sts(stage + lane * stage_row + (((q * 4 + e) ^ (lane & 7)) << 4),
+              pt_sts(mine + (((q * 4 + e) ^ (lane & 7)) << 4),
                      make_uint4(pd_pack<false>(v[8 * e], v[8 * e + 1]), pd_pack<false>(v[8 * e + 2], v[8 * e + 3]), pd_pack<false>(v[8 * e + 4], v[8 * e + 5]),
                                 pd_pack<false>(v[8 * e + 6], v[8 * e + 7])));
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              pt_sts(stage + lane * stage_row + ((((q & 1) * 8 + e) ^ (lane & 7)) << 4),
+              pt_sts(mine + ((((q & 1) * 8 + e) ^ (lane & 7)) << 4),
                      make_uint4(__float_as_uint(v[4 * e]), __float_as_uint(v[4 * e + 1]), __float_as_uint(v[4 * e + 2]), __float_as_uint(v[4 * e + 3])));
           }
           if (whole && a.out_bf16 ? q != 3 : !(q & 1)) continue;
@@ -786,7 +789,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
 #pragma unroll 4
             for (int i = 0; i < 16; ++i) {
               const int rl = 2 * i + (lane >> 4);
-              if (2 * i < n) *reinterpret_cast<uint4*>(d + 2 * i * PD_REC) = pt_lds(stage + rl * stage_row + ((ch ^ (rl & 7)) << 4));
+              if (2 * i < n) *reinterpret_cast<uint4*>(d + 2 * i * PD_REC) = pt_lds(stage + rl * stage_row + (rl >> 4) * stage_gap + ((ch ^ (rl & 7)) << 4));
             }
             __syncwarp();
             continue;
@@ -797,7 +800,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
 #pragma unroll 4
           for (int i = 0; i < 16; ++i) {
             const int rl = 2 * i + (lane >> 4), rr = first + 2 * i;
-            const uint4 x = pt_lds(stage + rl * stage_row + ((ch ^ (rl & 7)) << 4));
+            const uint4 x = pt_lds(stage + rl * stage_row + (rl >> 4) * stage_gap + ((ch ^ (rl & 7)) << 4));
             const size_t o = o0 + static_cast<size_t>(h) * a.out_stride_h;
             for (h += 2; h >= G; h -= G) o0 += a.out_stride_t;           // two rows on
             if (rr >= sg.rows) continue;

@@ -1,0 +1,114 @@
+"""Paged cache kernels at the edges of what their entry points allow, against plain 64-bit implementations (needs a B200).
+
+Tolerance of an attention output: probabilities that are each off by a relative d move it by at most 2 d sum_j p_j |v_j| (numerator and
+denominator); d is the rounding of P (fp16 2^-11 for bf16 queries over e4m3 pages, fp16 pairs 2^-22 for fp32 ones, bf16 pairs 2^-16, one bf16 2^-8), the
+error of the scores (see test_paged_gpu.py) and 2^-17 for fp32 sums and exponents; then half a step of the output type."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import paged_oracle as O
+from inferencehackathon_b200.ops import paged
+
+DEV = "cuda:0"
+F64 = torch.float64
+
+
+def _io(name):
+    return torch.bfloat16 if name == "bf16" else torch.float32
+
+
+def _reference(k, v, ks, vs, q, table, lens, news, nkv, mask=None, scale=128 ** -0.5):
+    """out, lse, sum_j p_j |v_j| [T, nq, 128 / - / 128] in 64 bits. NaN and infinities of V reach the rows that see them, in their channel."""
+    T, nq = q.shape[:2]
+    G = nq // nkv
+    out = torch.full((T, nq, 128), float("nan"), dtype=F64)
+    mag, lse = out.clone(), torch.full((T, nq), float("nan"), dtype=F64)
+    P, t = k.shape[2], 0
+    for b, (L, n) in enumerate(zip(lens, news)):
+        if n == 0:
+            continue
+        base, ids = L - n, table[b, :-(-L // P)].long()
+        j = torch.arange(L)[None, :]
+        i = torch.arange(n)[:, None]
+        if mask is None:
+            see = j <= base + i
+        else:
+            see = (j < base) | torch.nn.functional.pad(mask[t:t + n, :n].bool(), (base, 0))
+        for h in range(nkv):
+            kk, vv = k[ids, h].to(F64), v[ids, h].to(F64)
+            if ks is not None:
+                kk, vv = kk * ks[ids, h].to(F64)[:, None, None], vv * vs[ids, h].to(F64)[:, None, None]
+            kk, vv = kk.reshape(-1, 128)[:L].to(DEV), vv.reshape(-1, 128)[:L].to(DEV)
+            odd = ~torch.isfinite(vv)
+            clean = vv.masked_fill(odd, 0.0)
+            s = see.to(DEV)
+            for g in range(h * G, (h + 1) * G):
+                w = (q[t:t + n, g].to(F64).to(DEV) @ kk.T * scale).masked_fill(~s, -math.inf)
+                m = torch.logsumexp(w, 1, keepdim=True)
+                p = torch.where(torch.isinf(m), torch.zeros_like(w), torch.exp(w - m))
+                o = p @ clean
+                if bool(odd.any()):
+                    hit = s.to(F64) @ torch.isnan(vv).to(F64) > 0
+                    for c in torch.isinf(vv).any(0).nonzero().flatten().tolist():
+                        for r in torch.isinf(vv[:, c]).nonzero().flatten().tolist():
+                            o[s[:, r], c] += vv[r, c]
+                    o[hit] = float("nan")
+                out[t:t + n, g], lse[t:t + n, g], mag[t:t + n, g] = o.cpu(), m[:, 0].cpu(), (p @ clean.abs()).cpu()
+        t += n
+    return out, lse, mag
+
+
+def _check(out, ref, mag, d, out_io):
+    got = out.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(torch.isinf(got), torch.isinf(ref))
+    fin = torch.isfinite(ref)
+    tol = 2 * d * mag + ref.abs() * (torch.finfo(_io(out_io)).eps / 2)
+    far = ((got - ref).abs() - tol)[fin]
+    assert float(far.max()) <= 0, (float((got - ref)[fin].abs().max()), int((far > 0).sum()))
+
+
+def _score_bound(q, k, ks, cache, io, tiles, scale=128 ** -0.5):
+    """Largest error of a score: what the queries' split loses (test_paged_gpu.py) times |q| |k| scale, and fp32 sums."""
+    kk = torch.nan_to_num(k.to(F64) * (1.0 if ks is None else ks[:, :, None, None].to(F64)))
+    smax = float(q.to(F64).norm(dim=-1).max()) * float(kk.norm(dim=-1).max()) * scale
+    e = (2.0 ** -17 * 128 ** 0.5 if tiles and cache == "fp8" else 0.0) if io == "bf16" else (2.0 ** -22 if cache == "fp8" else 2.0 ** -16)
+    return e * smax + 2.0 ** -17
+
+
+def _p_step(cache, io, tiles):
+    if cache == "fp8":
+        return 2.0 ** -11 if io == "bf16" else 2.0 ** -22
+    return 2.0 ** -8 if tiles and io == "bf16" else 2.0 ** -16
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+def test_many_tile_pairs_per_block_with_values_that_are_not_finite(cache):
+    """Several items of two tiles for every SM, ragged last tiles, and NaN in V rows of some windows: their rows take much longer in the epilogue than
+    the others' of the same tile, whose warps must not touch what is staged for them meanwhile."""
+    gen = torch.Generator().manual_seed(41)
+    nq, nkv, page, B = 16, 4, 32, 44
+    news = [100 + 7 * (b * 5 % 19) for b in range(B)]
+    lens = [n + (0 if b % 3 == 0 else 13 * (b % 7)) for b, n in enumerate(news)]
+    table, n_pages = O.tables(lens, page, gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+    for b in range(0, B, 3):
+        row = lens[b] - news[b] + news[b] // 2 + b % 5
+        v[int(table[b, row // page]), b % nkv, row % page, 3 * b % 128] = torch.tensor(float("nan")).to(v.dtype)
+    q = torch.randn(sum(news), nq, 128, generator=gen).to(torch.bfloat16)
+    ref, ref_lse, mag = _reference(k, v, ks, vs, q, table, lens, news, nkv)
+    d = _p_step(cache, "bf16", True) + _score_bound(q, k, ks, cache, "bf16", True)
+    dev = [None if t is None else t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news))]
+    ld = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    lse = torch.empty(q.shape[:2], device=DEV)
+    first = None
+    for _ in range(4):
+        out = paged.paged_attention(*dev[:4], ld, cu_q=dev[6], max_q=max(news), k_scale=dev[4], v_scale=dev[5], lse=lse, err=err)
+        _check(out, ref, mag, d, "bf16")
+        assert int(err) == 0 and float((lse.double().cpu() - ref_lse).abs().max()) <= _score_bound(q, k, ks, cache, "bf16", True)
+        first = out if first is None else first
+        assert torch.equal(out.view(torch.int16), first.view(torch.int16))
