@@ -283,7 +283,8 @@ int ihb_moe_combine_rows(const float* yg, const int* inv, const float* tw, int k
 // sequence in the call (NULL: one token per sequence, T == B); token i of the n of sequence b stands at row kv_len[b] - n + i.
 // Tokens behind cu_q[B] are left alone. Everything that depends on lengths is read on the device: a captured graph replays
 // with other lengths. err (optional): ERR_BAD_ARGS when a page id, a position or a length does not fit; the rows
-// concerned are then skipped (append) or not seen (attention), nothing out of range is touched.
+// concerned are then skipped (append) or not seen (attention), nothing out of range is touched. An attention kernel whose internal wait
+// ran out leaves NaN in the call's rows and ERR_MBAR_* / ERR_TMEM_TIMEOUT in err.
 typedef struct {
   void* k;
   void* v;

@@ -66,6 +66,7 @@ constexpr int PT_SC = 8;                       // blocks whose page scales are k
 struct PtHdr {
   uint64_t k_full[4], k_empty[2][4], v_full[2], v_empty[2][2];         // empty: [group that used it][stage]
   uint64_t q_full[2], q_free, s_full[4], p_ready[4], pv_done[4], hand[2];     // s_full .. pv_done: [group][half of the block]
+  uint64_t drain[2];                           // an issuer's products are over (after a wait that ran out)
   uint32_t tmem;
   int abort_flag;
   int odd;                                     // V values that are not finite were met in keys that not every row sees (set by the loader)
@@ -167,7 +168,9 @@ struct PtIter {
 };
 
 // What a CTA tells the folding kernel. cont: the CTA's first segment continues an item of the CTA before (1: without a block of its
-// own, 2: with a piece in slot 0), ends: and ends it. tail: the CTA's last segment is the first piece of a cut item, in slot `slot`.
+// own, 2: with a piece in slot 0; PT_LOST: one of the CTA's waits ran out, nothing it left may be used), ends: and ends it. tail: the CTA's
+// last segment is the first piece of a cut item, in slot `slot`.
+constexpr int PT_LOST = -1;
 struct PtDesc {
   int cont, ends, tail, slot;
   int b, kvh, row0, rows;
@@ -449,6 +452,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       for (int j = 0; j < 4; ++j) mbar_init(&sh.k_empty[i][j], 1);
       for (int j = 0; j < 2; ++j) mbar_init(&sh.v_empty[i][j], 1);
       mbar_init(&sh.v_full[i], 128);
+      mbar_init(&sh.drain[i], 1);
       mbar_init(&sh.q_full[i], 128); mbar_init(&sh.s_full[2 * i], 2); mbar_init(&sh.s_full[2 * i + 1], 2);
       mbar_init(&sh.p_ready[2 * i], 128); mbar_init(&sh.p_ready[2 * i + 1], 128); mbar_init(&sh.pv_done[2 * i], 1); mbar_init(&sh.pv_done[2 * i + 1], 1);
     }
@@ -1125,6 +1129,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {                           // products may be under way: what they use is given back after them
+    if (tid == 0) descs[blockIdx.x].cont = PT_LOST;
+    const int w = warp - PT_MMA_WARP;
+    if ((w == 0 || w == 1) && lane == 0) {
+      tc_commit(&sh.drain[w]);
+      const unsigned long long t0 = globaltimer_ns();
+      while (!mbar_try_wait(&sh.drain[w], 0) && globaltimer_ns() - t0 < IHB_LOCAL_WAIT_NS) {}
+    }
+    __syncthreads();
+  }
   if (warp == PT_MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
@@ -1138,21 +1152,33 @@ __global__ void __launch_bounds__(256) paged_tiles_fold_kernel(const __grid_cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.nq / a.c.nkv;
   pdl_wait();
   const PtDesc d = descs[blockIdx.x];
+  if (d.cont == PT_LOST) {
+    // A wait of this CTA ran out, so its items are not all done: NaN for the call's tokens, so that no caller takes what the memory held for a result.
+    const int t0 = a.c.cu_q != nullptr ? max(a.c.cu_q[0], 0) : 0, t1 = a.c.cu_q != nullptr ? min(a.c.cu_q[a.c.B], a.c.T) : a.c.T;
+    const float nan = __uint_as_float(0x7fffffffu);
+    for (int t = t0 + blockIdx.y; t < t1; t += gridDim.y)
+      for (int h = warp; h < a.nq; h += 8) {
+        pd_store4(a, t, h, lane * 4, make_float4(nan, nan, nan, nan));
+        if (lane == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(t) * a.nq + h] = nan;
+      }
+    return;
+  }
   if (!d.tail) return;
   if (warp == 0) {
-    int n = 1;
+    int n = 1, lost = 0;
     if (lane == 0) list[0] = blockIdx.x * 2 + d.slot;
     for (int y0 = blockIdx.x + 1; y0 < grid; y0 += 32) {
       PtDesc e = {0, 0, 0, 0, 0, 0, 0, 0};
       if (y0 + lane < grid) e = descs[y0 + lane];
-      const unsigned stop = __ballot_sync(0xffffffffu, e.ends || e.cont == 0);
+      const unsigned stop = __ballot_sync(0xffffffffu, e.ends || e.cont == 0 || e.cont == PT_LOST);
       const int upto = stop ? __ffs(stop) - 1 : 31;                    // (this lane included: the piece that ends the item)
       const unsigned mine = __ballot_sync(0xffffffffu, lane <= upto && e.cont == 2);
       if (lane <= upto && e.cont == 2) list[n + __popc(mine & ((1u << lane) - 1u))] = (y0 + lane) * 2;
       n += __popc(mine);
+      lost = __any_sync(0xffffffffu, lane <= upto && e.cont == PT_LOST);
       if (stop) break;
     }
-    if (lane == 0) n_s = n;
+    if (lane == 0) n_s = lost ? 0 : n;
   }
   __syncthreads();
   const int n = n_s;
@@ -1173,6 +1199,7 @@ __global__ void __launch_bounds__(256) paged_tiles_fold_kernel(const __grid_cons
       if (f != 0.f) { acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w; }
     }
     const int tok = (d.row0 + r) / G, head = d.kvh * G + (d.row0 + r) % G;
+    if (n == 0) L = __uint_as_float(0x7fffffffu);                        // a piece is missing: NaN, as its CTA left for its own rows
     const float inv = L == 0.f ? 0.f : 1.f / L;
     pd_store4(a, s.t0 + tok, head, lane * 4, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     if (lane == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(s.t0 + tok) * a.nq + head] = pd_lse<KV8>(M, L);

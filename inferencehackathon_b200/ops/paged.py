@@ -9,7 +9,8 @@ of sequence ``b`` stands at row ``kv_len[b] - n + i``; ``kv_len[b] <= 0`` marks 
 Lengths and tables live on the device: nothing here synchronises, and a captured graph replays with other lengths in the same
 tensors. Kernels run on the current stream of the device that holds the tensors; scratch comes from PyTorch's allocator for each
 call, so calls on different streams and graphs share nothing. A page id or position that does not fit sets ``err``
-(:data:`..lib.ERR_NAMES` 6) and its rows are left out; nothing out of range is read or written.
+(:data:`..lib.ERR_NAMES` 6) and its rows are left out; nothing out of range is read or written. A kernel whose internal wait ran out (a
+device fault) leaves NaN in the call's rows, whether there is an ``err`` or not.
 
 The contiguous, one-sequence siblings are :func:`..lib.qk_norm_rope_kv`, :func:`..lib.qk_norm_rope_rows`,
 :func:`..lib.flash_decode` and :func:`..lib.window_attention`; :class:`..runtime.paged_kv.PagedKVCache` owns pages and tables.

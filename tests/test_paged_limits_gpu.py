@@ -112,3 +112,35 @@ def test_many_tile_pairs_per_block_with_values_that_are_not_finite(cache):
         assert int(err) == 0 and float((lse.double().cpu() - ref_lse).abs().max()) <= _score_bound(q, k, ks, cache, "bf16", True)
         first = out if first is None else first
         assert torch.equal(out.view(torch.int16), first.view(torch.int16))
+
+
+class _DirtyEmpty:
+    """torch for the module under test, with every new tensor full of 0xff bytes."""
+
+    def __getattr__(self, name):
+        return getattr(torch, name)
+
+    def empty(self, *a, **kw):
+        t = torch.empty(*a, **kw)
+        t.view(torch.uint8).fill_(255)
+        return t
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("lens,news,nq,nkv", [([900, 1, 3000], [1, 1, 1], 16, 2), ([700, 90, 2500], [300, 90, 40], 16, 2), ([40, 0], [40, 0], 8, 1)])
+def test_scratch_may_hold_anything(cache, lens, news, nq, nkv, monkeypatch):
+    """The pieces that a second kernel folds are read only where the first one wrote them."""
+    gen = torch.Generator().manual_seed(7)
+    table, n_pages = O.tables(lens, 64, gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, 64, cache, gen)
+    q = torch.randn(sum(news), nq, 128, generator=gen).to(torch.bfloat16)
+    q, k, v, table, ks, vs, cu = [None if t is None else t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news))]
+    ld = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    outs = []
+    for dirty in (False, True):
+        if dirty:
+            monkeypatch.setattr(paged, "torch", _DirtyEmpty())
+        out = torch.zeros_like(q)
+        paged.paged_attention(q, k, v, table, ld, cu_q=cu, max_q=max(news), k_scale=ks, v_scale=vs, out=out)
+        outs.append(out)
+    assert torch.equal(*outs) and bool(torch.isfinite(outs[0]).all())
