@@ -94,7 +94,7 @@ __device__ __forceinline__ PtWork pt_work(const IhbPagedAttn& p, const PgSeq& s,
     w.a = static_cast<long long>(s.len + PT_START) * G;
     w.d = 0;
   } else {
-    w.a = static_cast<long long>(max(s.base, 0) + PT_START) * G;
+    w.a = static_cast<long long>(min(max(s.base, 0), s.len) + PT_START) * G;   // (a length that its table does not hold may be near 2^31)
     w.d = RT;
   }
   const long long t = w.tiles;

@@ -144,3 +144,45 @@ def test_scratch_may_hold_anything(cache, lens, news, nq, nkv, monkeypatch):
         paged.paged_attention(q, k, v, table, ld, cu_q=cu, max_q=max(news), k_scale=ks, v_scale=vs, out=out)
         outs.append(out)
     assert torch.equal(*outs) and bool(torch.isfinite(outs[0]).all())
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("n", [2, 40])
+@pytest.mark.parametrize("masked", [False])
+@pytest.mark.parametrize("long", [200, 2 ** 31 - 1, 2 ** 31 - 300])
+def test_a_length_that_its_table_does_not_hold_costs_only_its_own_rows(cache, n, masked, long):
+    """Short windows and tiles: the other sequences' results are those of a call without it; its own tokens see the rows that the table holds."""
+    gen = torch.Generator().manual_seed(n)
+    nq, nkv, page = 8, 1, 16
+    lens, news = [300, 128, 90, n], [n, n, n, n]
+    table, n_pages = O.tables(lens, page, gen)
+    table = table[:, :19].contiguous()
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+    table[1, 8:] = -1
+    table = table[:, :8].contiguous() if long == 200 else table
+    lens[0] = min(lens[0], table.shape[1] * page)
+    q = torch.randn(4 * n, nq, 128, generator=gen).to(torch.bfloat16)
+    mask = torch.ones(4 * n, n, dtype=torch.bool).tril() if masked else None
+    qd, kd, vd, td, ksd, vsd, cu, md = [None if t is None else t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news), mask)]
+
+    def run(ls):
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        o = paged.paged_attention(qd, kd, vd, td, torch.tensor(ls, dtype=torch.int32, device=DEV), cu_q=cu, max_q=n, mask=md, k_scale=ksd,
+                                  v_scale=vsd, err=err)
+        return o, int(err)
+
+    good, code = run(lens)
+    assert code == 0
+    table[1, 8:] = table[0, 0]                                       # (rows of another page: whatever the table names is seen)
+    td = table.to(DEV)
+    held = table.shape[1] * page
+    bad, code = run([lens[0], long, lens[2], lens[3]])
+    assert code == 6
+    keep = [t for t in range(4 * n) if not n <= t < 2 * n]
+    d = _p_step(cache, "bf16", n * nq > 32) + _score_bound(q, k, ks, cache, "bf16", True)
+    ref, _, mag = _reference(k, v, ks, vs, q[n:2 * n], table[1:2].expand(n, -1), [held] * n, [1] * n, nkv)
+    assert long - n >= held                                          # (none of its tokens' own rows is held: they see all that is)
+    _check(bad[n:2 * n], ref, mag, d, "bf16")
+    want, _, mag = _reference(k, v, ks, vs, q, table, [lens[0], n, lens[2], lens[3]], news, nkv, mask)
+    for o in (good, bad):
+        _check(o[keep], want[keep], mag[keep], d, "bf16")
