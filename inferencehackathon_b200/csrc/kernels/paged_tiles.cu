@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       const int r = (pair ? wg * PT_M : 0) + r_tile;                    // row of the item
       const bool live = r < sg.rows;
       const int tok = live ? (sg.row0 + r) / G : 0, head = sg.kvh * G + (live ? (sg.row0 + r) % G : 0);
-      const int vis = !live ? max(sg.seen_end, 0) : (a.mask != nullptr ? max(s.base, 0) : min(max(s.base + tok + 1, 0), s.len));   // keys [0, vis) are seen
+      const int vis = !live ? max(sg.seen_end, 0) : min(max(a.mask != nullptr ? s.base : s.base + tok + 1, 0), s.len);   // keys [0, vis) are seen
       const unsigned char* mrow = a.mask != nullptr && live ? a.mask + static_cast<size_t>(s.t0 + tok) * a.mask_stride : nullptr;
       const int* table = c.block_table + static_cast<size_t>(sg.b) * c.table_stride;
       // ---- Q: a warp brings its 32 rows, two at a time, 16 bytes per lane ----

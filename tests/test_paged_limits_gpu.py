@@ -148,7 +148,7 @@ def test_scratch_may_hold_anything(cache, lens, news, nq, nkv, monkeypatch):
 
 @pytest.mark.parametrize("cache", ["fp8", "bf16"])
 @pytest.mark.parametrize("n", [2, 40])
-@pytest.mark.parametrize("masked", [False])
+@pytest.mark.parametrize("masked", [False, True])
 @pytest.mark.parametrize("long", [200, 2 ** 31 - 1, 2 ** 31 - 300])
 def test_a_length_that_its_table_does_not_hold_costs_only_its_own_rows(cache, n, masked, long):
     """Short windows and tiles: the other sequences' results are those of a call without it; its own tokens see the rows that the table holds."""
