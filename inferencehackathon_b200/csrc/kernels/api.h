@@ -324,7 +324,8 @@ typedef struct {
 int ihb_paged_append(const IhbPagedAppend* a, cudaStream_t stream);
 
 // out[t][h] = softmax(scale * q . K) V over the rows the token sees: its own row and those before it, or with mask
-// [T][mask_stride] (bytes) the rows before the call's and row j of the call's where mask[t][j] != 0. lse (optional) [T][nq]:
+// [T][mask_cols] (bytes, mask_stride apart: 0 shares a row among the tokens, less than mask_cols overlaps them) the rows before the call's and
+// row j < mask_cols of the call's where mask[t][j] != 0. lse (optional) [T][nq]:
 // natural log of the softmax denominator. A token that sees nothing gets zeros (lse -inf). q / out: fp32 or bf16,
 // element strides per token and head. max_q: most tokens any sequence has in the call. scratch: ihb_paged_attention_scratch
 // bytes, not read before it is written (no initialisation).
@@ -339,6 +340,7 @@ typedef struct {
   float* lse;
   const unsigned char* mask;
   long long mask_stride;
+  int mask_cols;
   int max_q;
   float scale;
   void* scratch;

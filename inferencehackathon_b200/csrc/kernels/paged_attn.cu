@@ -123,7 +123,7 @@ __device__ __forceinline__ bool pd_sees(const IhbPagedAttn& a, const PgSeq& s, i
   if (i >= s.n || p >= s.len) return false;
   const int j = p - s.base;
   if (a.mask == nullptr) return j <= i;
-  return j < 0 || (j < a.mask_stride && a.mask[static_cast<size_t>(s.t0 + i) * a.mask_stride + j] != 0);
+  return j < 0 || (j < a.mask_cols && a.mask[static_cast<size_t>(s.t0 + i) * a.mask_stride + j] != 0);
 }
 
 // Shared memory of a CTA: ST key steps per warp in flight (per group 16 rows of K, 16 of V, the page's scales), the Q fragments of the row
@@ -720,7 +720,7 @@ using namespace ihb;
 
 static bool paged_attn_ok(const IhbPagedAttn& a) {
   return paged_ok(a.c) && a.nq > 0 && a.nq % a.c.nkv == 0 && a.nq / a.c.nkv <= 256 &&
-         a.q != nullptr && a.out != nullptr && a.max_q > 0 && (a.mask == nullptr || a.mask_stride >= 1) &&
+         a.q != nullptr && a.out != nullptr && a.max_q > 0 && (a.mask == nullptr || (a.mask_stride >= 0 && a.mask_cols >= 1)) &&
          a.q_stride_t % 8 == 0 && a.q_stride_h % 8 == 0;
 }
 

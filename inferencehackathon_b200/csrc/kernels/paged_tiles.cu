@@ -414,7 +414,7 @@ __device__ __forceinline__ void pt_sts(uint32_t a, uint4 v) {
 // Does a row see key p? vis: keys below it are seen; mrow: the row's mask over the call's tokens, or NULL.
 __device__ __forceinline__ bool pt_sees(const IhbPagedAttn& a, const PgSeq& s, const unsigned char* mrow, int vis, int p) {
   if (p < vis) return true;
-  return mrow != nullptr && p < s.len && p - s.base < a.mask_stride && mrow[p - s.base] != 0;
+  return mrow != nullptr && p < s.len && p - s.base < a.mask_cols && mrow[p - s.base] != 0;
 }
 // One element of V as a float, for the rare correction of values that are not finite.
 template <bool KV8>
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
               unsigned w = n == 32 ? ~0u : (1u << n) - 1u;               // bit e: the row sees key kc + e
               if (mrow != nullptr && n < 32 && kc < s.len) {             // (vis = base: the keys from there on are the call's tokens)
                 unsigned char b[32];
-                const int j0 = kc - s.base, j1 = min(static_cast<int>(min(a.mask_stride, static_cast<long long>(s.n))), s.len - s.base);
+                const int j0 = kc - s.base, j1 = min(min(a.mask_cols, s.n), s.len - s.base);
 #pragma unroll
                 for (int e = 0; e < 32; ++e) b[e] = j0 + e >= 0 && j0 + e < j1 ? mrow[j0 + e] : 0;       // all in flight at once
 #pragma unroll

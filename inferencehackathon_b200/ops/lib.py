@@ -144,7 +144,7 @@ class IhbPagedAttn(C.Structure):
     _fields_ = [("c", IhbPaged), ("q", _vp), ("q_bf16", C.c_int), ("nq", C.c_int), ("q_stride_t", C.c_longlong),
                 ("q_stride_h", C.c_longlong), ("out", _vp), ("out_bf16", C.c_int), ("out_stride_t", C.c_longlong),
                 ("out_stride_h", C.c_longlong), ("lse", _vp), ("mask", _vp), ("mask_stride", C.c_longlong),
-                ("max_q", C.c_int), ("scale", C.c_float), ("scratch", _vp)]
+                ("mask_cols", C.c_int), ("max_q", C.c_int), ("scale", C.c_float), ("scratch", _vp)]
 
 
 def load(build_if_missing: bool = True) -> C.CDLL:

@@ -31,7 +31,7 @@ _F32, _BF16, _I32, _E4M3 = torch.float32, torch.bfloat16, torch.int32, torch.flo
 # NULL): packed in 1 us where filling the structures takes 4.
 _CACHE = "PPPPiiiiiiqPPPP"
 _APPEND = struct.Struct("@" + _CACHE + "PiiqPiqPPfPPiP")
-_ATTN = struct.Struct("@" + _CACHE + "PiiqqPiqqPPqifP")
+_ATTN = struct.Struct("@" + _CACHE + "PiiqqPiqqPPqiifP")
 _PTR = struct.Struct("@P")
 
 
@@ -196,12 +196,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                     err: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of ``q [T, nq, 128]`` (fp32 or bf16, any token / head strides that are multiples of 8) over the pages.
 
-    A token sees its own row and those before it; with ``mask [T, >= max_q]`` (bool or uint8) it sees all rows ahead of the
-    call's and row ``j`` of its sequence's tokens where ``mask[t, j]`` is set (token trees). A token that sees nothing gets zeros
-    (and ``lse`` -inf); values in rows that a token does not see never reach it, NaN and infinities included. ``max_q``: an
-    upper bound of the tokens per sequence. ``scale`` defaults to 128 ** -0.5. ``out [T, nq, 128]`` fp32 or bf16 (default: new, of
-    ``q``'s type; tokens behind ``cu_q[B]`` are left as they are, so a new tensor holds nothing there). ``lse [T, nq]`` fp32
-    receives the natural log of each softmax denominator, for merging with attention over other rows."""
+    A token sees its own row and those before it; with ``mask [T, >= max_q]`` (bool or uint8; a view of any row stride, rows may
+    overlap or be one) it sees all rows ahead of the call's and row ``j`` of its sequence's tokens where ``mask[t, j]`` is set (token
+    trees). A token that sees nothing gets zeros (and ``lse`` -inf); values in rows that a token does not see never reach it, NaN and
+    infinities included. ``max_q``: an upper bound of the tokens per sequence. ``scale`` defaults to 128 ** -0.5. ``out [T, nq, 128]``
+    fp32 or bf16 (default: new, of ``q``'s type; tokens behind ``cu_q[B]`` are left as they are, so a new tensor holds nothing there).
+    ``lse [T, nq]`` fp32 receives the natural log of each softmax denominator, for merging with attention over other rows."""
     shape = q.shape
     if len(shape) != 3 or shape[2] != HEAD_DIM or shape[0] < 1:
         _bad(f"q must be [T, nq, {HEAD_DIM}]")
@@ -224,7 +224,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     elif not 0.0 < scale < 1e30:
         _bad("scale must be positive and finite")
     lp = mp = 0
-    mask_stride = 0
+    mask_stride = mask_cols = 0
     if lse is not None:
         if lse.dtype != _F32 or lse.shape != (T, nq) or not lse.is_contiguous() or lse.get_device() != dev:
             _bad("lse must be contiguous fp32 [T, nq] on the pages' device")
@@ -233,7 +233,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if mask.dtype not in (torch.bool, torch.uint8) or mask.dim() != 2 or mask.shape[0] != T or mask.shape[1] < max_q or mask.get_device() != dev:
             _bad("mask must be bool or uint8 [T, >= max_q] on the pages' device")
         mask_stride, last = mask.stride()
-        if last != 1 and mask.shape[1] > 1:
+        mask_cols = mask.shape[1]
+        if last != 1 and mask_cols > 1:
             _bad("mask must have contiguous rows")
         mp = mask.data_ptr()
     if out is None:
@@ -251,7 +252,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             _bad("rows of out overlap")
         if dev < 0:
             _bad("the paged cache kernels need CUDA tensors")
-    a = _ATTN.pack(*c, qp, dtype == _BF16, nq, qs[0], qs[1], op, od == _BF16, os[0], os[1], lp, mp, mask_stride, max_q, scale, 0)
+    a = _ATTN.pack(*c, qp, dtype == _BF16, nq, qs[0], qs[1], op, od == _BF16, os[0], os[1], lp, mp, mask_stride, mask_cols, max_q, scale, 0)
     lib = K.load()
     scratch = torch.empty(lib.ihb_paged_attention_scratch(a), dtype=torch.uint8, device=q.device)
     _launch(lib.ihb_paged_attention, a[:-_PTR.size] + _PTR.pack(scratch.data_ptr()), dev, "ihb_paged_attention")

@@ -186,3 +186,65 @@ def test_a_length_that_its_table_does_not_hold_costs_only_its_own_rows(cache, n,
     want, _, mag = _reference(k, v, ks, vs, q, table, [lens[0], n, lens[2], lens[3]], news, nkv, mask)
     for o in (good, bad):
         _check(o[keep], want[keep], mag[keep], d, "bf16")
+
+
+def _mask_views(n, width, T, gen):
+    """name -> (a view [T, >= n] that is not plain contiguous bool, the same bits as a contiguous bool tensor)."""
+    flat = (torch.rand(T + n - 1, generator=gen) < 0.6).to(DEV)
+    row = (torch.rand(1, n, generator=gen) < 0.6).to(DEV)
+    full = (torch.rand(T, n, generator=gen) < 0.6).to(DEV)
+    wide = torch.ones(T, width, dtype=torch.bool, device=DEV)
+    wide[:, 3:3 + n] = full
+    bytes_ = torch.where(full, torch.randint(1, 256, (T, n), generator=gen).to(DEV), torch.zeros((), dtype=torch.long, device=DEV)).to(torch.uint8)
+    band = flat.unfold(0, n, 1)
+    return {"band of one vector": (band, band.contiguous()), "one row for all": (row.expand(T, -1), row.repeat(T, 1)),
+            "columns of a wider one": (wide[:, 3:3 + n], full), "bytes": (bytes_, full), "one row, odd stride": (full.as_strided((1, n), (1, 1)), full[:1])}
+
+
+@pytest.mark.parametrize("cache,io", [("fp8", "bf16"), ("bf16", "bf16"), ("bf16", "fp32")])
+@pytest.mark.parametrize("n", [3, 30, 45])
+def test_mask_views_are_their_contiguous_copies(cache, io, n):
+    """Rows that overlap, one row for all tokens, columns of a wider mask, bytes: short windows and tiles (45 tokens of 8 heads)."""
+    gen = torch.Generator().manual_seed(n)
+    nq, nkv, page, news = 8, 1, 16, [n, n - 1, n]
+    lens = [100 + n, n - 1, 7 + n]
+    T = sum(news)
+    table, n_pages = O.tables(lens, page, gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+    q = torch.randn(T, nq, 128, generator=gen).to(_io(io))
+    qd, kd, vd, td, ksd, vsd, cu = [None if t is None else t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news))]
+    ld = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    d = _p_step(cache, io, n * nq > 32) + _score_bound(q, k, ks, cache, io, n * nq > 32)
+    for name, (view, plain) in _mask_views(n, n + 24, T, gen).items():
+        a = (qd, kd, vd, td, ld)
+        kw = dict(cu_q=cu, max_q=n, k_scale=ksd, v_scale=vsd)
+        want_lens, want_news, q_of, table_of = lens, news, q, table
+        if view.shape[0] == 1:                                       # (a call of one token)
+            a = (qd[:1], kd, vd, td[:1], ld[:1])
+            kw = dict(max_q=1, k_scale=ksd, v_scale=vsd)
+            want_lens, want_news, q_of, table_of = lens[:1], [1], q[:1], table[:1]
+        ref, _, mag = _reference(k, v, ks, vs, q_of, table_of, want_lens, want_news, nkv, plain.cpu())
+        got = paged.paged_attention(*a, mask=view, **kw)
+        _check(got, ref, mag, d, io)
+        assert torch.equal(got, paged.paged_attention(*a, mask=plain, **kw)), name
+
+
+def test_tokens_beyond_the_mask_are_not_read_from_it():
+    """More tokens than max_q and than a mask's columns: an error word, and no byte outside of the view counts."""
+    gen = torch.Generator().manual_seed(2)
+    nq, nkv, page, n = 8, 1, 16, 6
+    table, n_pages = O.tables([40], page, gen)
+    k, v, _, _ = O.random_pages(n_pages, nkv, page, "bf16", gen, spread=False)
+    q = torch.randn(n, nq, 128, generator=gen)
+    qd, kd, vd, td = (t.to(DEV) for t in (q, k, v, table))
+    outs = []
+    for outside in (False, True):
+        wide = torch.full((n, 64), outside, dtype=torch.bool, device=DEV)
+        wide[:, 5:9] = torch.ones(n, 4, dtype=torch.bool, device=DEV).tril()
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        out = torch.zeros(n, nq, 128, device=DEV)
+        paged.paged_attention(qd, kd, vd, td, torch.tensor([40], dtype=torch.int32, device=DEV), cu_q=torch.tensor([0, n], dtype=torch.int32, device=DEV),
+                              max_q=4, mask=wide[:, 5:9], out=out, err=err)
+        assert int(err) == 6
+        outs.append(out)
+    assert torch.equal(*outs)
