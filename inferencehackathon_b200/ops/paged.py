@@ -190,7 +190,7 @@ def paged_append(qkv: torch.Tensor, nq: int, nkv: int, k_pages: torch.Tensor, v_
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor, *,
-                    cu_q: Optional[torch.Tensor] = None, max_q: int = 1, mask: Optional[torch.Tensor] = None,
+                    cu_q: Optional[torch.Tensor] = None, max_q: Optional[int] = None, mask: Optional[torch.Tensor] = None,
                     k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
                     err: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -199,9 +199,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     A token sees its own row and those before it; with ``mask [T, >= max_q]`` (bool or uint8; a view of any row stride, rows may
     overlap or be one) it sees all rows ahead of the call's and row ``j`` of its sequence's tokens where ``mask[t, j]`` is set (token
     trees). A token that sees nothing gets zeros (and ``lse`` -inf); values in rows that a token does not see never reach it, NaN and
-    infinities included. ``max_q``: an upper bound of the tokens per sequence. ``scale`` defaults to 128 ** -0.5. ``out [T, nq, 128]``
-    fp32 or bf16 (default: new, of ``q``'s type; tokens behind ``cu_q[B]`` are left as they are, so a new tensor holds nothing there).
-    ``lse [T, nq]`` fp32 receives the natural log of each softmax denominator, for merging with attention over other rows."""
+    infinities included. ``max_q``, required with ``cu_q``: an upper bound of the tokens per sequence (a sequence with more sets ``err``
+    and may leave rows of ``out`` unwritten). ``scale`` defaults to 128 ** -0.5. ``out [T, nq, 128]`` fp32 or bf16 (default: new, of
+    ``q``'s type; tokens behind ``cu_q[B]`` are left as they are, so a new tensor holds nothing there). ``lse [T, nq]`` fp32 receives
+    the natural log of each softmax denominator, for merging with attention over other rows."""
     shape = q.shape
     if len(shape) != 3 or shape[2] != HEAD_DIM or shape[0] < 1:
         _bad(f"q must be [T, nq, {HEAD_DIM}]")
@@ -217,7 +218,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _bad(f"{nq} query heads do not share {nkv} KV heads evenly")
     if nq > 256 * nkv:
         _bad("a KV head can have at most 256 query heads")
-    if max_q < 1 or (cu_q is None and max_q != 1):
+    if max_q is None:
+        if cu_q is not None:
+            _bad("cu_q needs max_q, an upper bound of the tokens per sequence")
+        max_q = 1
+    elif max_q < 1 or (cu_q is None and max_q != 1):
         _bad("max_q must be positive, and 1 without cu_q")
     if scale is None:
         scale = HEAD_DIM ** -0.5

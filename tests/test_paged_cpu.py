@@ -228,3 +228,13 @@ def test_more_query_heads_per_kv_head_than_the_work_split_counts_are_refused():
     c = K.IhbPaged(k=16, v=16, n_pages=4, nkv=1, page=16, B=1, T=1, max_blocks=1, block_table=16, kv_len=16)
     b = K.IhbPagedAttn(c=c, q=16, nq=257, out=16, max_q=1, scratch=16, q_stride_t=8, q_stride_h=8)
     assert lib.ihb_paged_attention(C.byref(b), None) != 0
+
+
+def test_ragged_calls_name_their_longest_window():
+    """With cu_q a forgotten max_q would leave rows of longer windows unwritten."""
+    a = _attn_args(cu_q=torch.tensor([0, 1, 2, 3], dtype=torch.int32))
+    with pytest.raises(ValueError, match="cu_q needs max_q"):
+        paged.paged_attention(**a)
+    for bound in (1, 3):
+        with pytest.raises(ValueError, match="CUDA tensors"):            # all that it lacks
+            paged.paged_attention(**a, max_q=bound)
