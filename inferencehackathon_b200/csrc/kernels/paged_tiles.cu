@@ -543,9 +543,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             const uint4 v = pt_lds(row + (p & 1) * PT_HALF + (((p >> 1) ^ (lane & 7)) << 4));
             mx2 = __vmaxu2(mx2, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
           }
-          const unsigned mx = max(mx2 & 0xffffu, mx2 >> 16);             // (NaN is larger than anything: its row then gets the factor NaN)
+          // A row with NaN (larger than anything) or an infinity (e4m3 has none) becomes NaN in all channels, and so do its scores: those that are seen
+          const unsigned mx = max(mx2 & 0xffffu, mx2 >> 16), nan = mx < 0x7f80u ? 0u : 0x7f7f7f7fu;
           const int e2 = min(max(static_cast<int>(mx >> 7) - 127 - 7, -100), 100);
-          rowf *= mx < 0x7f80u ? __uint_as_float(static_cast<unsigned>(127 + e2) << 23) : __uint_as_float(0x7fffffffu);   // e4m3 has no infinity
+          rowf *= __uint_as_float(static_cast<unsigned>(127 + e2) << 23);
           const float inv = __uint_as_float(static_cast<unsigned>(127 - e2) << 23);
 #pragma unroll 2
           for (int p = 0; p < 8; ++p) {
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 const __half2 z = __hsub2(y, cvt_e4m3x2(static_cast<unsigned short>(h8[k])));
                 l8[k] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(z), __NV_SATFINITE, __NV_E4M3);
               }
-              hi[e] = h8[0] | h8[1] << 16;
+              hi[e] = h8[0] | h8[1] << 16 | nan;
               lo[e] = l8[0] | l8[1] << 16;
             }
             pt_sts(at, make_uint4(hi[0], hi[1], hi[2], hi[3]));

@@ -248,3 +248,32 @@ def test_tokens_beyond_the_mask_are_not_read_from_it():
         assert int(err) == 6
         outs.append(out)
     assert torch.equal(*outs)
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("io", ["fp32", "bf16"])
+@pytest.mark.parametrize("n", [4, 40])
+def test_a_token_that_sees_nothing_gets_zeros_whatever_its_query_holds(cache, io, n):
+    """NaN and infinities in the queries of padded tokens, whose mask is empty; the other tokens of their tile are not touched."""
+    gen = torch.Generator().manual_seed(n)
+    nq, nkv, page = 8, 1, 32
+    lens, news = [n], [n]
+    table, n_pages = O.tables(lens, page, gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+    q = torch.randn(n, nq, 128, generator=gen)
+    mask = torch.ones(n, n, dtype=torch.bool).tril()
+    for t, x in ((1, float("nan")), (2, float("inf")), (n - 1, float("-inf"))):
+        q[t, :, 7 * t % 128] = x
+        mask[t] = False
+    q = q.to(_io(io))
+    qd, kd, vd, td, ksd, vsd, cu, md = [None if t is None else t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news), mask)]
+    lse = torch.empty(n, nq, device=DEV)
+    out = paged.paged_attention(qd, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=n, mask=md, k_scale=ksd, v_scale=vsd, lse=lse)
+    fine = [t for t in range(n) if t not in (1, 2, n - 1)]
+    ref, _, mag = _reference(k, v, ks, vs, torch.nan_to_num(q, posinf=0.0, neginf=0.0), table, lens, news, nkv, mask)
+    _check(out[fine], ref[fine], mag[fine], _p_step(cache, io, n * nq > 32) + _score_bound(torch.nan_to_num(q, posinf=0.0, neginf=0.0), k, ks, cache, io, n * nq > 32), io)
+    for t in (1, 2, n - 1):
+        assert bool((out[t] == 0).all()) and bool(torch.isneginf(lse[t]).all())
+    md[1, 0] = True                                                  # seen: NaN
+    out = paged.paged_attention(qd, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=n, mask=md, k_scale=ksd, v_scale=vsd)
+    assert bool(torch.isnan(out[1]).all()) and bool((out[2] == 0).all())
