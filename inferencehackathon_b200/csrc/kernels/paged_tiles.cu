@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
       const unsigned char* mrow = a.mask != nullptr && live ? a.mask + static_cast<size_t>(s.t0 + tok) * a.mask_stride : nullptr;
       const int* table = c.block_table + static_cast<size_t>(sg.b) * c.table_stride;
       // ---- Q: a warp brings its 32 rows, two at a time, 16 bytes per lane ----
-      float rowf = a.scale * PG_LOG2E;
+      float rowf = fmaxf(a.scale * PG_LOG2E, 1.17549435e-38f);            // (never 0: times a masked -inf it would be NaN)
       if (ok && n_seg > 0) ok = pt_wait(&sh.q_free, (n_seg - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
       if (ok && n_hand > 0) ok = pt_wait(&sh.hand[1], (n_hand - 1) & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
       __syncwarp();
@@ -545,8 +545,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           }
           // A row with NaN (larger than anything) or an infinity (e4m3 has none) becomes NaN in all channels, and so do its scores: those that are seen
           const unsigned mx = max(mx2 & 0xffffu, mx2 >> 16), nan = mx < 0x7f80u ? 0u : 0x7f7f7f7fu;
-          const int e2 = min(max(static_cast<int>(mx >> 7) - 127 - 7, -100), 100);
-          rowf *= __uint_as_float(static_cast<unsigned>(127 + e2) << 23);
+          // (not below 2^-45, and the factor not below 2^-49: times the least page scale it is not 0, see above. Of a row below 2^-38 that loses 2^-55.)
+          const int e2 = min(max(static_cast<int>(mx >> 7) - 127 - 7, -45), 100);
+          rowf = fmaxf(rowf * __uint_as_float(static_cast<unsigned>(127 + e2) << 23), 1.7763568394002505e-15f);
           const float inv = __uint_as_float(static_cast<unsigned>(127 - e2) << 23);
 #pragma unroll 2
           for (int p = 0; p < 8; ++p) {

@@ -277,3 +277,33 @@ def test_a_token_that_sees_nothing_gets_zeros_whatever_its_query_holds(cache, io
     md[1, 0] = True                                                  # seen: NaN
     out = paged.paged_attention(qd, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=n, mask=md, k_scale=ksd, v_scale=vsd)
     assert bool(torch.isnan(out[1]).all()) and bool((out[2] == 0).all())
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("io", ["fp32", "bf16"])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_rows_of_zeros(cache, io, n):
+    """Queries of zeros and keys of zeros, as a warm-up call or padded tokens bring them (e4m3 pages of zeros have the least scale, 2^-60): uniform
+    probabilities over the keys that a token sees, for single tokens, short windows and tiles."""
+    gen = torch.Generator().manual_seed(n)
+    nq, nkv, page = 8, 1, 16
+    lens, news = [n + 30, n, 200 + n], [n] * 3
+    T = 3 * n
+    table, n_pages = O.tables(lens, page, gen)
+    qkv = torch.zeros(T, (nq + 2 * nkv) * 128)
+    qkv[:, -128:] = torch.randn(T, 128, generator=gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+    k.zero_()
+    if ks is not None:
+        ks.fill_(2.0 ** -60)
+    kd, vd, td, ksd, vsd, cu, x = [None if t is None else t.to(DEV) for t in (k, v, table, ks, vs, O.cu_of(news), qkv.to(_io(io)))]
+    cos, sin = (t.to(DEV) for t in O.rope_tables(300))
+    ld = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    q = paged.paged_append(x, nq, nkv, kd, vd, td, ld, cos, sin, cu_q=cu, q_gamma=torch.ones(128, device=DEV), k_gamma=torch.ones(128, device=DEV),
+                           k_scale=ksd, v_scale=vsd)
+    assert bool((q == 0).all()) and bool((kd.float() == 0).all())
+    lse = torch.empty(T, nq, device=DEV)
+    out = paged.paged_attention(q, kd, vd, td, ld, cu_q=cu, max_q=n, k_scale=ksd, v_scale=vsd, lse=lse)
+    ref, ref_lse, mag = _reference(kd.cpu(), vd.cpu(), None if ks is None else ksd.cpu(), None if ks is None else vsd.cpu(), q.cpu(), table, lens, news, nkv)
+    _check(out, ref, mag, _p_step(cache, io, n * nq > 32) + 2.0 ** -17, io)
+    assert float((lse.double().cpu() - ref_lse).abs().max()) <= 2.0 ** -17
