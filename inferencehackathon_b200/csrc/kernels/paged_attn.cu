@@ -31,7 +31,7 @@ namespace ihb {
 
 constexpr int PD_WARPS = 4;
 constexpr int PD_UNIT = 128;                 // keys per unit of the work split
-constexpr float PD_NONE = 1e30f;             // OFF - running maximum before the first key
+constexpr float PD_NONE = 3.402823466e38f;   // OFF - running maximum before the first key: any finite score is above it
 
 template <bool F16>
 __device__ __forceinline__ void pd_mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {

@@ -307,3 +307,26 @@ def test_rows_of_zeros(cache, io, n):
     ref, ref_lse, mag = _reference(kd.cpu(), vd.cpu(), None if ks is None else ksd.cpu(), None if ks is None else vsd.cpu(), q.cpu(), table, lens, news, nkv)
     _check(out, ref, mag, _p_step(cache, io, n * nq > 32) + 2.0 ** -17, io)
     assert float((lse.double().cpu() - ref_lse).abs().max()) <= 2.0 ** -17
+
+
+@pytest.mark.parametrize("io", ["fp32", "bf16"])
+def test_scores_of_any_finite_size(io):
+    """A token that sees one key has that key's value for its result, however large or small the score; of two keys 2^40 apart the larger one's."""
+    gen = torch.Generator().manual_seed(3)
+    nq, P = 8, 16
+    k = torch.ones(1, 1, P, 128, dtype=torch.bfloat16) * 2.0 ** 60
+    v = torch.randn(1, 1, P, 128, generator=gen).to(torch.bfloat16)
+    q = (torch.tensor([-(2.0 ** 50), 2.0 ** 50, -(2.0 ** 20), 2.0 ** 20, -(2.0 ** -80), 0.0, -(2.0 ** 41), 1.0]) / 128)[None, :, None].expand(1, -1, 128).contiguous()
+    table = torch.zeros(1, 1, dtype=torch.int32)
+    for n in (1, 2):
+        if n == 2:
+            k[0, 0, 1] = 2.0 ** 20                                   # the scores' sign decides
+        out = paged.paged_attention(q.to(_io(io)).to(DEV), k.to(DEV), v.to(DEV), table.to(DEV), torch.tensor([n], dtype=torch.int32, device=DEV))
+        want = v[0, 0, 0].expand(nq, -1).clone()
+        if n == 2:
+            want[torch.tensor([0, 2, 6])] = v[0, 0, 1]
+            rows = [0, 1, 2, 3, 6, 7]
+        else:
+            rows = list(range(nq))
+        got = out[0].to(torch.bfloat16).cpu()
+        assert torch.equal(got[rows], want[rows])
