@@ -330,3 +330,33 @@ def test_scores_of_any_finite_size(io):
             rows = list(range(nq))
         got = out[0].to(torch.bfloat16).cpu()
         assert torch.equal(got[rows], want[rows])
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("io", ["fp32", "bf16"])
+@pytest.mark.parametrize("nq,nkv", [(256, 1), (100, 1), (34, 2), (250, 2)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_many_query_heads_per_kv_head(cache, io, nq, nkv, masked):
+    """A token over several row tiles, decode and windows, odd groups."""
+    gen = torch.Generator().manual_seed(nq)
+    page = 32
+    for lens, news in (([70, 0, 1, 300], [1, 1, 1, 1]), ([150, 9, 2], [5, 9, 2])):
+        table, n_pages = O.tables(lens, page, gen)
+        k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+        q = torch.randn(sum(news), nq, 128, generator=gen).to(_io(io))
+        mask = O.tree_mask(news, max(news), 5) if masked else None
+        qd, kd, vd, td, ksd, vsd, cu, md = [None if t is None else t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news), mask)]
+        lse = torch.empty(sum(news), nq, device=DEV)
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        out = paged.paged_attention(qd, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=max(news), mask=md, k_scale=ksd,
+                                    v_scale=vsd, lse=lse, err=err)
+        tiles = max(news) * (nq // nkv) > 32
+        eff = [max(n, 0) for n in lens]
+        live = [m if L else 0 for L, m in zip(eff, news)]
+        keep = torch.cat([torch.full((m,), bool(L), dtype=torch.bool) for L, m in zip(eff, news)])
+        ref, ref_lse, mag = _reference(k, v, ks, vs, q[keep], table, eff, live, nkv, None if mask is None else mask[keep])
+        bound = _score_bound(q, k, ks, cache, io, tiles)
+        _check(out[keep.to(DEV)], ref, mag, _p_step(cache, io, tiles) + bound, io)
+        assert float((lse[keep.to(DEV)].double().cpu() - ref_lse).abs().max()) <= bound
+        gone = ~keep.to(DEV)
+        assert int(err) == 0 and bool((out[gone] == 0).all()) and bool(torch.isneginf(lse[gone]).all())
