@@ -66,10 +66,17 @@ __device__ __forceinline__ void pa_norm_rope(PaRow& r, bool norm, const PaRow& g
   }
 }
 
-// K rows of e4m3 pages: in fp32 one byte of a million falls on the wrong side of a tie, a whole step off. A row with a value that close is done
-// again in 64 bits (8 K tokens of 64 / 4 heads: 70 us, 68 without, 90 with all rows in 64 bits). Is x within 4 units in the last place of a tie of
-// e4m3's three mantissa bits? (Ties of its subnormals are not looked for: a step is 2^-17 of the page's largest there.)
-__device__ __forceinline__ bool pa_tie(float x) { return ((__float_as_uint(x) + 0x80004u) & 0xfffffu) <= 8u; }
+// K rows of e4m3 pages: in fp32 about one byte of a million falls on the wrong side of a tie, a whole step off. How far a value x of a rotated
+// pair (x, y) may be from the exact one, in units of 2^-24: the norm's factor 10 |x| (a sum of 128 squares, 10 roundings deep, halved by the root; eps;
+// rsqrtf 2 ulp), its products and the gammas' 2 M, the rotation's M + |x|, with M = |a c| + |b s| <= sqrt(x^2 + y^2) <= |x| + |y|, for any c and s.
+// A row in which that decides the byte of a value, or the scale of the page, is done again in 64 bits: bytes and scales are those of
+// exact arithmetic, whatever the call's size. 0.7 % of random rows are. (Decode step of 64 tokens, 4 heads: 5.7 us, 5.1 without; 8 K tokens: 71.5,
+// 67.6 without, 90 with all rows in 64 bits.)
+constexpr float PA_ULP = 5.9604645e-08f;                     // 2^-24
+struct PaError {
+  float x, y;                                                 // factors of |x| and |y|
+  __device__ __forceinline__ explicit PaError(bool norm) : x((norm ? 15.f : 3.f) * PA_ULP), y((norm ? 4.f : 2.f) * PA_ULP) {}
+};
 // Rounded to odd (an inexact value has its last bit set): rounding that to e4m3 gives what rounding d itself gives.
 __device__ __forceinline__ float pa_odd(double d) {
   const float f = __double2float_rn(d);
@@ -77,8 +84,8 @@ __device__ __forceinline__ float pa_odd(double d) {
   return __uint_as_float(__float_as_uint(__double2float_rz(d)) | 1u);
 }
 template <bool BF16>
-__device__ __noinline__ PaRow pa_row64(const void* src, size_t at, const float* gamma, float eps, const float* cos_r, const float* sin_r, int c) {
-  PaRow r, g;
+__device__ __forceinline__ PaRow pa_row64(const void* src, size_t at, const float* gamma, float eps, const float* cos_r, const float* sin_r, int c) {
+  PaRow r, g = {};
   float cs[4], sn[4];
   pa_load_row<BF16>(r, src, at, c);
   pa_load4<false>(cos_r, 4 * c, cs);
@@ -87,10 +94,16 @@ __device__ __noinline__ PaRow pa_row64(const void* src, size_t at, const float* 
   if (gamma != nullptr) {
     pa_load_row<false>(g, gamma, 0, c);
     double ss = 0.;
+#pragma unroll
     for (int j = 0; j < 4; ++j) ss += static_cast<double>(r.x[j]) * r.x[j] + static_cast<double>(r.y[j]) * r.y[j];
+#pragma unroll
     for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    rinv = rsqrt(ss * (1. / PG_HD) + static_cast<double>(eps));
+    const double v = ss * (1. / PG_HD) + static_cast<double>(eps);
+    rinv = rsqrtf(static_cast<float>(v));                     // 2^-22; each of Newton's steps squares that
+#pragma unroll
+    for (int i = 0; i < 2; ++i) rinv += rinv * (0.5 - 0.5 * v * rinv * rinv);
   }
+#pragma unroll
   for (int j = 0; j < 4; ++j) {
     const double a = gamma != nullptr ? r.x[j] * rinv * g.x[j] : r.x[j], b = gamma != nullptr ? r.y[j] * rinv * g.y[j] : r.y[j];
     r.x[j] = pa_odd(a * cs[j] - b * sn[j]);
@@ -108,6 +121,23 @@ __device__ __forceinline__ int pa_exponent(float amax) {
 __device__ __forceinline__ unsigned pa_e4m3x4(float x, float y, float z, float w, float f) {
   return static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(x * f, y * f), __NV_SATFINITE, __NV_E4M3)) |
          static_cast<unsigned>(__nv_cvt_float2_to_fp8x2(make_float2(z * f, w * f), __NV_SATFINITE, __NV_E4M3)) << 16;
+}
+// Does the error of a value decide its byte? inv: 1 / scale of the page.
+__device__ __forceinline__ bool pa_unsure(const PaRow& r, const PaError& e, float inv) {
+  bool any = false;
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    float lo[4], hi[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float x = r.x[j + i] * inv, y = r.y[j + i] * inv;
+      const float dx = fabsf(x) * e.x + fabsf(y) * e.y, dy = fabsf(y) * e.x + fabsf(x) * e.y;
+      lo[i] = x - dx; hi[i] = x + dx;
+      lo[2 + i] = y - dy; hi[2 + i] = y + dy;
+    }
+    any |= pa_e4m3x4(lo[0], lo[1], lo[2], lo[3], 1.f) != pa_e4m3x4(hi[0], hi[1], hi[2], hi[3], 1.f);
+  }
+  return any;
 }
 __device__ __forceinline__ float pa_pow2(int e) { return __uint_as_float(static_cast<unsigned>(e + 127) << 23); }
 
@@ -156,7 +186,7 @@ __device__ __forceinline__ bool pa_segment(const IhbPaged& c, int seg, int lane,
 // Blocks [0, kv_blocks): one (segment, KV head, K or V) each; 2 * RPW rows per warp cover the page. The others: hq query heads of one
 // token per warp, two at a time.
 template <bool BF16, bool KV8, int RPW>
-__global__ void __launch_bounds__(PA_WARPS * 32, RPW == 1 ? 4 : RPW == 8 ? 2 : 1) paged_append_kernel(const __grid_constant__ IhbPagedAppend a, int kv_blocks, int hq) {
+__global__ void __launch_bounds__(PA_WARPS * 32, RPW == 1 ? 4 : RPW == 8 ? 2 : 3) paged_append_kernel(const __grid_constant__ IhbPagedAppend a, int kv_blocks, int hq) {
   __shared__ float red[PA_WARPS];
   const IhbPaged& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = lane >> 4, ch = lane & 15;
@@ -229,6 +259,14 @@ __global__ void __launch_bounds__(PA_WARPS * 32, RPW == 1 ? 4 : RPW == 8 ? 2 : 1
   if (norm) pa_load_row<false>(g, a.k_gamma, 0, ch);
   unsigned live = 0;                                         // bit i: row 2 (warp + PA_WARPS i) + half is written
   float amax = 0.f;
+  auto take_amax = [&](const PaRow& v) {                     // infinities saturate, NaN stays NaN: neither sets the scale
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float s = fabsf(v.x[j]), t = fabsf(v.y[j]);
+      if (s <= 3.4028235e38f) amax = fmaxf(amax, s);
+      if (t <= 3.4028235e38f) amax = fmaxf(amax, t);
+    }
+  };
 #pragma unroll
   for (int i = 0; i < RPW; ++i) {
     const int r = 2 * (warp + PA_WARPS * i) + half;
@@ -254,14 +292,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32, RPW == 1 ? 4 : RPW == 8 ? 2 : 1
       }
     }
     if (!is_v) pa_norm_rope(x[i], norm, g, a.eps, cs, sn);
-    if (KV8 && (live >> i & 1)) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {                          // infinities saturate, NaN stays NaN: neither sets the scale
-        const float u = fabsf(x[i].x[j]), v = fabsf(x[i].y[j]);
-        if (u <= 3.4028235e38f) amax = fmaxf(amax, u);
-        if (v <= 3.4028235e38f) amax = fmaxf(amax, v);
-      }
-    }
+    if (KV8 && (live >> i & 1)) take_amax(x[i]);
   }
   if constexpr (!KV8) {
     void* dst = is_v ? c.v : c.k;
@@ -276,39 +307,67 @@ __global__ void __launch_bounds__(PA_WARPS * 32, RPW == 1 ? 4 : RPW == 8 ? 2 : 1
     unsigned char* dst = reinterpret_cast<unsigned char*>(is_v ? c.v : c.k);
     float* sc = (is_v ? c.v_scale : c.k_scale) + static_cast<size_t>(page) * nkv + h;
     const float old = r0 > 0 ? *sc : 0.f;
-    amax = warp_max(amax);
-    if (lane == 0) red[warp] = amax;
-    __syncthreads();
+    auto block_amax = [&]() {
+      amax = warp_max(amax);
+      if (lane == 0) red[warp] = amax;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) amax = fmaxf(amax, red[w]);
-    const float now = fmaxf(old, pa_pow2(pa_exponent(amax)));
-    const float inv = 1.f / now;
-    if (r0 > 0 && now > old) {                                // rows of earlier calls move to the larger scale
-      const float f = old * inv;
+      for (int w = 0; w < PA_WARPS; ++w) amax = fmaxf(amax, red[w]);
+    };
+    auto move = [&](float now) {                              // rows of earlier calls move to a larger scale
+      if (r0 == 0 || !(now > old)) return;
+      const float f = old / now;
       uint2* rowp = reinterpret_cast<uint2*>(dst + head_row * PG_HD);
       for (int i = tid; i < r0 * (PG_HD / 8); i += PA_WARPS * 32) {
         const uint2 w = rowp[i];
         const float4 p = e4m3x4_to_float4(w.x), q = e4m3x4_to_float4(w.y);
         rowp[i] = make_uint2(pa_e4m3x4(p.x, p.y, p.z, p.w, f), pa_e4m3x4(q.x, q.y, q.z, q.w, f));
       }
-    }
-#pragma unroll
-    for (int i = 0; i < RPW; ++i) {
-      if (!is_v) {
-        bool near = false;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) near |= pa_tie(x[i].x[j] * inv) || pa_tie(x[i].y[j] * inv);
-        if (__any_sync(0xffffffffu, near && (live >> i & 1))) {          // (rare; a dead half does row 0 of the call's part along, and drops it)
-          const int r = live >> i & 1 ? 2 * (warp + PA_WARPS * i) + half : 0;
-          const int pos = live >> i & 1 ? (a.positions != nullptr ? a.positions[tok0 + r] : first + r) : 0;
-          x[i] = pa_row64<BF16>(a.qkv, static_cast<size_t>(tok0 + r) * a.qkv_stride + static_cast<size_t>(nq + h) * PG_HD, a.k_gamma, a.eps,
-                                a.cos_t + static_cast<size_t>(pos) * 64, a.sin_t + static_cast<size_t>(pos) * 64, ch);
-        }
-      }
-      if (!(live >> i & 1)) continue;
+    };
+    auto put = [&](int i, const PaRow& v, float inv) {
       unsigned char* o = dst + (head_row + r0 + 2 * (warp + PA_WARPS * i) + half) * PG_HD + 4 * ch;
-      *reinterpret_cast<unsigned*>(o) = pa_e4m3x4(x[i].x[0], x[i].x[1], x[i].x[2], x[i].x[3], inv);
-      *reinterpret_cast<unsigned*>(o + 64) = pa_e4m3x4(x[i].y[0], x[i].y[1], x[i].y[2], x[i].y[3], inv);
+      *reinterpret_cast<unsigned*>(o) = pa_e4m3x4(v.x[0], v.x[1], v.x[2], v.x[3], inv);
+      *reinterpret_cast<unsigned*>(o + 64) = pa_e4m3x4(v.y[0], v.y[1], v.y[2], v.y[3], inv);
+    };
+    auto row64 = [&](int i) {                                 // (whole warp; a dead half does row 0 of the call's part along, and drops it)
+      const int r = live >> i & 1 ? 2 * (warp + PA_WARPS * i) + half : 0;
+      const int pos = live >> i & 1 ? (a.positions != nullptr ? a.positions[tok0 + r] : first + r) : 0;
+      return pa_row64<BF16>(a.qkv, static_cast<size_t>(tok0 + r) * a.qkv_stride + static_cast<size_t>(nq + h) * PG_HD, a.k_gamma, a.eps,
+                            a.cos_t + static_cast<size_t>(pos) * 64, a.sin_t + static_cast<size_t>(pos) * 64, ch);
+    };
+    block_amax();
+    const PaError e(norm);
+    const float d = (e.x + e.y) * amax;
+    float now;
+    unsigned again = 0;                                       // rows to be done in 64 bits, the same for the warp. Behind everything else: the rows in registers
+                                                              // need not outlive a call, which costs a block its place on the SM
+    if (is_v || pa_exponent(amax - d) == pa_exponent(amax + d)) {
+      now = fmaxf(old, pa_pow2(pa_exponent(amax)));
+      const float inv = 1.f / now;
+      move(now);
+#pragma unroll
+      for (int i = 0; i < RPW; ++i) {
+        if (live >> i & 1) put(i, x[i], inv);
+        if (!is_v && __any_sync(0xffffffffu, (live >> i & 1) && pa_unsure(x[i], e, inv))) again |= 1u << i;
+      }
+    } else {                                                  // one page of 250 thousand, the same for the whole block
+      amax = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < RPW && 2 * (warp + PA_WARPS * i) < rows; ++i) {
+        const PaRow v = row64(i);
+        if (live >> i & 1) take_amax(v);
+        again |= 1u << i;
+      }
+      __syncthreads();                                        // (red has been read)
+      block_amax();
+      now = fmaxf(old, pa_pow2(pa_exponent(amax)));
+      move(now);
+    }
+#pragma unroll 1
+    for (; again; again &= again - 1) {
+      const int i = __ffs(again) - 1;
+      const PaRow v = row64(i);
+      if (live >> i & 1) put(i, v, 1.f / now);
     }
     if (tid == 0) *sc = now;
   }

@@ -128,7 +128,7 @@ def paged_append(qkv: torch.Tensor, nq: int, nkv: int, k_pages: torch.Tensor, v_
     token's row, or by ``positions[t]`` (int32) where a token's angle is not its row (token trees).
 
     e4m3 pages: a page's scale is the least power of two with ``amax / 448 <= scale`` over the rows it holds (exponent -60 to
-    60; infinities saturate, NaN stays NaN, neither counts). Writing row 0 starts a page anew; otherwise the scale only grows, and
+    60; infinities saturate, NaN stays NaN, neither counts). Scales and bytes are what exact arithmetic gives (bf16 pages and queries: fp32). Writing row 0 starts a page anew; otherwise the scale only grows, and
     rows already there are brought to it in place, so a page that is written to must belong to one sequence. Rows behind the last
     token and pages of other sequences are left as they are."""
     if nq < 1 or nkv < 1:

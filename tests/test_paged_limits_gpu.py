@@ -360,3 +360,65 @@ def test_many_query_heads_per_kv_head(cache, io, nq, nkv, masked):
         assert float((lse[keep.to(DEV)].double().cpu() - ref_lse).abs().max()) <= bound
         gone = ~keep.to(DEV)
         assert int(err) == 0 and bool((out[gone] == 0).all()) and bool(torch.isneginf(lse[gone]).all())
+
+
+def _near_ties(T, nkv, norm, io, gen, gamma, cos, sin, pos, edge, every):
+    """K rows [T, nkv, 128] with normed, rotated values that lie within a few units of fp32 rounding of a tie between two e4m3 numbers, the sums that
+    form them cancelling up to a hundredfold: in ``every`` pair, or in one of a row. ``edge``: the largest value of each row next to 448 instead, where
+    the page scale changes."""
+    y = torch.rand(T, nkv, 128, generator=gen, dtype=F64) * 300 + 100
+    y = y * torch.where(torch.rand(y.shape, generator=gen) < 0.5, 1.0, -1.0)
+    c, s = cos[pos].double()[:, None], sin[pos].double()[:, None]
+    off = torch.rand(T, nkv, 64, generator=gen, dtype=F64) * 0.3 + 0.1
+    if every:
+        off.zero_()
+    else:
+        off.scatter_(2, torch.randint(0, 64, (T, nkv, 1), generator=gen), 0.0)
+    t = (torch.randint(8, 16, (T, nkv, 64), generator=gen) + 0.5 + off) * torch.exp2(torch.randint(-1, 3, (T, nkv, 64), generator=gen).double())
+    t = t * torch.where(torch.rand(t.shape, generator=gen) < 0.5, 1.0, -1.0)
+    if edge:
+        y = y / 4
+        t = t / 4
+        t[:, :, 5] = 448.0
+        y[:, :, 5] = 300.0
+    y[..., 64:] = (y[..., :64] * c - t) / s                          # a c - b s = t
+    if norm:                                                         # y = x / rms(x) gamma: mean((y / gamma)^2) = 1
+        f = torch.sqrt(((y / gamma.double()) ** 2).mean(-1, keepdim=True))
+        f = torch.exp2(torch.ceil(torch.log2(f)))                    # a power of two keeps the ties
+        y = y / f
+        rest = 1 - ((y / gamma.double()) ** 2).mean(-1)              # the missing part in a pair that is no tie: its a c - b s is as it comes
+        a = y[..., 20] / gamma[20].double()
+        y[..., 20] = torch.sqrt(a * a + 128 * rest) * gamma[20].double()
+        y = y * 3 / gamma.double()                                   # x: any multiple of y / gamma
+    return y.to(_io(io))
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("every", [False, True])
+@pytest.mark.parametrize("page,lens,news", [(16, [5, 40, 3], [5, 17, 3]), (128, [200, 7, 300], [200, 7, 131]), (64, [1, 64, 65, 130, 20], [1, 1, 1, 1, 1]),
+                                            (32, [700], [700])])
+def test_bytes_next_to_ties_are_those_of_64_bits(norm, edge, every, page, lens, news):
+    """Every byte and scale of e4m3 pages equals the 64-bit ones, with and without gammas, odd row counts, rotation angles of their own."""
+    if edge and norm:
+        pytest.skip("with a norm the largest value is the free one")
+    gen = torch.Generator().manual_seed(page + norm)
+    nq, nkv, T = 2, 2, sum(news)
+    ang = torch.rand(2000, 64, generator=gen, dtype=F64) * 0.9 + 0.35          # no angle near a multiple of a quarter turn
+    cos, sin = ang.cos().float(), ang.sin().float()
+    pos = torch.randint(0, 2000, (T,), generator=gen).to(torch.int32)
+    qg, kg = ((1 + 0.2 * torch.randn(128, generator=gen)) for _ in range(2)) if norm else (None, None)
+    qkv = torch.randn(T, nq + 2 * nkv, 128, generator=gen)
+    qkv[:, nq:nq + nkv] = _near_ties(T, nkv, norm, "fp32", gen, kg, cos, sin, pos.long(), edge, every)
+    qkv = qkv.flatten(1)
+    table, n_pages = O.tables(lens, page, gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, "fp8", gen)
+    ref = O.Pages(k, v, ks, vs)
+    O.append(ref, qkv, nq, nkv, table, lens, O.cu_of(news), cos, sin, qg, kg, positions=pos)
+    x, kd, vd, ksd, vsd, td, cu, cosd, sind, qgd, kgd, pd = [None if t is None else t.to(DEV) for t in
+                                                             (qkv, k, v, ks, vs, table, O.cu_of(news), cos, sin, qg, kg, pos)]
+    paged.paged_append(x, nq, nkv, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cosd, sind, cu_q=cu, positions=pd, q_gamma=qgd,
+                       k_gamma=kgd, k_scale=ksd, v_scale=vsd)
+    assert torch.equal(ksd.double().cpu(), ref.ks) and torch.equal(vsd.double().cpu(), ref.vs)
+    for got, want in ((kd, ref.k), (vd, ref.v)):
+        assert torch.equal(got.float().double().cpu(), want), int((got.float().double().cpu() != want).sum())
