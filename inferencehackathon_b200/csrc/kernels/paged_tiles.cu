@@ -427,7 +427,8 @@ __device__ __forceinline__ float pt_v_at(const IhbPaged& c, size_t row, int ch) 
   }
 }
 
-template <bool KV8>
+// P2 (bf16 pages): the probabilities go into the product as two bf16 terms, as those of paged_attn.cu do, and not as one.
+template <bool KV8, bool P2>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid_constant__ IhbPagedAttn a, int grid, int rec_rows) {
   extern __shared__ __align__(1024) uint8_t smem[];            // (checked below: the swizzle goes by address)
   PtHdr& sh = *reinterpret_cast<PtHdr*>(smem);
@@ -593,7 +594,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         // warp of the SM pays for it.
 #pragma unroll 1
         for (int hf = 0; hf < 2; ++hf) {
-          unsigned pk[32];
+          unsigned pk[32], pl[P2 ? 32 : 1];
           float sum;
           if (hf == 1) {
             if (ok) ok = pt_wait(&sh.s_full[2 * wg + 1], n_blk & 1u, abort_flag, c.err, ERR_TMEM_TIMEOUT);
@@ -658,6 +659,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 p1 = pd_ex2(p1);
                 s2 = pt_add2(s2, pt_pair(p0, p1));
                 pk[h * 8 + e / 2] = pd_pack<KV8>(p0, p1);
+                if constexpr (P2) {
+                  const float2 r = pd_unpack<false>(pk[h * 8 + e / 2]);
+                  pl[h * 8 + e / 2] = pd_pack<false>(p0 - r.x, p1 - r.y);
+                }
               }
               mx = fmaxf(mx, x);
               float s0, s1;
@@ -689,6 +694,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           l += sum;
           have = true;
           pt_st32(t_s + hf * 64, pk);          // in the place of the scores
+          if constexpr (P2) pt_st32(t_s + hf * 64 + 32, pl);
           pt_wait_st();
           tc_fence_before();
           mbar_arrive(&sh.p_ready[2 * wg + hf]);                         // (a barrier per half: both may be through before the issuer looks)
@@ -1107,6 +1113,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
           if (!ok) break;
           tc_fence_after();
           pt_mma8<PT_PV>(tmem + 256 + w * 128, tmem + w * 128 + hf * 64, v_lo + (g & 1) * (PT_TILE >> 4) + hf * 512, idesc_v, t > 2);
+          if constexpr (P2)
+            pt_mma8<PT_PV>(tmem + 256 + w * 128, tmem + w * 128 + hf * 64 + 32, v_lo + (g & 1) * (PT_TILE >> 4) + hf * 512, idesc_v, 1);
           tc_commit(&sh.pv_done[2 * w + hf]);
           if (hf == 1) {
             n_p ^= 1u;
@@ -1217,19 +1225,19 @@ size_t paged_tiles_scratch(const IhbPagedAttn& a) {
   return PT_MAX_GRID * sizeof(PtDesc) + static_cast<size_t>(PT_MAX_GRID) * 2 * pt_rec_rows(a) * PD_REC * sizeof(float);
 }
 
-template <bool KV8>
+template <bool KV8, bool P2>
 static cudaError_t pt_launch(const IhbPagedAttn& a, cudaStream_t stream) {
   const int grid = PT_MAX_GRID, rec_rows = pt_rec_rows(a);             // one CTA per SM
   static_assert(sizeof(PtHdr) <= 1024, "header");
   static const int regs = [] {                 // the register split draws on what the block is launched with
     cudaFuncAttributes f;
-    return cudaFuncGetAttributes(&f, paged_tiles_kernel<KV8>) == cudaSuccess ? f.numRegs : 0;
+    return cudaFuncGetAttributes(&f, paged_tiles_kernel<KV8, P2>) == cudaSuccess ? f.numRegs : 0;
   }();
   if (regs < PT_REGS) return cudaErrorInvalidConfiguration;
   constexpr int bytes = pt_smem<KV8>();
-  cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  cudaError_t e = cudaFuncSetAttribute(paged_tiles_kernel<KV8, P2>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  paged_tiles_kernel<KV8><<<grid, PT_THREADS, bytes, stream>>>(a, grid, rec_rows);
+  paged_tiles_kernel<KV8, P2><<<grid, PT_THREADS, bytes, stream>>>(a, grid, rec_rows);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -1245,7 +1253,11 @@ static cudaError_t pt_launch(const IhbPagedAttn& a, cudaStream_t stream) {
 }
 
 cudaError_t paged_tiles_launch(const IhbPagedAttn& a, cudaStream_t stream) {
-  return a.c.k_scale != nullptr ? pt_launch<true>(a, stream) : pt_launch<false>(a, stream);
+  // Up to 128 rows the width of the block table chooses between this kernel and paged_attn.cu (use_tiles): both keep two terms of P over bf16 pages, so
+  // that a wider table does not change the precision. Above, where every call comes here, one: it adds at most one more half step of bf16 to
+  // the result's own (1.8e-3 from 64 bits against 1.5e-3), and the second product would cost a sixth (prompt of 4096 tokens: 200 us, 233 with two).
+  if (a.c.k_scale != nullptr) return pt_launch<true, false>(a, stream);
+  return static_cast<long long>(a.max_q) * (a.nq / a.c.nkv) <= PT_M ? pt_launch<false, true>(a, stream) : pt_launch<false, false>(a, stream);
 }
 
 }  // namespace ihb

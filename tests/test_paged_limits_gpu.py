@@ -422,3 +422,23 @@ def test_bytes_next_to_ties_are_those_of_64_bits(norm, edge, every, page, lens, 
     assert torch.equal(ksd.double().cpu(), ref.ks) and torch.equal(vsd.double().cpu(), ref.vs)
     for got, want in ((kd, ref.k), (vd, ref.v)):
         assert torch.equal(got.float().double().cpu(), want), int((got.float().double().cpu() != want).sum())
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("lens,news,nq,nkv,page", [([700, 128, 90], [5, 8, 8], 16, 1, 32), ([300, 0, 61], [16, 0, 16], 8, 1, 128), ([130], [5], 28, 4, 64),
+                                                   ([1000], [2], 128, 2, 16)])
+def test_a_wider_table_does_not_cost_bits(cache, lens, news, nq, nkv, page):
+    """33 to 128 rows: the table's width chooses the kernel. An fp32 result shows what is left of the probabilities in each."""
+    gen = torch.Generator().manual_seed(23)
+    table, n_pages = O.tables(lens, page, gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+    q = torch.randn(sum(news), nq, 128, generator=gen).to(torch.bfloat16)
+    ref, _, mag = _reference(k, v, ks, vs, q, table, lens, news, nkv)
+    wide = torch.full((len(lens), 300000 // page), 1 << 30, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    qd, kd, vd, ksd, vsd, cu = [None if t is None else t.to(DEV) for t in (q, k, v, ks, vs, O.cu_of(news))]
+    for t in (table, wide):
+        out = torch.empty(q.shape, device=DEV)
+        paged.paged_attention(qd, kd, vd, t.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=max(news), k_scale=ksd,
+                              v_scale=vsd, out=out)
+        _check(out, ref, mag, _p_step(cache, "bf16", False) + _score_bound(q, k, ks, cache, "bf16", t is wide), "fp32")
