@@ -128,9 +128,10 @@ def paged_append(qkv: torch.Tensor, nq: int, nkv: int, k_pages: torch.Tensor, v_
     token's row, or by ``positions[t]`` (int32) where a token's angle is not its row (token trees).
 
     e4m3 pages: a page's scale is the least power of two with ``amax / 448 <= scale`` over the rows it holds (exponent -60 to
-    60; infinities saturate, NaN stays NaN, neither counts). Scales and bytes are what exact arithmetic gives (bf16 pages and queries: fp32). Writing row 0 starts a page anew; otherwise the scale only grows, and
-    rows already there are brought to it in place, so a page that is written to must belong to one sequence. Rows behind the last
-    token and pages of other sequences are left as they are."""
+    60; infinities saturate, NaN stays NaN, neither counts). Scales and bytes are what exact arithmetic gives (bf16 pages and queries:
+    fp32, rounded once). Writing row 0 starts a page anew; otherwise the scale only grows, and rows already there are brought to it in
+    place, so a page that is written to must belong to one sequence. Rows behind the last token and pages of other sequences are left
+    as they are."""
     if nq < 1 or nkv < 1:
         _bad("nq and nkv must be positive")
     shape = qkv.shape
@@ -202,7 +203,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     infinities included. ``max_q``, required with ``cu_q``: an upper bound of the tokens per sequence (a sequence with more sets ``err``
     and may leave rows of ``out`` unwritten). ``scale`` defaults to 128 ** -0.5. ``out [T, nq, 128]`` fp32 or bf16 (default: new, of
     ``q``'s type; tokens behind ``cu_q[B]`` are left as they are, so a new tensor holds nothing there). ``lse [T, nq]`` fp32 receives
-    the natural log of each softmax denominator, for merging with attention over other rows."""
+    the natural log of each softmax denominator, for merging with attention over other rows.
+
+    Sums, maxima and denominators are fp32. What else is rounded, relative to the result: fp32 queries 2^-18 over both kinds of pages;
+    bf16 queries over e4m3 pages 2^-11 (probabilities in fp16; in windows of more than 32 rows, tokens x query heads of a KV head, what
+    lies below 2^-17 of a query's largest element is lost too); over bf16 pages 2^-16, and 2^-8 where ``out`` is bf16 and a window has
+    more than 128 rows. Infinities in a value row that every token sees come out as infinity or NaN. Scales of e4m3 pages are taken
+    between 2^-60 and 2^60, scores (to base 2) up to 2^24 in magnitude."""
     shape = q.shape
     if len(shape) != 3 or shape[2] != HEAD_DIM or shape[0] < 1:
         _bad(f"q must be [T, nq, {HEAD_DIM}]")

@@ -442,3 +442,18 @@ def test_a_wider_table_does_not_cost_bits(cache, lens, news, nq, nkv, page):
         paged.paged_attention(qd, kd, vd, t.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=max(news), k_scale=ksd,
                               v_scale=vsd, out=out)
         _check(out, ref, mag, _p_step(cache, "bf16", False) + _score_bound(q, k, ks, cache, "bf16", t is wide), "fp32")
+
+
+@pytest.mark.parametrize("io", ["bf16", "fp32"])
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+def test_an_fp32_result_of_a_prompt_has_the_bits_of_its_probabilities(cache, io):
+    gen = torch.Generator().manual_seed(29)
+    nq, nkv, page, lens, news = 16, 2, 64, [700, 250], [200, 250]
+    table, n_pages = O.tables(lens, page, gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+    q = torch.randn(sum(news), nq, 128, generator=gen).to(_io(io))
+    ref, _, mag = _reference(k, v, ks, vs, q, table, lens, news, nkv)
+    qd, kd, vd, td, ksd, vsd, cu = [None if t is None else t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news))]
+    out = torch.empty(q.shape, device=DEV)
+    paged.paged_attention(qd, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=max(news), k_scale=ksd, v_scale=vsd, out=out)
+    _check(out, ref, mag, _p_step(cache, io, False) + _score_bound(q, k, ks, cache, io, True), "fp32")
