@@ -457,3 +457,44 @@ def test_an_fp32_result_of_a_prompt_has_the_bits_of_its_probabilities(cache, io)
     out = torch.empty(q.shape, device=DEV)
     paged.paged_attention(qd, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=max(news), k_scale=ksd, v_scale=vsd, out=out)
     _check(out, ref, mag, _p_step(cache, io, False) + _score_bound(q, k, ks, cache, io, True), "fp32")
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("io", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,lens", [(1, [2000]), (12, [2000, 1999]), (100, [2000])])
+def test_norm_of_the_error_over_many_keys(cache, io, n, lens):
+    """Roundings of P have no sign in common: over all outputs the error's norm is that of independent ones, each at most d of its p_j v_j. A single V row
+    out of place among 2000, which an elementwise bound would let pass, is far above that."""
+    gen = torch.Generator().manual_seed(n)
+    nq, nkv, page = 16, 2, 16
+    news = [n] * len(lens)
+    T, G = n * len(lens), nq // nkv
+    table, n_pages = O.tables(lens, page, gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+    q = torch.randn(T, nq, 128, generator=gen).to(_io(io))
+    qd, kd, vd, td, ksd, vsd, cu = [None if t is None else t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news))]
+    out = paged.paged_attention(qd, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=n, k_scale=ksd, v_scale=vsd).double()
+    off = worst = split = 0.0
+    for b, L in enumerate(lens):
+        ids = table[b, :-(-L // page)].long()
+        for h in range(nkv):
+            f = 1.0 if ks is None else ks[ids, h].to(F64)[:, None, None]
+            g = 1.0 if vs is None else vs[ids, h].to(F64)[:, None, None]
+            kk = (k[ids, h].to(F64) * f).reshape(-1, 128)[:L].to(DEV)
+            vv = (v[ids, h].to(F64) * g).reshape(-1, 128)[:L].to(DEV)
+            x = qd[b * n:(b + 1) * n, h * G:(h + 1) * G].to(F64)
+            w = x.flatten(0, 1) @ kk.T * 128 ** -0.5
+            seen = torch.arange(L, device=DEV)[None, :] <= L - n + torch.arange(n, device=DEV).repeat_interleave(G)[:, None]
+            p = torch.softmax(w.masked_fill(~seen, -math.inf), 1)
+            want = p @ vv
+            got = out[b * n:(b + 1) * n, h * G:(h + 1) * G].flatten(0, 1)
+            off += float((got - want).pow(2).sum())
+            # scores: what each channel of a query loses is independent of the others, so it counts with the norm of the key (e), and a score's error
+            # moves the output by e p_j (v_j - out), at most 2 e p_j |v_j| in the mean square
+            lost = (2.0 ** -17 if n * G > 32 and cache == "fp8" else 0.0) if io == "bf16" else (2.0 ** -22 if cache == "fp8" else 2.0 ** -16)
+            e = lost * float(x.abs().max()) * float(kk.norm(dim=1).max()) * 128 ** -0.5 + 2.0 ** -17
+            worst += float((p.pow(2) @ vv.pow(2)).sum()) * (_p_step(cache, io, n * G > 128) ** 2 + 4 * e * e) + float(want.pow(2).sum()) * (torch.finfo(_io(io)).eps / 2) ** 2
+            moved = vv.clone()
+            moved[1000] = vv[1001]
+            split += float((p @ moved - want).pow(2).sum())
+    assert off <= worst < split / 4, (off, worst, split)
