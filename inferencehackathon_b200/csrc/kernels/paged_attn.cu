@@ -698,7 +698,10 @@ static cudaError_t pd_launch(const IhbPagedAttn& a, const PdPlan& p, cudaStream_
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int G = a.nq / a.c.nkv, RT = 8 * NT;
-  const long long items = static_cast<long long>(a.c.B) * a.c.nkv * ((static_cast<long long>(a.max_q) * G + RT - 1) / RT);
+  // items of the batch at most: by the longest window, and by the tokens of the call (a caller's bound of the window may be far above)
+  const long long by_q = static_cast<long long>(a.c.B) * ((static_cast<long long>(a.max_q) * G + RT - 1) / RT);
+  const long long by_t = static_cast<long long>(a.c.T) * G / RT + a.c.B;
+  const long long items = (by_q < by_t ? by_q : by_t) * a.c.nkv;
   if (items > 0x7fffffffll) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

@@ -231,6 +231,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         max_q = 1
     elif max_q < 1 or (cu_q is None and max_q != 1):
         _bad("max_q must be positive, and 1 without cu_q")
+    elif max_q > T:
+        max_q = T
     if scale is None:
         scale = HEAD_DIM ** -0.5
     elif not 0.0 < scale < 1e30:

@@ -498,3 +498,18 @@ def test_norm_of_the_error_over_many_keys(cache, io, n, lens):
             moved[1000] = vv[1001]
             split += float((p @ moved - want).pow(2).sum())
     assert off <= worst < split / 4, (off, worst, split)
+
+
+@pytest.mark.parametrize("io", ["bf16", "fp32"])
+@pytest.mark.parametrize("bound", [40, 1000, 2 ** 31 - 1, 10 ** 12])
+def test_max_q_may_be_any_upper_bound(io, bound):
+    gen = torch.Generator().manual_seed(31)
+    nq, nkv, page, news = 8, 2, 32, [40] + [1] * 60 + [17]
+    lens = [n + 90 for n in news]
+    table, n_pages = O.tables(lens, page, gen)
+    k, v, ks, vs = O.random_pages(n_pages, nkv, page, "fp8", gen, spread=False)
+    q = torch.randn(sum(news), nq, 128, generator=gen).to(_io(io))
+    ref, _, mag = _reference(k, v, ks, vs, q, table, lens, news, nkv)
+    qd, kd, vd, td, ksd, vsd, cu = [t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news))]
+    out = paged.paged_attention(qd, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=bound, k_scale=ksd, v_scale=vsd)
+    _check(out, ref, mag, _p_step("fp8", io, True) + _score_bound(q, k, ks, "fp8", io, True), io)
