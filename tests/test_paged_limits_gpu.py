@@ -513,3 +513,31 @@ def test_max_q_may_be_any_upper_bound(io, bound):
     qd, kd, vd, td, ksd, vsd, cu = [t.to(DEV) for t in (q, k, v, table, ks, vs, O.cu_of(news))]
     out = paged.paged_attention(qd, kd, vd, td, torch.tensor(lens, dtype=torch.int32, device=DEV), cu_q=cu, max_q=bound, k_scale=ksd, v_scale=vsd)
     _check(out, ref, mag, _p_step("fp8", io, True) + _score_bound(q, k, ks, "fp8", io, True), io)
+
+
+@pytest.mark.parametrize("n", [1, 3, 64])
+def test_pages_beyond_32_bits(n):
+    """Page ids whose rows lie more than 2^32 elements into the pool, through append and attention (short windows and tiles)."""
+    gen = torch.Generator().manual_seed(n)
+    nq, nkv, page, n_pages = 16, 4, 128, 70000
+    k = torch.empty(n_pages, nkv, page, 128, dtype=torch.bfloat16, device=DEV)                       # 9.2 GB each
+    v = torch.empty_like(k)
+    lens, news = [300, n], [n, n]
+    table = torch.tensor([[69999, 3, 69000], [66000, -1, -1]], dtype=torch.int32)
+    small = torch.randn(2, 4, nkv, page, 128, generator=gen).to(torch.bfloat16)
+    ids = [69999, 3, 69000, 66000]
+    for i, g in enumerate(ids):
+        k[g], v[g] = small[0, i].to(DEV), small[1, i].to(DEV)
+    qkv = torch.randn(2 * n, (nq + 2 * nkv) * 128, generator=gen)
+    cos, sin = O.rope_tables(301)
+    td, cu, ld = table.to(DEV), O.cu_of(news).to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    q = paged.paged_append(qkv.to(DEV), nq, nkv, k, v, td, ld, cos.to(DEV), sin.to(DEV), cu_q=cu, q_out=torch.empty(2 * n, nq, 128, dtype=torch.bfloat16, device=DEV))
+    here = torch.tensor([[0, 1, 2], [3, 0, 0]], dtype=torch.int32)
+    ref = O.Pages(small[0], small[1])
+    O.append(ref, qkv, nq, nkv, here, lens, O.cu_of(news), cos, sin)
+    got_k, got_v = (torch.stack([t[g] for g in ids]).cpu() for t in (k, v))
+    for got, want in ((got_k, ref.k), (got_v, ref.v)):
+        assert bool(((got.double() - want).abs() <= want.abs() * 2.0 ** -8 + want.abs().amax(-1, keepdim=True) * 2.0 ** -20).all())
+    out = paged.paged_attention(q, k, v, td, ld, cu_q=cu, max_q=n)
+    want, _, mag = _reference(got_k, got_v, None, None, q.cpu(), here, lens, news, nkv)
+    _check(out, want, mag, _p_step("bf16", "bf16", n * 4 > 128) + 2.0 ** -17, "bf16")
