@@ -20,10 +20,11 @@
 // leaves one record (O, m, l) per piece, folded by a second kernel in a fixed order: results do not depend on timing. The folding
 // kernel is launched with the first one and works out its pieces while that runs.
 //
-// Measured (64 query heads, 4 KV heads): 64 sequences of 129 to 8191 keys, e4m3 pages, 64 us, 66 % of the measured copy bandwidth; one
-// sequence of 131071 keys 42 us, 50 %; bf16 pages of 16 tokens, 32 / 4 heads, fp32 queries, 24 sequences of up to 4096 keys, 29 us, 52 %.
-// Bound by instructions and their latency: 47 % of the issue slots at 12
-// warps per SM (shared memory for the rings), each 16-byte chunk of e4m3 being eight conversions and two matrix instructions.
+// Measured (64 query heads, 4 KV heads): 64 sequences of 129 to 8191 keys, e4m3 pages, 65 us, 66 % of the measured copy bandwidth; one
+// sequence of 131071 keys 42 us, 49 %; bf16 pages of 16 tokens, 32 / 4 heads, fp32 queries, 24 sequences of up to 4096 keys, 29 us, 53 %.
+// Bound by the latency of dependent instructions at 12 warps per SM (shared memory for the rings): over e4m3 pages, where a 16-byte chunk is eight
+// conversions and two matrix instructions, 47 % of the issue slots and 28 % of the matrix pipe; over bf16 pages with fp32 queries 33 % and 20 %, with waits
+// for pages and tables, the ring's loads and the barrier at an item's end beside it (the three-term products are not what bounds it).
 #include "paged.cuh"
 #include "paged_tiles.h"
 
@@ -729,13 +730,15 @@ static bool paged_attn_ok(const IhbPagedAttn& a) {
 
 // Which kernel. The tiles of paged_tiles.cu cost the same from 1 to 128 rows ((token, head) pairs of a sequence) and some 13 us more to
 // start; here each 16 rows read the keys again. Measured, 32 / 4 heads, us here / there:
-//   32 sequences of 2048 keys  32 rows 40 / 63 (bf16 pages 52 / 57)   64: 69 / 66 (91 / 58)   128: 122 / 73 (166 / 64)
-//    8 sequences of 4096       32: 28 / 49 (34 / 42)                  64: 38 / 49 (50 / 43)   128:  61 / 51 ( 83 / 47)
-//    1 sequence of 8192        32: 19 / 48 (23 / 44)                  64: 21 / 48 (25 / 44)   128:  27 / 49 ( 33 / 46)
-//    4 sequences of 32768      32: 58 / 91 (81 / 81)                  64: 100 / 92 (143 / 81) 128: 182 / 94 (300 / 85)
+//   32 sequences of 2048 keys  32 rows 40 / 54 (bf16 pages 52 / 64)   64: 68 / 55 (89 / 65)   128: 121 / 58 (165 / 66)
+//    8 sequences of 4096       32: 27 / 45 (33 / 47)                  64: 38 / 41 (49 / 49)   128:  61 / 43 ( 81 / 52)
+//    1 sequence of 8192        32: 19 / 47 (21 / 45)                  64: 20 / 48 (23 / 46)   128:  26 / 50 ( 31 / 47)
+//    4 sequences of 32768      32: 58 / 82 (101 / 104)                64: 99 / 84 (144 / 106) 128: 182 / 87 (291 / 108)
 // so up to 32 rows they stay here, above 128 they go there, and between it is where the lines cross: with t sixteens of rows and W keys
-// of all heads, 50 t W us a million here (bf16 pages 80), 180 W + 10 there. The lengths are on the device: W comes from the table's width,
-// and a table much wider than its sequences gets the tiles earlier than it need. fp32 queries always stay: their precision has no tile form.
+// of all heads, 50 t W us a million here (bf16 pages 80), 180 W + 10 there (fitted to earlier times of the tiles: they are 5 to 15 % faster now over
+// e4m3 pages, some windows are on the slower side of it). The lengths are on the device: W comes from the table's width,
+// and a table much wider than its sequences gets the tiles earlier than it need: that costs time, not bits (over bf16 pages both keep two terms of P, over
+// e4m3 pages P is fp16 in both). fp32 queries always stay: their precision has no tile form.
 static bool use_tiles(const IhbPagedAttn& a) {
   const long long rows = static_cast<long long>(a.max_q) * (a.nq / a.c.nkv);
   if (!a.q_bf16 || rows <= 32) return false;

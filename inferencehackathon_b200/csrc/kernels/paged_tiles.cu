@@ -7,7 +7,8 @@
 //                    probabilities (16 bits) back into tensor memory in the place of the scores
 //   warps 8-11       bring V: page lookups, 16-byte asynchronous copies, e4m3 -> fp16 on the way into the swizzled tile
 //   warps 14, 15     bring K, and the page scales. e4m3 K needs no conversion: a bf16 query row, scaled by a power of two, is the sum of two
-//                    e4m3 rows (8 significant bits: 4 + 4), so S = Qhi K^T + Qlo K^T runs on e4m3 products, which are twice as fast
+//                    e4m3 rows (8 significant bits: 4 + 4), so S = Qhi K^T + Qlo K^T runs on e4m3 products, which are twice as fast. What lies below
+//                    2^-17 of a row's largest element is lost: 2^-8 of what that element's own rounding to bf16 was, and far below P's fp16
 //   warps 12, 13     one issuer per tile (waits, fences and commits cost it more than the products' issue): S = Q K^T (both operands
 //                    in shared memory) and O += P V (P in tensor memory, V as an MN-major operand: the rows of the cache are used as
 //                    they lie, no transpose)
@@ -21,7 +22,7 @@
 // key ranges, and cut into one equal range per SM; pieces of a cut item are folded by a second kernel.
 //
 // Bound by the groups' latency: a half block is 512 cycles of the exponential unit per warp, two warps share the unit, and a half takes 2050
-// cycles with loads from tensor memory, conversion, vote, store and hand-over. The tensor pipe is busy half of the time. Per segment
+// cycles with loads from tensor memory, conversion, vote, store and hand-over. The tensor pipe is busy 40 % of the time. Per segment
 // 5 us of set-up and result, most of what a batch of short windows costs.
 #include "paged.cuh"
 #include "paged_tiles.h"
@@ -631,7 +632,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             }
             pt_wait_st();
           }
-          for (int turn = 0;; ++turn) {        // (a third turn would only come from scores beyond fp32's whole numbers)
+          for (int turn = 0;; ++turn) {        // (a third turn would only come from scores beyond fp32's whole numbers, 2^24)
             float v[64];                       // (nothing but waits may stand between the loads and theirs: the registers fill behind the compiler's back)
             __syncwarp();
             pt_ld32_issue(t_s + hf * 64, v);
