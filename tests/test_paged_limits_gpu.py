@@ -393,15 +393,12 @@ def _near_ties(T, nkv, norm, io, gen, gamma, cos, sin, pos, edge, every):
     return y.to(_io(io))
 
 
-@pytest.mark.parametrize("norm", [False, True])
-@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("norm,edge", [(False, False), (False, True), (True, False)])       # (with a norm the largest value is the free one)
 @pytest.mark.parametrize("every", [False, True])
 @pytest.mark.parametrize("page,lens,news", [(16, [5, 40, 3], [5, 17, 3]), (128, [200, 7, 300], [200, 7, 131]), (64, [1, 64, 65, 130, 20], [1, 1, 1, 1, 1]),
                                             (32, [700], [700])])
 def test_bytes_next_to_ties_are_those_of_64_bits(norm, edge, every, page, lens, news):
     """Every byte and scale of e4m3 pages equals the 64-bit ones, with and without gammas, odd row counts, rotation angles of their own."""
-    if edge and norm:
-        pytest.skip("with a norm the largest value is the free one")
     gen = torch.Generator().manual_seed(page + norm)
     nq, nkv, T = 2, 2, sum(news)
     ang = torch.rand(2000, 64, generator=gen, dtype=F64) * 0.9 + 0.35          # no angle near a multiple of a quarter turn
@@ -541,3 +538,51 @@ def test_pages_beyond_32_bits(n):
     out = paged.paged_attention(q, k, v, td, ld, cu_q=cu, max_q=n)
     want, _, mag = _reference(got_k, got_v, None, None, q.cpu(), here, lens, news, nkv)
     _check(out, want, mag, _p_step("bf16", "bf16", n * 4 > 128) + 2.0 ** -17, "bf16")
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("n", [1, 40])
+def test_two_captured_steps_replayed_at_once(cache, n):
+    """Append and attention of two batches, captured apart, replayed on two streams at the same time, then with other lengths in the same
+    tensors: what eager calls of each give."""
+    cos, sin = (t.to(DEV) for t in O.rope_tables(3000))
+    steps = []
+    for seed in (1, 2):
+        gen = torch.Generator().manual_seed(seed)
+        nq, nkv, page, B = 16, 2, 32, 5
+        lens, news = [n + r for r in (2000 * seed, 0, 31, 700, 90)], [n] * B
+        table, n_pages = O.tables(lens, page, gen)
+        k, v, ks, vs = O.random_pages(n_pages, nkv, page, cache, gen, spread=False)
+        qkv = torch.randn(B * n, (nq + 2 * nkv) * 128, generator=gen).to(torch.bfloat16)
+        k, v, ks, vs, table, qkv, cu = [None if t is None else t.to(DEV) for t in (k, v, ks, vs, table, qkv, O.cu_of(news))]
+        lens = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        q = torch.empty(B * n, nq, 128, dtype=torch.bfloat16, device=DEV)
+        out = torch.empty_like(q)
+
+        def step(k=k, v=v, ks=ks, vs=vs, table=table, qkv=qkv, cu=cu, lens=lens, q=q, out=out):
+            paged.paged_append(qkv, 16, 2, k, v, table, lens, cos, sin, cu_q=cu, k_scale=ks, v_scale=vs, q_out=q)
+            paged.paged_attention(q, k, v, table, lens, cu_q=cu, max_q=n, k_scale=ks, v_scale=vs, out=out)
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        steps.append((step, graph, out, lens))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for change in (False, True):
+        want = []
+        for step, _, out, lens in steps:
+            if change:
+                lens.copy_(torch.tensor([n + 5, n, n + 64, n + 1, n + 33], dtype=torch.int32))
+            step()
+            want.append(out.clone())
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for s, (_, graph, out, _) in zip(streams, steps):
+                with torch.cuda.stream(s):
+                    out.zero_()
+                    graph.replay()
+            torch.cuda.synchronize()
+            for w, (_, _, out, _) in zip(want, steps):
+                assert torch.equal(out, w)
