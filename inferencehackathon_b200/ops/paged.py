@@ -205,7 +205,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``q``'s type; tokens behind ``cu_q[B]`` are left as they are, so a new tensor holds nothing there). ``lse [T, nq]`` fp32 receives
     the natural log of each softmax denominator, for merging with attention over other rows.
 
-    Sums, maxima and denominators are fp32. What else is rounded, relative to the result: fp32 queries 2^-18 over both kinds of pages;
+    Sums, maxima and denominators are fp32. What else is rounded, relative to the result: fp32 queries 2^-20 over both kinds of pages;
     bf16 queries over e4m3 pages 2^-11 (probabilities in fp16; in windows of more than 32 rows, tokens x query heads of a KV head, what
     lies below 2^-17 of a query's largest element is lost too); over bf16 pages 2^-16, and 2^-8 where ``out`` is bf16 and a window has
     more than 128 rows. Infinities in a value row that every token sees come out as infinity or NaN. Scales of e4m3 pages are taken

@@ -586,3 +586,26 @@ def test_two_captured_steps_replayed_at_once(cache, n):
             torch.cuda.synchronize()
             for w, (_, _, out, _) in zip(want, steps):
                 assert torch.equal(out, w)
+
+
+@pytest.mark.parametrize("cache", ["fp8", "bf16"])
+@pytest.mark.parametrize("B,n,nq,L", [(200, 1, 4, 16000), (100, 1, 16, 16000), (12, 40, 8, 9000)])
+def test_fp32_results_keep_their_bits_over_many_keys(cache, B, n, nq, L):
+    """fp32 queries, every warp adding hundreds of steps up (the sequences share their pages): the norm of the error stays below 2^-20 of the result's.
+    (Independent roundings: exponents of up to 16 give 2^-21 per probability, P and q in pairs 2^-22, sums with rounded additions 2^-24 sqrt(hundreds);
+    additions that cut off would give 2^-25 times hundreds.)"""
+    gen = torch.Generator().manual_seed(L)
+    page = 128
+    table, n_pages = O.tables([L], page, gen)
+    k, v, ks, vs = O.random_pages(n_pages, 1, page, cache, gen, spread=False)
+    q = torch.randn(B * n, nq, 128, generator=gen)
+    qd, kd, vd, td, ksd, vsd = [None if t is None else t.to(DEV) for t in (q, k, v, table, ks, vs)]
+    out = paged.paged_attention(qd, kd, vd, td.expand(B, -1), torch.full((B,), L, dtype=torch.int32, device=DEV), cu_q=O.cu_of([n] * B).to(DEV), max_q=n,
+                                k_scale=ksd, v_scale=vsd)
+    ids = td[0].long()
+    kk = (kd[ids, 0].to(F64) * (1.0 if ksd is None else ksd[ids, 0].to(F64)[:, None, None])).reshape(-1, 128)[:L]
+    vv = (vd[ids, 0].to(F64) * (1.0 if vsd is None else vsd[ids, 0].to(F64)[:, None, None])).reshape(-1, 128)[:L]
+    w = qd.to(F64).flatten(0, 1) @ kk.T * 128 ** -0.5
+    see = torch.arange(L, device=DEV)[None, :] <= L - n + torch.arange(n, device=DEV).repeat(B).repeat_interleave(nq)[:, None]
+    ref = (torch.softmax(w.masked_fill(~see, -math.inf), 1) @ vv).view(B * n, nq, 128)
+    assert float((out.to(F64) - ref).norm() / ref.norm()) <= 2.0 ** -20
