@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(PD_WARPS * 32, PdSmem<NT, KV8, QT>::PER_SM) pa
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               // fp32 queries: the matrix unit cuts its sums off, always towards zero, and over thousands of keys that adds up (110 K keys: 2.2e-6 of the
-              // result, 4e-7 with a sum of each step's own and rounded additions; up to 5 % of the time)
+              // result, 4.8e-7 with a sum of each step's own and rounded additions; up to 5 % of the time)
               if constexpr (QT > 1) {
                 float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
