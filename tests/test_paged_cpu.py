@@ -238,3 +238,21 @@ def test_ragged_calls_name_their_longest_window():
     for bound in (1, 3):
         with pytest.raises(ValueError, match="CUDA tensors"):            # all that it lacks
             paged.paged_attention(**a, max_q=bound)
+
+
+def test_c_entry_refuses_masks_without_columns():
+    lib = K.load()
+    c = K.IhbPaged(k=16, v=16, n_pages=4, nkv=1, page=16, B=1, T=1, max_blocks=1, block_table=16, kv_len=16)
+    for stride, cols in ((-1, 4), (4, 0), (0, -3)):
+        b = K.IhbPagedAttn(c=c, q=16, nq=1, out=16, max_q=1, scratch=16, q_stride_t=8, q_stride_h=8, mask=16, mask_stride=stride, mask_cols=cols)
+        assert lib.ihb_paged_attention(C.byref(b), None) != 0
+
+
+def test_mask_views_pass_the_checks():
+    """Shared, overlapping and sliced rows are masks like any other (what is left to refuse is the missing GPU)."""
+    flat, wide = torch.ones(8, dtype=torch.bool), torch.ones(3, 9, dtype=torch.uint8)
+    for mask in (flat.unfold(0, 3, 1)[:3], flat[:4].expand(3, -1), wide[:, 2:6], torch.ones(3, 1, dtype=torch.bool)):
+        with pytest.raises(ValueError, match="CUDA tensors"):
+            paged.paged_attention(**_attn_args(mask=mask))
+    with pytest.raises(ValueError, match="contiguous rows"):
+        paged.paged_attention(**_attn_args(mask=wide[:, ::2]))
