@@ -1256,8 +1256,8 @@ static cudaError_t pt_launch(const IhbPagedAttn& a, cudaStream_t stream) {
 cudaError_t paged_tiles_launch(const IhbPagedAttn& a, cudaStream_t stream) {
   // Up to 128 rows the width of the block table chooses between this kernel and paged_attn.cu (use_tiles): both keep two terms of P over bf16 pages, so
   // that a wider table does not change the precision. Above, where every call comes here, a bf16 result takes one: that adds at most one more half
-  // step of bf16 to the result's own (1.8e-3 from 64 bits against 1.5e-3), and the second product costs a sixth (prompt of 4096 tokens: 200 us,
-  // 233 with two). An fp32 result always gets two.
+  // step of bf16 to the result's own (random inputs: 2.3e-3 from 64 bits against 1.65e-3), and the second product costs a sixth (prompt of 4096 tokens:
+  // 200 us, 233 with two). An fp32 result always gets two.
   if (a.c.k_scale != nullptr) return pt_launch<true, false>(a, stream);
   const bool one = a.out_bf16 && static_cast<long long>(a.max_q) * (a.nq / a.c.nkv) > PT_M;
   return one ? pt_launch<false, false>(a, stream) : pt_launch<false, true>(a, stream);
